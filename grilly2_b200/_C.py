@@ -67,6 +67,15 @@ class _Storage:
         self.handle, self.bytes, self.parent = out.value, int(nbytes), parent
         return self
 
+    @classmethod
+    def wrap(cls, ptr: int, nbytes: int) -> "_Storage":
+        """A handle onto device memory the caller owns and keeps alive (gq_buffer_wrap)."""
+        out = ctypes.c_uint64()
+        check(_l().gq_buffer_wrap(context(), ctypes.c_void_p(ptr), int(nbytes), ctypes.byref(out)))
+        self = object.__new__(cls)
+        self.handle, self.bytes, self.parent = out.value, int(nbytes), None
+        return self
+
     def __del__(self) -> None:
         try:
             if self.handle and _ctx is not None:
@@ -105,6 +114,16 @@ class Tensor:
         if a.size:
             check(_l().gq_upload(context(), t.storage.handle, 0, a.ctypes.data_as(ctypes.c_void_p), a.nbytes))
         return t
+
+    @staticmethod
+    def from_pointer(ptr: int, shape, dtype: str = F32) -> "Tensor":
+        """A tensor over device memory that another library owns (its data pointer): no copy, and the caller keeps the
+        memory alive as long as the tensor, or a graph that was captured with it. This backend's work runs on a stream of
+        its own: what wrote the memory must have finished (or be on that stream) before the next call reads it."""
+        if dtype not in _NP:
+            raise NotImplementedError(f"grilly: dtype {dtype} is not implemented yet (this backend has float32 and int32)")
+        shape = tuple(int(s) for s in shape)
+        return Tensor(_Storage.wrap(ptr, 4 * (int(np.prod(shape, dtype=np.int64)) if shape else 1)), shape, dtype)
 
     def numel(self) -> int:
         return int(np.prod(self.shape, dtype=np.int64)) if self.shape else 1

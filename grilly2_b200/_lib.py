@@ -47,6 +47,15 @@ class DecodeDesc(ctypes.Structure):
                 [("layer", P(DecodeLayer))])
 
 
+class PagedCache(ctypes.Structure):
+    _fields_ = [(n, u64) for n in ("layers", "blocks", "block_size", "kv_heads", "dim", "seqs", "max_blocks", "k", "v", "kscale", "vscale",
+                                   "table", "lens")]
+
+
+class PagedStep(ctypes.Structure):
+    _fields_ = [(n, u64) for n in ("max_tokens", "starts", "slots", "positions", "runs", "last", "info")]
+
+
 # name -> argument types; every function but the three noted returns int32 status
 PROTOTYPES = {
     "gq_create": [i32, P(vp)],
@@ -100,6 +109,12 @@ PROTOTYPES = {
     "gq_decode_plan_create": [vp, P(DecodeDesc), P(vp)],
     "gq_decode_plan_step": [vp, vp, u64, u64, u64],
     "gq_sample": [vp, u64, u64, u64, u64, u64, u64, u32, u32, ctypes.c_double, u64, ctypes.c_double, ctypes.c_double, u64, u64, u64, u64, u64, u64],
+    "gq_paged_plan": [vp, P(PagedCache), u64, u64, u64, P(PagedStep)],
+    "gq_paged_advance": [vp, P(PagedCache), P(PagedStep)],
+    "gq_paged_release": [vp, P(PagedCache), u64, u64, u64],
+    "gq_paged_append": [vp, P(PagedCache), u64, u64, u64, u64, u64, u64, P(PagedStep), u64],
+    "gq_paged_attn": [vp, P(PagedCache), u64, u64, u64, ctypes.c_float, P(PagedStep), u64, u64],
+    "gq_sample_rows": [vp, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64],
     "gq_comm_unique_id": [vp, u64],
     "gq_comm_create": [vp, i32, i32, vp, P(vp)],
     "gq_all_gather_columns": [vp, vp, u64, u64, u64, u64],

@@ -276,6 +276,19 @@ uint64_t sample_state_bytes();
 void launch_sample(cudaStream_t s, const float* logits, uint64_t rows, uint64_t v, int32_t* history, uint64_t hist_cap, uint32_t* hist_len,
                    bool do_sample, float temperature, uint64_t top_k, float one_minus_p, float penalty, const float* uniforms,
                    uint64_t uniform_rows, uint32_t* draws, float* scores, float* ex, int32_t* tokens, float* probs, bool append, void* state);
+void launch_sample_rows(cudaStream_t s, const float* logits, uint32_t rows, uint32_t vocab, const float* temperature, const int32_t* top_k,
+                        const float* top_p, const float* min_p, const float* uniforms, uint32_t uniform_rows, uint32_t* draws, int32_t* tokens, float* probs,
+                        uint32_t* ticket);
+
+// the paged int8 KV cache (paged.cu, paged_attn.cu)
+struct PagedView;
+struct StepView;
+void launch_paged_plan(cudaStream_t s, const PagedView& c, const StepView& st, const int32_t* counts, const int32_t* free_list, int32_t* free_count);
+void launch_paged_advance(cudaStream_t s, const PagedView& c, const StepView& st);
+void launch_paged_release(cudaStream_t s, const PagedView& c, const int32_t* which, int32_t* free_list, int32_t* free_count);
+void launch_paged_append(cudaStream_t s, const PagedView& c, const StepView& st, const float* qkv, uint32_t heads, const float* cosv, const float* sinv,
+                         uint32_t max_pos, float* q_out);
+void launch_paged_attn(cudaStream_t s, const PagedView& c, const StepView& st, const float* q, uint32_t heads, float scale, float* out);
 uint64_t argmax_state_bytes();
 void launch_argmax_rows(cudaStream_t s, const float* v, uint64_t rows, uint64_t n, int32_t* out, void* state);
 

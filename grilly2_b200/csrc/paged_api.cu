@@ -1,0 +1,171 @@
+// C ABI of the paged int8 KV cache and of sampling by rows (include/gq.h): argument checks against buffer sizes, then the
+// launchers of paged.cu, paged_attn.cu and sample_rows.cu.
+#include "gq_internal.h"
+#include "paged.cuh"
+
+using namespace gq;
+
+namespace {
+
+using ull = unsigned long long;
+
+// The geometry of a cache, refused where a kernel's index could leave its buffer or 32 bits.
+PagedView cache_view(gq_ctx* ctx, const char* op, const gq_paged_cache* c, uint64_t layer, bool pool) {
+    if (!c) fail("%s: null cache", op);
+    if (c->block_size != 16 && c->block_size != 32 && c->block_size != 64 && c->block_size != 128)
+        fail("%s: block_size must be 16, 32, 64 or 128, got %llu", op, (ull)c->block_size);
+    if (c->seqs == 0 || c->seqs > kPagedMaxSeqs) fail("%s: 1 to %u requests, got %llu", op, kPagedMaxSeqs, (ull)c->seqs);
+    if (c->blocks == 0 || c->max_blocks == 0) fail("%s: a cache of no blocks", op);
+    check_dims(op, c->blocks, c->max_blocks, c->layers);
+    if (c->blocks * c->block_size > 0x7fffffffull || c->seqs * c->max_blocks > 0x7fffffffull || c->max_blocks * c->block_size > 0x7fffffffull)
+        fail("%s: the pool and the tables must stay below 2^31 tokens and entries", op);
+    PagedView v;
+    v.blocks = (uint32_t)c->blocks, v.block = (uint32_t)c->block_size, v.seqs = (uint32_t)c->seqs, v.max_blocks = (uint32_t)c->max_blocks;
+    while ((1u << v.shift) < v.block) ++v.shift;
+    v.table = (int32_t*)view(ctx, c->table, 0, c->seqs * c->max_blocks, 4, "the block table");
+    v.lens = (int32_t*)view(ctx, c->lens, 0, c->seqs, 4, "the cached lengths");
+    if (!pool) return v;
+    if (c->kv_heads == 0 || c->kv_heads > 4096) fail("%s: 1 to 4096 KV heads, got %llu", op, (ull)c->kv_heads);
+    if (c->dim != 32 && c->dim != 64 && c->dim != 128) fail("%s: head_dim must be 32, 64 or 128, got %llu", op, (ull)c->dim);
+    if (layer >= c->layers) fail("%s: layer %llu of %llu", op, (ull)layer, (ull)c->layers);
+    v.kv_heads = (uint32_t)c->kv_heads, v.dim = (uint32_t)c->dim;
+    const uint64_t scales = c->blocks * c->kv_heads, codes = scales * c->block_size * c->dim;  // < 2^31 * 2^12 * 2^7
+    v.k = (int8_t*)view(ctx, c->k, layer * codes, codes, 1, "the key pool");
+    v.v = (int8_t*)view(ctx, c->v, layer * codes, codes, 1, "the value pool");
+    v.kscale = (float*)view(ctx, c->kscale, layer * scales, scales, 4, "the key scales");
+    v.vscale = (float*)view(ctx, c->vscale, layer * scales, scales, 4, "the value scales");
+    if (((uintptr_t)v.k | (uintptr_t)v.v) & 15) fail("%s: the pool must lie on 16-byte boundaries", op);
+    return v;
+}
+
+StepView step_view(gq_ctx* ctx, const char* op, const gq_paged_cache* c, const gq_paged_step* st) {
+    if (!st) fail("%s: null step", op);
+    check_dims(op, st->max_tokens, 1);
+    if (st->max_tokens == 0) fail("%s: a step of no rows", op);
+    StepView v;
+    v.tokens = (uint32_t)st->max_tokens, v.runs_cap = (uint32_t)GQ_PAGED_RUNS(st->max_tokens, c->block_size, c->seqs);
+    v.starts = (int32_t*)view(ctx, st->starts, 0, c->seqs + 1, 4, "the step's starts");
+    v.slots = (int32_t*)view(ctx, st->slots, 0, st->max_tokens, 4, "the step's slots");
+    v.positions = (int32_t*)view(ctx, st->positions, 0, st->max_tokens, 4, "the step's positions");
+    v.runs = (int32_t*)view(ctx, st->runs, 0, (uint64_t)v.runs_cap + 1, 4, "the step's runs");
+    v.last = (int32_t*)view(ctx, st->last, 0, c->seqs, 4, "the step's last rows");
+    v.info = (int32_t*)view(ctx, st->info, 0, 2, 4, "the step's info");
+    return v;
+}
+
+void check_aligned(const char* op, std::initializer_list<const void*> ptrs) {
+    for (const void* p : ptrs)
+        if ((uintptr_t)p & 15) fail("%s: buffers must lie on 16-byte boundaries", op);
+}
+
+uint64_t check_heads(const char* op, const PagedView& c, uint64_t heads) {
+    if (heads == 0 || heads > 65536 || heads % c.kv_heads)
+        fail("%s: %llu heads do not group over %u kv heads", op, (ull)heads, c.kv_heads);
+    return heads * c.dim;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t gq_paged_plan(gq_ctx* ctx, const gq_paged_cache* cache, gq_buf counts, gq_buf free_list, gq_buf free_count, const gq_paged_step* step) {
+    return guarded([&] {
+        Locked l(ctx);
+        const PagedView c = cache_view(ctx, "gq_paged_plan", cache, 0, false);
+        const StepView st = step_view(ctx, "gq_paged_plan", cache, step);
+        auto np = (const int32_t*)view(ctx, counts, 0, c.seqs, 4, "gq_paged_plan counts");
+        auto fp = (const int32_t*)view(ctx, free_list, 0, c.blocks, 4, "gq_paged_plan free list");
+        auto fc = (int32_t*)view(ctx, free_count, 0, 1, 4, "gq_paged_plan free count");
+        launch_paged_plan(ctx->stream, c, st, np, fp, fc);
+        after_launch(ctx, "paged_plan", {cache->table, cache->lens, counts, free_list, free_count, step->starts, step->slots, step->positions, step->runs,
+                                         step->last, step->info});
+    });
+}
+
+int32_t gq_paged_advance(gq_ctx* ctx, const gq_paged_cache* cache, const gq_paged_step* step) {
+    return guarded([&] {
+        Locked l(ctx);
+        const PagedView c = cache_view(ctx, "gq_paged_advance", cache, 0, false);
+        const StepView st = step_view(ctx, "gq_paged_advance", cache, step);
+        launch_paged_advance(ctx->stream, c, st);
+        after_launch(ctx, "paged_advance", {cache->table, cache->lens, step->starts});
+    });
+}
+
+int32_t gq_paged_release(gq_ctx* ctx, const gq_paged_cache* cache, gq_buf which, gq_buf free_list, gq_buf free_count) {
+    return guarded([&] {
+        Locked l(ctx);
+        const PagedView c = cache_view(ctx, "gq_paged_release", cache, 0, false);
+        auto wp = (const int32_t*)view(ctx, which, 0, c.seqs, 4, "gq_paged_release requests");
+        auto fp = (int32_t*)view(ctx, free_list, 0, c.blocks, 4, "gq_paged_release free list");
+        auto fc = (int32_t*)view(ctx, free_count, 0, 1, 4, "gq_paged_release free count");
+        launch_paged_release(ctx->stream, c, wp, fp, fc);
+        after_launch(ctx, "paged_release", {cache->table, cache->lens, which, free_list, free_count});
+    });
+}
+
+int32_t gq_paged_append(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer, gq_buf qkv, uint64_t heads, gq_buf cos, gq_buf sin,
+                        uint64_t max_pos, const gq_paged_step* step, gq_buf q_out) {
+    return guarded([&] {
+        Locked l(ctx);
+        const char* op = "gq_paged_append";
+        const PagedView c = cache_view(ctx, op, cache, layer, true);
+        const StepView st = step_view(ctx, op, cache, step);
+        const uint64_t width = check_heads(op, c, heads), row = width + 2 * (uint64_t)c.kv_heads * c.dim;
+        check_dims(op, max_pos, row);
+        if (max_pos == 0) fail("%s: rotary tables of no positions", op);
+        auto qp = (const float*)view(ctx, qkv, 0, st.tokens * row, 4, "gq_paged_append qkv");
+        auto cp = (const float*)view(ctx, cos, 0, max_pos * c.dim, 4, "gq_paged_append cos");
+        auto sp = (const float*)view(ctx, sin, 0, max_pos * c.dim, 4, "gq_paged_append sin");
+        auto op_ = (float*)view(ctx, q_out, 0, st.tokens * width, 4, "gq_paged_append q output");
+        check_aligned(op, {qp, cp, sp, op_});
+        if (ranges_overlap(op_, st.tokens * width * 4, qp, st.tokens * row * 4)) fail("%s: the output must not overlap qkv", op);
+        launch_paged_append(ctx->stream, c, st, qp, (uint32_t)heads, cp, sp, (uint32_t)max_pos, op_);
+        after_launch(ctx, "paged_append", {cache->k, cache->v, cache->kscale, cache->vscale, cache->table, cache->lens, qkv, cos, sin, step->starts,
+                                           step->slots, step->positions, step->runs, q_out});
+    });
+}
+
+int32_t gq_paged_attn(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer, gq_buf q, uint64_t heads, float scale, const gq_paged_step* step,
+                      uint64_t max_count, gq_buf out) {
+    return guarded([&] {
+        Locked l(ctx);
+        const char* op = "gq_paged_attn";
+        const PagedView c = cache_view(ctx, op, cache, layer, true);
+        const StepView st = step_view(ctx, op, cache, step);
+        const uint64_t width = check_heads(op, c, heads);
+        check_dims(op, max_count, 1);
+        if (max_count == 0) fail("%s: max_count must be at least 1", op);
+        auto qp = (const float*)view(ctx, q, 0, st.tokens * width, 4, "gq_paged_attn q");
+        auto yp = (float*)view(ctx, out, 0, st.tokens * width, 4, "gq_paged_attn output");
+        check_aligned(op, {qp, yp});
+        if (ranges_overlap(yp, st.tokens * width * 4, qp, st.tokens * width * 4)) fail("%s: the output must not overlap q", op);
+        launch_paged_attn(ctx->stream, c, st, qp, (uint32_t)heads, scale, yp);
+        after_launch(ctx, "paged_attn", {cache->k, cache->v, cache->kscale, cache->vscale, cache->table, cache->lens, q, step->starts, out});
+    });
+}
+
+int32_t gq_sample_rows(gq_ctx* ctx, gq_buf logits, uint64_t l_off, uint64_t rows, uint64_t vocab, gq_buf temperature, gq_buf top_k, gq_buf top_p,
+                       gq_buf min_p, gq_buf uniforms, uint64_t uniform_rows, gq_buf draws, gq_buf tokens, gq_buf probs) {
+    return guarded([&] {
+        Locked l(ctx);
+        check_dims("gq_sample_rows", rows, vocab, uniform_rows);
+        if (uniform_rows == 0) fail("gq_sample_rows: sampling needs at least one row of uniform numbers");
+        if (vocab == 0) fail("gq_sample_rows: expected (batch, vocab) with vocab > 0");
+        auto lp = (const float*)view(ctx, logits, l_off, rows * vocab, 4, "gq_sample_rows logits");
+        auto tp = (const float*)view(ctx, temperature, 0, rows, 4, "gq_sample_rows temperature");
+        auto kp = (const int32_t*)view(ctx, top_k, 0, rows, 4, "gq_sample_rows top_k");
+        auto pp = (const float*)view(ctx, top_p, 0, rows, 4, "gq_sample_rows top_p");
+        auto mp = (const float*)view(ctx, min_p, 0, rows, 4, "gq_sample_rows min_p");
+        auto up = (const float*)view(ctx, uniforms, 0, uniform_rows * rows, 4, "gq_sample_rows uniforms");
+        auto dp = draws ? (uint32_t*)view(ctx, draws, 0, 1, 4, "gq_sample_rows draw counter") : nullptr;
+        auto op = (int32_t*)view(ctx, tokens, 0, rows, 4, "gq_sample_rows tokens");
+        auto rp = probs ? (float*)view(ctx, probs, 0, rows, 4, "gq_sample_rows probabilities") : nullptr;
+        if (rows == 0) return;
+        launch_sample_rows(ctx->stream, lp, (uint32_t)rows, (uint32_t)vocab, tp, kp, pp, mp, up, (uint32_t)uniform_rows, dp, op, rp,
+                           (uint32_t*)ctx->sample_state);
+        after_launch(ctx, "sample_rows", {logits, temperature, top_k, top_p, min_p, uniforms, draws, tokens, probs});
+    });
+}
+
+}  // extern "C"

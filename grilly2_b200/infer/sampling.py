@@ -20,7 +20,7 @@ import numpy as np
 from .. import _C, _lib
 from .._lib import check
 
-__all__ = ["Generator", "Sampler", "next_token", "probabilities"]
+__all__ = ["Generator", "Sampler", "next_token", "probabilities", "sample_rows"]
 
 
 class Generator:
@@ -116,3 +116,39 @@ def probabilities(logits: "_C.Tensor", history=None, *, temperature: float = 1.0
     _one_shot(logits, history, None, probs, do_sample=True, temperature=temperature, top_k=top_k, top_p=top_p,
               repetition_penalty=repetition_penalty)
     return probs
+
+
+def sample_rows(logits: "_C.Tensor", uniforms: "_C.Tensor", *, temperature: "_C.Tensor", top_k: "_C.Tensor", top_p: "_C.Tensor",
+                min_p: "_C.Tensor", draws: "_C.Tensor | None" = None, tokens: "_C.Tensor | None" = None,
+                probs: "_C.Tensor | None" = None) -> "_C.Tensor":
+    """Every row's next token with settings of its own, all on the device (gq_sample_rows): ``temperature``, ``top_p`` and
+    ``min_p`` float32 [rows], ``top_k`` int32 [rows]; temperature 0 is greedy, top_k 0, top_p 1 and min_p 0 are off. ``uniforms``:
+    float32 [rows], or with the int32 counter ``draws`` [n, rows], of which each call takes the next row.
+    Returns int32 [rows] (-1 where nothing can be drawn); ``probs`` float32 [rows] receives each token's share of what was
+    kept. No counterpart in the reference, whose sampler has one setting for all rows and no min_p."""
+    if not isinstance(logits, _C.Tensor) or len(logits.shape) != 2:
+        raise RuntimeError("expected logits as a (batch, vocab) tensor")
+    rows, vocab = logits.shape
+    tokens = tokens if tokens is not None else _C.Tensor.empty((rows,), "int32")
+
+    def handle(name, t, dtype):
+        _C._require(t, dtype, name)
+        if t.numel() != rows or t.offset:
+            raise RuntimeError(f"{name} must hold one value per row ({rows}) at offset 0, got {list(t.shape)} at {t.offset}")
+        return t.storage.handle
+
+    _C._require(logits, "float32", "logits")
+    _C._require(uniforms, "float32", "uniforms")
+    n = uniforms.numel() // rows if rows else 1
+    if uniforms.offset or n < 1 or uniforms.numel() != n * rows or (draws is None and n != 1):
+        raise RuntimeError(f"uniforms must hold one value per row ({rows}), or rows of them with a draw counter, got {list(uniforms.shape)}")
+    if draws is not None:
+        _C._require(draws, "int32", "draws")
+        if draws.numel() != 1 or draws.offset:
+            raise RuntimeError(f"draws must be one word at offset 0, got {list(draws.shape)}")
+    check(_lib.load().gq_sample_rows(
+        _C.context(), logits.storage.handle, logits.offset, rows, vocab, handle("temperature", temperature, "float32"),
+        handle("top_k", top_k, "int32"), handle("top_p", top_p, "float32"), handle("min_p", min_p, "float32"),
+        uniforms.storage.handle, n, draws.storage.handle if draws is not None else 0, handle("tokens", tokens, "int32"),
+        handle("probs", probs, "float32") if probs is not None else 0))
+    return tokens

@@ -388,6 +388,81 @@ void gq_decode_plan_destroy(gq_ctx* ctx, gq_decode_plan* plan);
 /* out[r] = index of the maximum of row r (int32; the first on ties) — g2-argreduce-rows.glsl:42-77. */
 int32_t gq_argmax_rows(gq_ctx* ctx, gq_buf v, uint64_t rows, uint64_t n, gq_buf out);
 
+/* ── a paged int8 KV cache for several requests at once ──────────────────
+ * No counterpart in the reference (its cache is contiguous, float32 and of batch 1, kv_cache.rs:1-33). Keys and values of
+ * `seqs` requests live in a pool of `blocks` blocks of block_size tokens; table[seqs][max_blocks] names each request's
+ * blocks in order (-1: none yet) and lens[seqs] says how many tokens are cached. Everything a step must know is read
+ * from device memory, so a captured step replays. The codes are int8 with ONE float32 scale per (layer, block, KV head)
+ * for the keys and one for the values; what is cached is code * scale. The layout is the one the tensor cores read, so a
+ * block goes from memory to the multiplication as it lies:
+ *   k       int8 [layers][blocks][kv_heads][block_size / 8][dim / 16][8][16]   (8 tokens x 16 components contiguous)
+ *   v       int8 [layers][blocks][kv_heads][dim / 8][block_size / 16][8][16]   (8 components x 16 tokens: transposed)
+ *   kscale, vscale  float32 [layers][blocks][kv_heads]
+ *   table   int32 [seqs][max_blocks];  lens  int32 [seqs]
+ * block_size 16, 32, 64 or 128; dim 32, 64 or 128; seqs at most 4096; blocks * block_size and seqs * max_blocks below
+ * 2^31; k and v on 16-byte boundaries. An entry of the table or the slot map outside the pool is treated as -1. */
+typedef struct gq_paged_cache {
+    uint64_t layers, blocks, block_size, kv_heads, dim, seqs, max_blocks;
+    gq_buf k, v, kscale, vscale, table, lens;
+} gq_paged_cache;
+/* What one step's new tokens are and where they go, made by gq_paged_plan once per step and read by every layer. The
+ * step has room for max_tokens rows; the rows of request b are starts[b] .. starts[b + 1] - 1, those behind
+ * starts[seqs] belong to nobody and are neither read nor written. All int32:
+ *   starts    [seqs + 1]    rows before request b
+ *   slots     [max_tokens]  block * block_size + offset of a row's token in the pool; -1 = no room, or no token
+ *   positions [max_tokens]  its position in its request (also its rotary position); -1 = no token
+ *   runs      [GQ_PAGED_RUNS(max_tokens, block_size, seqs) + 1]  the first row of each stretch of rows that share a block;
+ *             behind the last one starts[seqs]
+ *   last      [seqs]        the last row of request b, -1 where it has none
+ *   info      [2]           rows in use; blocks that were wanted when the free list was empty */
+typedef struct gq_paged_step {
+    uint64_t max_tokens;
+    gq_buf starts, slots, positions, runs, last, info;
+} gq_paged_step;
+#define GQ_PAGED_RUNS(max_tokens, block_size, seqs)                                                              \
+    ((uint64_t)(max_tokens) < (uint64_t)(max_tokens) / (block_size) + 2 * (uint64_t)(seqs)                       \
+         ? (uint64_t)(max_tokens)                                                                                \
+         : (uint64_t)(max_tokens) / (block_size) + 2 * (uint64_t)(seqs))
+/* The step's maps from the requests' lengths: counts[b] (int32, negative = 0) new tokens for request b, at positions
+ * lens[b] .. lens[b] + counts[b] - 1. Where these reach a table entry without a block one is taken off the free list (int32
+ * [blocks], of which the first *free_count are free; the last is taken first), in order of (b, entry). Rows beyond max_tokens
+ * are cut; tokens beyond max_blocks * block_size, or without a block because the list is empty, get slot -1. lens is not
+ * advanced (gq_paged_advance), so calling it again gives the same maps and takes no more blocks. */
+int32_t gq_paged_plan(gq_ctx* ctx, const gq_paged_cache* cache, gq_buf counts, gq_buf free_list, gq_buf free_count, const gq_paged_step* step);
+/* lens[b] += the step's rows of request b (at most max_blocks * block_size): once per step, behind the last layer. */
+int32_t gq_paged_advance(gq_ctx* ctx, const gq_paged_cache* cache, const gq_paged_step* step);
+/* For every b with which[b] != 0 (int32 [seqs]): its blocks go back on the free list in table order, its table entries become -1
+ * and lens[b] 0. A block that several requests name must not be released through more than one of them. */
+int32_t gq_paged_release(gq_ctx* ctx, const gq_paged_cache* cache, gq_buf which, gq_buf free_list, gq_buf free_count);
+/* The step's rows of fused q | k | v (float32 [max_tokens][(heads + 2 kv_heads) dim]) at one layer: rotary on q and k at
+ * the rows' positions (cos / sin [max_pos][dim], the last row beyond), q to q_out [max_tokens][heads dim], k and v into
+ * the pool. A block's scale is max|value| / 127 over the tokens it holds: where a new token raises it, the codes that
+ * are there already are rounded again, code' = rint(code * (old / new)), so a cached value is off by half a step of the
+ * scale of each time it was rounded. A block whose first token is written starts anew. rint(value / scale) with IEEE division;
+ * a non-finite value makes its block's scale non-finite and the block read as NaN. One writer per block: two requests of
+ * a step must not append to the same block. The dimensions and layers as gq_paged_cache says; 16-byte boundaries. */
+int32_t gq_paged_append(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer, gq_buf qkv, uint64_t heads, gq_buf cos, gq_buf sin,
+                        uint64_t max_pos, const gq_paged_step* step, gq_buf q_out);
+/* Causal grouped-query attention of the step's rows over the cache: row t of request b, at position p = lens[b] + t -
+ * starts[b], attends to positions 0 .. p. out[t] = softmax(scale q k^T) v. Positions whose block is missing are
+ * skipped; a row that is left with none gives zeros. q and out float32 [max_tokens][heads dim], not overlapping; rows behind
+ * starts[seqs] are left as they were. max_count is the largest counts[b] the caller expects (1 for a decode step): it chooses
+ * how the work is cut, never what is computed. */
+int32_t gq_paged_attn(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer, gq_buf q, uint64_t heads, float scale, const gq_paged_step* step,
+                      uint64_t max_count, gq_buf out);
+/* The next token of every row, each row with settings of its own (float32 or int32 [rows], on the device, so that a captured
+ * step follows them): x = logits of the row (NaN counts as -inf), weights w = exp((x - max x) / temperature), then
+ *   top_k   (int32; <= 0 or >= vocab: off) keeps the k largest, ties with the k-th stay;
+ *   top_p   (>= 1: off) keeps a token while the weight of the kept tokens strictly above it is less than top_p of theirs all;
+ *   min_p   (<= 0: off) keeps w >= min_p;
+ * the largest always stays. The draw is the inverse CDF in token order with u in [0, 1): the first kept token whose cumulative
+ * weight exceeds u * total. u is uniforms[*draws % uniform_rows][row] (uniform_rows x rows floats), and the uint32 word
+ * `draws` is advanced by one, so that a captured step takes the next numbers at each replay; draws == 0: the first row. temperature <= 0 takes the first largest. tokens: int32 per row, -1
+ * where every logit is -inf; probs (0 = none) receives the token's share of what was kept. Sums and weights in 64 bits.
+ * Replaces nothing of the reference: its sampler has one setting for all rows and no min_p (gq_sample). */
+int32_t gq_sample_rows(gq_ctx* ctx, gq_buf logits, uint64_t l_off, uint64_t rows, uint64_t vocab, gq_buf temperature, gq_buf top_k, gq_buf top_p,
+                       gq_buf min_p, gq_buf uniforms, uint64_t uniform_rows, gq_buf draws, gq_buf tokens, gq_buf probs);
+
 /* ── multi-GPU: column-sharded linears over the GPUs of one box ──────────
  * No counterpart in the reference, which runs on a single device. One process
  * (and one context) per GPU. Rank r owns output features [r n/W, (r+1) n/W):
