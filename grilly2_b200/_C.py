@@ -9,6 +9,7 @@ is a call into the C ABI of include/gq.h.
 from __future__ import annotations
 
 import ctypes
+import math
 import threading
 
 import numpy as np
@@ -126,7 +127,7 @@ class Tensor:
         return Tensor(_Storage.wrap(ptr, 4 * (int(np.prod(shape, dtype=np.int64)) if shape else 1)), shape, dtype)
 
     def numel(self) -> int:
-        return int(np.prod(self.shape, dtype=np.int64)) if self.shape else 1
+        return math.prod(self.shape)
 
     def numpy(self) -> np.ndarray:
         out = np.empty(self.shape, dtype=_NP[self.dtype])

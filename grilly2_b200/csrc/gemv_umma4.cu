@@ -198,13 +198,6 @@ __global__ void __launch_bounds__(128) x_digits_kernel(const float* __restrict__
     if (r == rows - 1 && l < 16 - rows) xsinv[rows + l] = make_float2(0.0f, 0.0f);
 }
 
-// Shared-memory matrix descriptor for a K-major operand of 32 bytes of K in unswizzled core-matrix order: a core matrix is
-// 8 rows x 16 bytes stored contiguously (128 bytes); the two core matrices of a row block lie `lbo` bytes apart, row
-// blocks `sbo` bytes apart.
-__device__ __forceinline__ uint64_t umma_desc_plain(uint32_t smem_addr, uint32_t lbo, uint32_t sbo) {
-    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | ((uint64_t)1 << 46);
-}
-
 // 16 lanes x 256 bits, eight times along the columns: register 4 i + {0, 1} = lane (t / 4), columns 8 i + 2 (t % 4) + {0, 1};
 // register 4 i + {2, 3} = lane (t / 4) + 8, same columns (t = the thread's index in the warp). No memory clobber: the compiler
 // may move shared-memory loads across it; what orders the registers' uses is tmem_wait_ld_of.

@@ -188,6 +188,8 @@ int32_t gq_create(int32_t device, gq_ctx** out) {
             GQ_CUDA(cudaMemset(ctx->argmax_state, 0, argmax_state_bytes()));
             GQ_CUDA(cudaMalloc(&ctx->sample_state, sample_state_bytes()));
             GQ_CUDA(cudaMemset(ctx->sample_state, 0, sample_state_bytes()));
+            GQ_CUDA(cudaMalloc(&ctx->paged_state, paged_attn_state_bytes()));
+            GQ_CUDA(cudaMemset(ctx->paged_state, 0, paged_attn_state_bytes()));
             const char* lb = getenv("GQ_LAUNCH_BLOCKING");
             ctx->launch_blocking = lb && lb[0] == '1';
         } catch (...) {
@@ -212,6 +214,7 @@ void gq_destroy(gq_ctx* ctx) {
             for (auto& kv : ctx->pool) cudaFree(kv.second);
             if (ctx->argmax_state) cudaFree(ctx->argmax_state);
             if (ctx->sample_state) cudaFree(ctx->sample_state);
+            if (ctx->paged_state) cudaFree(ctx->paged_state);
             if (ctx->scratch) cudaFree(ctx->scratch);
             for (void* p : ctx->retired_scratch) cudaFree(p);
             if (ctx->status_host) cudaFreeHost(ctx->status_host);

@@ -80,6 +80,7 @@ struct gq_ctx {
     gq_buf prev_written[4] = {0, 0, 0, 0};
     void* argmax_state = nullptr;  // keys and counters of gq_argmax_rows, zero between calls
     void* sample_state = nullptr;  // gq_sample's arrival ticket, zero between calls
+    void* paged_state = nullptr;   // arrival counters of gq_paged_attn, zero between calls
     // How long a kernel waits for another GPU's data before it gives up and reports through the status word, in SM
     // clock cycles (gq_set_wait_limit_us).
     long long peer_wait_cycles = 4000000000ll;
@@ -288,7 +289,10 @@ void launch_paged_advance(cudaStream_t s, const PagedView& c, const StepView& st
 void launch_paged_release(cudaStream_t s, const PagedView& c, const int32_t* which, int32_t* free_list, int32_t* free_count);
 void launch_paged_append(cudaStream_t s, const PagedView& c, const StepView& st, const float* qkv, uint32_t heads, const float* cosv, const float* sinv,
                          uint32_t max_pos, float* q_out);
-void launch_paged_attn(cudaStream_t s, const PagedView& c, const StepView& st, const float* q, uint32_t heads, float scale, float* out);
+uint64_t paged_attn_state_bytes();
+uint64_t paged_attn_scratch_bytes(uint32_t dim, int sm_count);
+void launch_paged_attn(cudaStream_t s, int sm_count, uint32_t* status, const PagedView& c, const StepView& st, const float* q, uint32_t heads, float scale,
+                       uint64_t max_count, float* out, void* state, void* scratch);
 uint64_t argmax_state_bytes();
 void launch_argmax_rows(cudaStream_t s, const float* v, uint64_t rows, uint64_t n, int32_t* out, void* state);
 

@@ -262,10 +262,12 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedView 
     if (tid == 0) *scale_at = scale;
     uint32_t* pool = reinterpret_cast<uint32_t*>((is_v ? c.v : c.k) + ((size_t)block * c.kv_heads + head) * c.block * dim);
     if (!is_v) {
-        if (grows)  // the tokens that are there already, a word = four components of one token
-            for (uint32_t i = tid; i < off0 * 2 * quads; i += kAppendThreads) {
-                uint32_t* w = pool + key_at(dim, i / (2 * quads), (i % (2 * quads)) * 4) / 4;
-                const uint32_t was = *w;
+        if (grows)  // the block's other tokens, a word = four components of one token
+            for (uint32_t i = tid; i < (c.block - n) * 2 * quads; i += kAppendThreads) {
+                uint32_t t = i / (2 * quads);
+                t += t < off0 ? 0 : n;
+                uint32_t* w = pool + key_at(dim, t, (i % (2 * quads)) * 4) / 4;
+                const uint32_t was = off0 ? *w : 0u;  // a block that starts anew starts as zeros
                 *w = recode(was, 0, ratio) | recode(was, 1, ratio) << 8 | recode(was, 2, ratio) << 16 | recode(was, 3, ratio) << 24;
             }
         for (uint32_t i = tid; i < n * quads; i += kAppendThreads) {
@@ -277,17 +279,17 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedView 
                 code_of(hi.x, scale) | code_of(hi.y, scale) << 8 | code_of(hi.z, scale) << 16 | code_of(hi.w, scale) << 24;
         }
     } else {
-        // a word = four tokens of one component: the first may hold tokens of both kinds
-        const uint32_t w0 = grows ? 0 : off0 >> 2, w1 = (off0 + n + 3) >> 2;
+        // a word = four tokens of one component: the run's first and last may hold others too
+        const uint32_t w0 = grows ? 0 : off0 >> 2, w1 = grows ? c.block >> 2 : (off0 + n + 3) >> 2;
         for (uint32_t i = tid; i < (w1 - w0) * dim; i += kAppendThreads) {
             const uint32_t d = i % dim, t = (w0 + i / dim) * 4;
             uint32_t* at = pool + value_at(c.block, t, d) / 4;
-            uint32_t word = (t < off0 || t + 4 > off0 + n) ? *at : 0u;
+            uint32_t word = (t < off0 || t + 4 > off0 + n) && (off0 || !grows) ? *at : 0u;
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) {
                 uint32_t code = word >> (8 * j) & 0xffu;
-                if (t + j < off0) code = grows ? recode(word, j, ratio) : code;
-                else if (t + j < off0 + n) code = code_of(src[(size_t)(t + j - off0) * pitch + d], scale);
+                if (t + j >= off0 && t + j < off0 + n) code = code_of(src[(size_t)(t + j - off0) * pitch + d], scale);
+                else if (grows) code = recode(word, j, ratio);
                 word = (word & ~(0xffu << (8 * j))) | code << (8 * j);
             }
             *at = word;
@@ -301,7 +303,7 @@ void launch_paged_plan(cudaStream_t s, const PagedView& c, const StepView& st, c
     // One CTA fills 8192 rows of the maps in the time that the cluster's barrier takes.
     const uint32_t ctas = st.tokens > 8192 ? kPlanCluster : 1;
     const size_t smem = (size_t)(3 * c.seqs + 2) * 4;
-    if (smem > 48 * 1024) GQ_CUDA(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (smem + 256 > 48 * 1024) GQ_CUDA(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(kPlanThreads), cfg.dynamicSmemBytes = smem, cfg.stream = s;
     cudaLaunchAttribute attr[2]{};

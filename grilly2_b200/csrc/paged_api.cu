@@ -140,7 +140,9 @@ int32_t gq_paged_attn(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer, 
         auto yp = (float*)view(ctx, out, 0, st.tokens * width, 4, "gq_paged_attn output");
         check_aligned(op, {qp, yp});
         if (ranges_overlap(yp, st.tokens * width * 4, qp, st.tokens * width * 4)) fail("%s: the output must not overlap q", op);
-        launch_paged_attn(ctx->stream, c, st, qp, (uint32_t)heads, scale, yp);
+        const int sms = ctx->prop.multiProcessorCount;
+        void* scratch = context_scratch(ctx, paged_attn_scratch_bytes(c.dim, sms));
+        launch_paged_attn(ctx->stream, sms, ctx->status_dev, c, st, qp, (uint32_t)heads, scale, max_count, yp, ctx->paged_state, scratch);
         after_launch(ctx, "paged_attn", {cache->k, cache->v, cache->kscale, cache->vscale, cache->table, cache->lens, q, step->starts, out});
     });
 }

@@ -103,6 +103,13 @@ __device__ __forceinline__ uint64_t umma_desc_k128(uint32_t smem_addr, uint32_t 
            ((uint64_t)2 << 61);
 }
 
+// Shared-memory matrix descriptor for a K-major operand of 32 bytes of K in unswizzled core-matrix order: a core matrix is
+// 8 rows x 16 bytes stored contiguously (128 bytes); the two core matrices of a row block lie `lbo` bytes apart, row
+// blocks `sbo` bytes apart.
+__device__ __forceinline__ uint64_t umma_desc_plain(uint32_t smem_addr, uint32_t lbo, uint32_t sbo) {
+    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | ((uint64_t)1 << 46);
+}
+
 // Instruction descriptor: c format bits 4-5 (1 = f32, 2 = s32), a format bits
 // 7-9, b format bits 10-12 (f16 kinds: 0 f16, 1 bf16, 2 tf32; i8 kind: 0 u8,
 // 1 s8), a/b major bits 15/16 (0 = K-major), N >> 3 in bits 17-22, M >> 4 in

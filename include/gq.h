@@ -436,9 +436,9 @@ int32_t gq_paged_advance(gq_ctx* ctx, const gq_paged_cache* cache, const gq_page
 int32_t gq_paged_release(gq_ctx* ctx, const gq_paged_cache* cache, gq_buf which, gq_buf free_list, gq_buf free_count);
 /* The step's rows of fused q | k | v (float32 [max_tokens][(heads + 2 kv_heads) dim]) at one layer: rotary on q and k at
  * the rows' positions (cos / sin [max_pos][dim], the last row beyond), q to q_out [max_tokens][heads dim], k and v into
- * the pool. A block's scale is max|value| / 127 over the tokens it holds: where a new token raises it, the codes that
- * are there already are rounded again, code' = rint(code * (old / new)), so a cached value is off by half a step of the
- * scale of each time it was rounded. A block whose first token is written starts anew. rint(value / scale) with IEEE division;
+ * the pool. A block's scale is max|value| / 127 over the tokens it holds: where a new token raises it, the block's other
+ * codes are rounded again, code' = rint(code * (old / new)), so a cached value is off by half a step of the scale of each
+ * time it was rounded. A block whose first token is written starts anew, with an old scale of 0 and so as zeros. rint(value / scale) with IEEE division;
  * a non-finite value makes its block's scale non-finite and the block read as NaN. One writer per block: two requests of
  * a step must not append to the same block. The dimensions and layers as gq_paged_cache says; 16-byte boundaries. */
 int32_t gq_paged_append(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer, gq_buf qkv, uint64_t heads, gq_buf cos, gq_buf sin,

@@ -83,8 +83,8 @@ def append(codes, scales, values, steps, bs):
             grows = fresh.view(np.uint32) & 0x7FFFFFFF > old.view(np.uint32) & 0x7FFFFFFF
             new = np.where(grows, fresh, old).astype(f)
             ratio = np.where(grows, (old / new).astype(f), f(1))
-            kept = codes[block, :, :off].astype(f) * ratio[:, None, None]
-            codes[block, :, :off] = np.nan_to_num(np.rint(kept)).astype(np.int8)
+            kept = codes[block].astype(f) * ratio[:, None, None]  # the whole block: a new one starts as zeros
+            codes[block] = np.nan_to_num(np.rint(kept)).astype(np.int8)
             c = np.where(new[None, :, None] == 0, f(0), (x / new[None, :, None]).astype(f))
             c = np.clip(np.rint(np.nan_to_num(c, nan=0.0, posinf=127, neginf=-127)), -127, 127).astype(np.int8)
             codes[block, :, off:off + t1 - t0] = np.moveaxis(c, 0, 1)
