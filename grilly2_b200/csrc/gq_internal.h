@@ -277,7 +277,7 @@ uint64_t sample_state_bytes();
 void launch_sample(cudaStream_t s, const float* logits, uint64_t rows, uint64_t v, int32_t* history, uint64_t hist_cap, uint32_t* hist_len,
                    bool do_sample, float temperature, uint64_t top_k, float one_minus_p, float penalty, const float* uniforms,
                    uint64_t uniform_rows, uint32_t* draws, float* scores, float* ex, int32_t* tokens, float* probs, bool append, void* state);
-void launch_sample_rows(cudaStream_t s, const float* logits, uint32_t rows, uint32_t vocab, const float* temperature, const int32_t* top_k,
+void launch_sample_rows(cudaStream_t s, int sm_count, const float* logits, uint32_t rows, uint32_t vocab, const float* temperature, const int32_t* top_k,
                         const float* top_p, const float* min_p, const float* uniforms, uint32_t uniform_rows, uint32_t* draws, int32_t* tokens, float* probs,
                         uint32_t* ticket);
 

@@ -152,6 +152,7 @@ int32_t gq_sample_rows(gq_ctx* ctx, gq_buf logits, uint64_t l_off, uint64_t rows
     return guarded([&] {
         Locked l(ctx);
         check_dims("gq_sample_rows", rows, vocab, uniform_rows);
+        if (vocab > (1u << 23) || rows > (1u << 24)) fail("gq_sample_rows: at most 2^23 tokens and 2^24 rows");
         if (uniform_rows == 0) fail("gq_sample_rows: sampling needs at least one row of uniform numbers");
         if (vocab == 0) fail("gq_sample_rows: expected (batch, vocab) with vocab > 0");
         auto lp = (const float*)view(ctx, logits, l_off, rows * vocab, 4, "gq_sample_rows logits");
@@ -164,7 +165,7 @@ int32_t gq_sample_rows(gq_ctx* ctx, gq_buf logits, uint64_t l_off, uint64_t rows
         auto op = (int32_t*)view(ctx, tokens, 0, rows, 4, "gq_sample_rows tokens");
         auto rp = probs ? (float*)view(ctx, probs, 0, rows, 4, "gq_sample_rows probabilities") : nullptr;
         if (rows == 0) return;
-        launch_sample_rows(ctx->stream, lp, (uint32_t)rows, (uint32_t)vocab, tp, kp, pp, mp, up, (uint32_t)uniform_rows, dp, op, rp,
+        launch_sample_rows(ctx->stream, ctx->prop.multiProcessorCount, lp, (uint32_t)rows, (uint32_t)vocab, tp, kp, pp, mp, up, (uint32_t)uniform_rows, dp, op, rp,
                            (uint32_t*)ctx->sample_state);
         after_launch(ctx, "sample_rows", {logits, temperature, top_k, top_p, min_p, uniforms, draws, tokens, probs});
     });
