@@ -136,6 +136,7 @@ int32_t gq_paged_attn(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer, 
         const uint64_t width = check_heads(op, c, heads);
         check_dims(op, max_count, 1);
         if (max_count == 0) fail("%s: max_count must be at least 1", op);
+        check_dims(op, st.tokens * heads, 1);
         auto qp = (const float*)view(ctx, q, 0, st.tokens * width, 4, "gq_paged_attn q");
         auto yp = (float*)view(ctx, out, 0, st.tokens * width, 4, "gq_paged_attn output");
         check_aligned(op, {qp, yp});

@@ -8,19 +8,24 @@
 // meets them is held as an exact fixed-point integer in three base-256 digits, so three products in int32 and one join
 // give a float32 result:
 //   q_r = 2^(e_r - 22) Q, Q in signed digits; kscale_j is a factor of a lane;
-//   w vscale = 2^(n - 24) P, P in unsigned digits, where 2^n bounds the tile's largest w vscale of that row. The value scales are
-//   folded into P because the sum over j runs across blocks; n follows the tile's own largest product, so a block with large
-//   values and no weight does not coarsen the others' steps.
+//   w vscale = 2^-23 P, P in unsigned digits. The value scales are folded into P because the sum over j runs across blocks;
+//     so that P fits, the running maximum is the one of s + log2 vscale (the largest contribution, not the largest score) and
+//     P's steps are 2^-23 of the largest contribution so far, whatever the blocks' scales are. The denominator sums the w
+//     themselves in float32.
+// Scales of values from 2^-100 to 2^100 (and 0) are exact; larger, negative or non-finite ones read as NaN.
 //
 // A CTA takes a contiguous range of all (request, row tile, KV head, 128-key tile) units, equal ranges for all CTAs: with ragged
 // lengths no CTA waits for a long request, and a single request fills the GPU. A row tile is RP rows of (token, head of the
 // group), N = 3 RP digit rows. An (item = request, row tile, KV head) that ends inside one range is written out; the
 // others leave (max, sum, weighted V) per CTA and the last CTA of an item to arrive adds them in order (deterministic).
-//   warp 5  copies the tile's K and V blocks into a ring of stages (bulk copies; the table gives the addresses)
-//   warp 4  issues the products: S = K Q (128 x N), then D = V P (dim x N) when P is written
-//   warps 0-3  a thread owns a key of S: joins the digits, one maximum over the 128 keys per row (warp reductions and one
-//           exchange), P's digits to shared memory; then it owns a component of D and adds it to its float32 sums
-// Bound: the codes' bytes.
+//   last warp      copies the tile's K and V blocks into a ring of stages (bulk copies; the table gives the addresses)
+//   the one before issues the products: S = K Q (128 x N) of the next tile as soon as S is read, D = V P (dim x N) when P is written
+//   4 WG warps     a thread owns a key of S and RP / WG rows: joins the digits, one maximum over the 128 keys per row (warp
+//                  reductions and one exchange), P's digits to shared memory (four keys to a word: a 4 x 4 transposition
+//                  between neighbouring lanes; byte stores were 3/5 of the kernel); then it owns a component of D and adds it to
+//                  its float32 sums
+// Bound: for single tokens the codes' bytes; for prompts the float32 work per score (about thirty instructions) beside the
+// products.
 #include "gq_internal.h"
 #include "paged.cuh"
 #include "tc_common.cuh"
@@ -30,21 +35,28 @@ namespace gq {
 namespace {
 
 constexpr uint32_t kKeys = 128;    // keys of a tile
-constexpr int kThreads = 192;
 constexpr float kNone = -INFINITY;
 constexpr uint32_t kMostPerSm = 4;  // CTAs of an SM
+constexpr float kMagic = 8388608.0f;  // 2^23: x + 2^23 has rint(x) in its low 23 bits
 
-template <int RP, int DIM>
+template <int RP, int WG, int DIM>
 struct Split {
+    static constexpr int kRows = RP / WG;                                        // rows of a thread
+    static constexpr int kSoft = 128 * WG, kThreads = kSoft + 64;                // softmax threads; all
     static constexpr uint32_t kN = RP == 8 ? 32 : 3 * RP;                        // columns: a multiple of 16; digit d of row r in column d RP + r
-    static constexpr uint32_t kCols = RP == 8 ? 32 : RP == 16 ? 64 : 128;        // S at column 0, D at kCols
+    static constexpr uint32_t kCols = RP == 8 ? 32 : RP == 16 ? 64 : RP == 32 ? 128 : 256;  // S at column 0, D at kCols
     static constexpr uint32_t kM = DIM == 128 ? 128 : 64;                        // lanes of D: dim, at least 64
     static constexpr uint32_t kTileBytes = kKeys * DIM, kStageBytes = 2 * kTileBytes;
-    static constexpr uint32_t kStages = DIM == 128 ? 2 : DIM == 64 ? 3 : 4;
+    static constexpr uint32_t kStages = DIM == 128 ? (RP == 64 ? 3 : 2) : DIM == 64 ? 3 : 4;
     // (dim 32: the 64 lanes of D read 32 rows that are not there, up to 4 KB behind the last stage; nobody reads the sums)
     static constexpr uint32_t kQAt = kStages * kStageBytes + (DIM == 32 ? 4096 : 0);
     static constexpr uint32_t kPAt = kQAt + kN * DIM, kMiscAt = kPAt + kN * kKeys;
-    static constexpr uint32_t kSmem = kMiscAt + 1024 + 4 * RP * 16 + 2 * 4 * RP * 8 + RP * 8 + 4 * RP * 4;
+    // rows' arrays: scale, last position seen, [4] sums, [2][4] maxima, [4] reference and correction of each warp
+    static constexpr uint32_t kSmem = kMiscAt + 1024 + RP * 4 * (1 + 1 + 4 + 8 + 8);
+    // CTAs of an SM: what shared memory and tensor memory hold
+    static constexpr uint32_t kBySmem = (227 * 1024) / (kSmem + 1024), kByTmem = 512 / (2 * kCols), kHeld = kBySmem < kByTmem ? kBySmem : kByTmem;
+    static constexpr uint32_t kPerSm = kHeld < kMostPerSm ? kHeld : kMostPerSm;
+    static_assert(kPerSm >= 1 && kPerSm * RP <= kMostPerSm * 32, "the scratch holds the parts");
 };
 
 __device__ __forceinline__ float warp_max(float v) {  // the largest that is a number
@@ -57,100 +69,134 @@ __device__ __forceinline__ float exp2_fast(float v) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
-template <int R>
-__device__ __forceinline__ void tmem_ld_cols(uint32_t addr, uint32_t (&r)[R]) {
-    if constexpr (R == 8) tmem_ld8(addr, r);
-    else tmem_ld16(addr, r);
-}
-// three digit sums of up to 22 bits, joined with two roundings
+// Three digit sums of up to 22 bits, joined with two roundings. The upper one becomes a float by an integer addition (it is
+// below 2^22), which spares the conversion pipe the exponentials go through.
 __device__ __forceinline__ float join(uint32_t d0, uint32_t d1, uint32_t d2) {
-    return __fmaf_rn((float)(int)d2, 65536.0f, (float)((int)d0 + ((int)d1 << 8)));
+    const float high = __int_as_float((int)d2 + 0x4b400000) - 12582912.0f;
+    return __fmaf_rn(high, 65536.0f, (float)((int)d0 + ((int)d1 << 8)));
 }
 
-// One request's share of the units.
+// sum of floor((a i + b) / m) for i < n, by Euclid's steps on (a, m)
+__device__ uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
+    uint64_t sum = 0;
+    while (n) {
+        if (a >= m) sum += n * (n - 1) / 2 * (a / m), a %= m;
+        if (b >= m) sum += n * (b / m), b %= m;
+        const uint64_t y = a * n + b;
+        if (y < m) break;
+        n = y / m, b = y % m;
+        const uint64_t t = m;
+        m = a, a = t;
+    }
+    return sum;
+}
+
+// One request's share of the units. A row tile's units are the 128-key tiles that its last row sees: all of the request's
+// for the last row tile, floor((len + last token) / 128) + 1 for the others.
 struct Request {
-    uint32_t start, rows, len, keys, tiles, items;  // keys = cached and new ones, inside the table
-    __device__ uint64_t units() const { return (uint64_t)items * tiles; }
+    uint32_t start, rows, len, keys, tiles, row_tiles, group, kv_heads;  // keys = cached and new ones, inside the table
+    uint32_t rp;
+    __device__ uint32_t tiles_of(uint32_t qt) const { return qt + 1 == row_tiles ? tiles : (len + ((qt + 1) * rp - 1) / group) / kKeys + 1; }
+    __device__ uint64_t units_before(uint32_t qt) const {  // qt < row_tiles
+        return qt ? kv_heads * (qt + floor_sum(qt, (uint64_t)kKeys * group, rp, (uint64_t)len * group + rp - 1)) : 0;
+    }
+    __device__ uint64_t units() const { return row_tiles ? units_before(row_tiles - 1) + (uint64_t)kv_heads * tiles : 0; }
 };
 __device__ __forceinline__ Request request_of(const PagedView& c, const StepView& s, uint32_t b, uint32_t group, uint32_t rp) {
     Request r;
     r.start = paged_start(s, b);
     const uint32_t end = paged_start(s, b + 1), count = end > r.start ? end - r.start : 0;
-    r.rows = count * group, r.len = paged_len(c, b);
+    r.rows = count * group, r.len = paged_len(c, b), r.group = group, r.kv_heads = c.kv_heads, r.rp = rp;
     r.keys = min(r.len + count, c.max_blocks << c.shift);
-    r.tiles = (r.keys + kKeys - 1) / kKeys, r.items = (r.rows + rp - 1) / rp * c.kv_heads;
+    r.tiles = (r.keys + kKeys - 1) / kKeys, r.row_tiles = (r.rows + rp - 1) / rp;
     return r;
 }
 
 // What a stretch of one item's tiles is.
 struct Segment {
-    uint32_t b, item, t0, t1;      // tiles [t0, t1): those with a key that some row of the item sees
-    uint32_t row0, rows, head;     // rows of the request's count * group, KV head
-    uint64_t first, last;          // the item's units [first, last)
+    uint32_t b, t0, t1;          // tiles [t0, t1): those with a key that some row of the item sees
+    uint32_t row0, rows, head;   // rows of the request's count * group, KV head
+    uint32_t clear;              // keys that every row of the item sees
+    uint64_t first, last;        // the item's units [first, last)
     bool whole;
 };
 
-// Walks the units [lo, hi) of this CTA, segment by segment; every role runs the same walk.
+// Walks the units [u, hi) of this CTA, segment by segment; every role runs the same walk.
 struct Walk {
-    uint64_t u, hi, base;  // base = the units before request b
-    uint32_t b;
+    uint64_t u, hi, base;  // base = the units before row tile qt of request b
+    uint32_t b, qt;
     Request r;
-    __device__ bool next(const PagedView& c, const StepView& s, uint32_t group, uint32_t rp, Segment& g) {
+    __device__ bool next(const PagedView& c, const StepView& s, Segment& g) {
         if (u >= hi) return false;
-        while (u >= base + r.units()) base += r.units(), r = request_of(c, s, ++b, group, rp);
-        const uint64_t v = u - base;
-        g.b = b, g.item = (uint32_t)(v / r.tiles), g.t0 = (uint32_t)(v - (uint64_t)g.item * r.tiles);
-        g.first = base + (uint64_t)g.item * r.tiles, g.last = g.first + r.tiles;
+        uint32_t tiles;
+        for (;;) {
+            if (qt < r.row_tiles) {
+                tiles = r.tiles_of(qt);
+                if (u < base + (uint64_t)r.kv_heads * tiles) break;
+                base += (uint64_t)r.kv_heads * tiles, ++qt;
+            } else {
+                r = request_of(c, s, ++b, r.group, r.rp), qt = 0;
+            }
+        }
+        const uint32_t v = (uint32_t)(u - base);
+        g.b = b, g.head = v / tiles, g.t0 = v - g.head * tiles;
+        g.first = base + (uint64_t)g.head * tiles, g.last = g.first + tiles;
         const uint64_t end = min(hi, g.last);
         g.whole = u == g.first && end == g.last;
-        g.head = g.item % c.kv_heads, g.row0 = g.item / c.kv_heads * rp, g.rows = min(rp, r.rows - g.row0);
-        const uint32_t seen = min(r.len + (g.row0 + g.rows - 1) / group + 1, r.keys);  // keys of the tile's last token
+        g.row0 = qt * r.rp, g.rows = min(r.rp, r.rows - g.row0);
+        const uint32_t seen = min(r.len + (g.row0 + g.rows - 1) / r.group + 1, r.keys);  // keys of the tile's last token
+        g.clear = min(r.len + g.row0 / r.group + 1, r.keys);
         g.t1 = max(g.t0, min(g.t0 + (uint32_t)(end - u), (seen + kKeys - 1) / kKeys));
         u = end;
         return true;
     }
 };
 
-template <int RP, int DIM>
-__global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedView c, StepView s, const float* __restrict__ q, uint32_t heads, float scale,
-                                                             float* __restrict__ out, float* __restrict__ partials, uint32_t* counters, uint32_t* status) {
-    using T = Split<RP, DIM>;
+template <int RP, int WG, int DIM>
+__global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG, DIM>::kPerSm)) paged_attn_kernel(PagedView c, StepView s, const float* __restrict__ q, uint32_t heads,
+                                                                                 float scale, float* __restrict__ out, float* __restrict__ partials,
+                                                                                 uint32_t* counters, uint32_t* status) {
+    using T = Split<RP, WG, DIM>;
+    constexpr int R = T::kRows;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* misc = smem + T::kMiscAt;
     uint64_t* full = reinterpret_cast<uint64_t*>(misc);  // [kStages] a stage's blocks have landed
     uint64_t* empty = full + 4;                          // [kStages] its products are complete
     uint64_t* s_full = empty + 4;                        // S is complete
-    uint64_t* p_full = s_full + 1;                       // P is written, S and the D before are read
+    uint64_t* s_read = s_full + 1;                       // S is read
+    uint64_t* p_full = s_read + 1;                       // P is written, the D before is read
     uint64_t* d_full = p_full + 1;                       // D is complete
     uint64_t* q_full = d_full + 1;                       // Q is written
-    uint64_t* scan = q_full + 1;                         // [8]
-    uint64_t* found = scan + 8;                          // the units before the request that the range starts in
+    uint64_t* scan = q_full + 1;                         // [16]
+    uint64_t* found = scan + 16;                         // the units before the row tile that the range starts in
     uint32_t* found_b = reinterpret_cast<uint32_t*>(found + 1);
-    uint32_t* tmem_slot = found_b + 1;
+    uint32_t* found_qt = found_b + 1;
+    uint32_t* tmem_slot = found_qt + 1;
     uint32_t* arrived = tmem_slot + 1;
     volatile uint32_t* failed = arrived + 1;
-    float4* rowbuf = reinterpret_cast<float4*>(misc + 1024);             // [4 warps][RP] max, correction, digits' factor, sums' factor
-    float2* exchange = reinterpret_cast<float2*>(rowbuf + 4 * RP);       // [2][4][RP] warps' maxima
-    float2* row_in = exchange + 2 * 4 * RP;                              // [RP] scale of a row of q, last position it sees
-    float* lsum = reinterpret_cast<float*>(row_in + RP);                 // [4][RP]
+    float* row_scale = reinterpret_cast<float*>(misc + 1024);   // [RP] scale of a row's Q, times log2 e
+    int* row_seen = reinterpret_cast<int*>(row_scale + RP);     // [RP] the last position it sees
+    float* lsum = reinterpret_cast<float*>(row_seen + RP);      // [4][RP]
+    float* exchange = lsum + 4 * RP;                            // [2][4][RP] warps' maxima
+    float* refs = exchange + 8 * RP;                            // [4][RP] the rows' references, a copy per warp
+    float* corrs = refs + 4 * RP;                               // [4][RP] what older sums are multiplied by
 
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = heads / c.kv_heads;
     if (tid == 0) {
         for (uint32_t i = 0; i < T::kStages; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
-        mbar_init(s_full, 1), mbar_init(p_full, kKeys), mbar_init(d_full, 1), mbar_init(q_full, kKeys);
+        mbar_init(s_full, 1), mbar_init(s_read, T::kSoft), mbar_init(p_full, T::kSoft), mbar_init(d_full, 1), mbar_init(q_full, T::kSoft);
         *failed = 0;
         mbar_fence_init();
     }
-    if (warp == 4) tmem_alloc(tmem_slot, 2 * T::kCols);
+    if (warp == 4 * WG) tmem_alloc(tmem_slot, 2 * T::kCols);
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = *tmem_slot;
     GQ_GRID_DEP_SYNC();
 
-    // the units of all requests, and the request that this CTA's range starts in
-    const uint32_t per = (c.seqs + kThreads - 1) / kThreads, b0 = min(tid * per, c.seqs), b1 = min(b0 + per, c.seqs);
+    // the units of all requests, and the request and row tile that this CTA's range starts in
+    const uint32_t per = (c.seqs + T::kThreads - 1) / T::kThreads, b0 = min(tid * per, c.seqs), b1 = min(b0 + per, c.seqs);
     uint64_t mine = 0;
     for (uint32_t b = b0; b < b1; ++b) mine += request_of(c, s, b, group, RP).units();
     uint64_t upto = mine;
@@ -162,34 +208,47 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedView c, StepV
     if (lane == 31) scan[warp] = upto;
     __syncthreads();
     uint64_t total = 0, before = upto - mine;
-    for (uint32_t w = 0; w < kThreads / 32; ++w) {
+    for (uint32_t w = 0; w < T::kThreads / 32; ++w) {
         if (w < warp) before += scan[w];
         total += scan[w];
     }
     const uint64_t ctas = min((uint64_t)gridDim.x, total);
     auto range_at = [&](uint64_t i) { return total * i / ctas; };
     Walk walk;
+    walk.u = walk.hi = 0;
     if (blockIdx.x < ctas) {
         walk.u = range_at(blockIdx.x), walk.hi = range_at(blockIdx.x + 1);
         if (walk.u >= before && walk.u < before + mine) {
             uint32_t b = b0;
             uint64_t base = before, units;
             while (walk.u >= base + (units = request_of(c, s, b, group, RP).units())) base += units, ++b;
-            *found = base, *found_b = b;
+            *found = base, *found_b = b, *found_qt = 0;
         }
-    } else {
-        walk.u = walk.hi = 0;
     }
     __syncthreads();
-    walk.base = *found, walk.b = *found_b;
-    if (walk.u < walk.hi) walk.r = request_of(c, s, walk.b, group, RP);
+    if (walk.u < walk.hi) {
+        walk.b = *found_b, walk.base = *found;
+        walk.r = request_of(c, s, walk.b, group, RP);
+        if (walk.r.row_tiles > 1) {  // the same for all: the last row tile that begins at or before u, 32 candidates a round
+            const uint64_t v = walk.u - walk.base;
+            uint32_t lo = 0, hi = walk.r.row_tiles;
+            while (hi - lo > 1) {
+                const uint32_t step = (hi - lo + 31) / 32, k = lo + lane * step;
+                const uint32_t at = 31 - __clz(__ballot_sync(0xffffffffu, k < hi && walk.r.units_before(k) <= v));
+                lo += at * step, hi = min(hi, lo + step);
+            }
+            walk.base += walk.r.units_before(lo), walk.qt = lo;
+        } else {
+            walk.qt = 0;
+        }
+    }
     Segment g;
     bool ok = true;
 
-    if (warp == 5) {
+    if (warp == 4 * WG + 1) {
         uint32_t st = 0, round = 0;
         const uint32_t per_tile = kKeys >> c.shift, bytes = c.block * DIM;
-        while (walk.next(c, s, group, RP, g)) {
+        while (walk.next(c, s, g)) {
             const int32_t* table = c.table + (size_t)g.b * c.max_blocks;
             for (uint32_t t = g.t0; t < g.t1; ++t) {
                 const uint32_t j = t * per_tile + lane;  // one lane per block
@@ -218,27 +277,35 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedView c, StepV
                 }
             }
         }
-    } else if (warp == 4) {
+    } else if (warp == 4 * WG) {
         if (lane == 0) {
             constexpr uint32_t s_desc = umma_idesc(2, 1, 1, kKeys, T::kN);  // s32 sums, s8 codes x s8 digits of q
             constexpr uint32_t d_desc = umma_idesc(2, 1, 0, T::kM, T::kN);  // s32 sums, s8 codes x u8 digits of P
             const uint32_t q_addr = smem_u32(smem + T::kQAt), p_addr = smem_u32(smem + T::kPAt);
             uint32_t st = 0, round = 0, tile = 0, seg = 0;
-            while (walk.next(c, s, group, RP, g)) {
-                if (g.t0 == g.t1) continue;
-                ok = ok && mbar_wait(q_full, seg++ & 1, failed, status, kStatusMmaWaitTimedOut);
-                for (uint32_t t = g.t0; t < g.t1; ++t, ++tile) {
-                    ok = ok && mbar_wait(full + st, round & 1, failed, status, kStatusFullWaitTimedOut);
-                    if (!ok) break;
-                    tc_fence_after_sync();
-                    const uint32_t k_addr = smem_u32(smem + st * T::kStageBytes), v_addr = k_addr + T::kTileBytes;
+            auto score = [&](uint32_t stage, uint32_t parity) {  // S of the tile in `stage`
+                ok = ok && mbar_wait(full + stage, parity, failed, status, kStatusFullWaitTimedOut);
+                if (!ok) return;
+                tc_fence_after_sync();
+                const uint32_t k_addr = smem_u32(smem + stage * T::kStageBytes);
 #pragma unroll
-                    for (uint32_t d = 0; d < DIM / 32; ++d)
-                        umma_i8_ss(tmem, umma_desc_plain(k_addr + 256 * d, 128, 8 * DIM), umma_desc_plain(q_addr + 256 * d, 128, 8 * DIM), s_desc, d != 0);
-                    umma_commit(s_full);
-                    ok = mbar_wait(p_full, tile & 1, failed, status, kStatusMmaWaitTimedOut);
+                for (uint32_t d = 0; d < DIM / 32; ++d)
+                    umma_i8_ss(tmem, umma_desc_plain(k_addr + 256 * d, 128, 8 * DIM), umma_desc_plain(q_addr + 256 * d, 128, 8 * DIM), s_desc, d != 0);
+                umma_commit(s_full);
+            };
+            while (ok && walk.next(c, s, g)) {
+                if (g.t0 == g.t1) continue;
+                ok = mbar_wait(q_full, seg++ & 1, failed, status, kStatusMmaWaitTimedOut);
+                score(st, round & 1);
+                for (uint32_t t = g.t0; t < g.t1 && ok; ++t, ++tile) {
+                    const uint32_t here = st;
+                    if (++st == T::kStages) st = 0, ++round;
+                    ok = mbar_wait(s_read, tile & 1, failed, status, kStatusMmaWaitTimedOut);
+                    if (t + 1 < g.t1) score(st, round & 1);  // while the tile's weights are computed
+                    ok = ok && mbar_wait(p_full, tile & 1, failed, status, kStatusMmaWaitTimedOut);
                     if (!ok) break;
                     tc_fence_after_sync();
+                    const uint32_t v_addr = smem_u32(smem + here * T::kStageBytes) + T::kTileBytes;
 #pragma unroll
                     for (uint32_t i = 0; i < kKeys / 32; ++i) {
                         // keys 32 i ..: two core matrices of one block, or (blocks of 16) of two
@@ -248,34 +315,39 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedView c, StepV
                                    d_desc, i != 0);
                     }
                     umma_commit(d_full);
-                    umma_commit(empty + st);
-                    if (++st == T::kStages) st = 0, ++round;
+                    umma_commit(empty + here);
                 }
             }
         }
     } else {
-        constexpr int kChunk = RP == 8 ? 8 : 16;
-        const uint32_t comp = T::kM == 128 ? tid : 16 * warp + lane;  // the component of D on this thread's lane
+        constexpr int kChunk = 8;
+        const uint32_t quarter = warp & 3, wg = warp >> 2, key = tid & 127, wrow = wg * R;  // this thread's key, its first row
+        const uint32_t comp = T::kM == 128 ? key : 16 * quarter + lane;                    // the component of D on its lane
         const bool owner = T::kM == 128 || (lane < 16 && comp < (uint32_t)DIM);
+        // a 4 x 4 transposition of bytes between lanes: which bytes a lane keeps in its two steps
+        const uint32_t sel1 = lane & 1 ? 0x3715u : 0x6240u, sel2 = lane & 2 ? 0x3276u : 0x5410u;
+        uint8_t* const p_at = smem + T::kPAt + (2 * quarter + (lane >> 4)) * 128 + (lane & 3) * 16 + ((lane >> 2) & 3) * 4;
+        float* const my_refs = refs + quarter * RP + wrow;
+        float* const my_corrs = corrs + quarter * RP + wrow;
         uint32_t tile = 0;
-        float O[RP], l[RP];
+        float O[R], l[R];
         auto drain = [&](uint32_t of_tile) {
             ok = ok && mbar_wait(d_full, of_tile & 1, failed, status, kStatusMmaWaitTimedOut);
             tc_fence_after_sync();
 #pragma unroll
-            for (int r0 = 0; r0 < RP; r0 += kChunk) {
+            for (int r0 = 0; r0 < R; r0 += kChunk) {
                 uint32_t d0[kChunk], d1[kChunk], d2[kChunk];
-                const uint32_t at = tmem_addr(tmem, 32 * warp, T::kCols + r0);
-                tmem_ld_cols(at, d0), tmem_ld_cols(at + RP, d1), tmem_ld_cols(at + 2 * RP, d2);
+                const uint32_t at = tmem_addr(tmem, 32 * quarter, T::kCols + wrow + r0);
+                tmem_ld8(at, d0), tmem_ld8(at + RP, d1), tmem_ld8(at + 2 * RP, d2);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < kChunk; ++i) O[r0 + i] = __fmaf_rn(join(d0[i], d1[i], d2[i]), rowbuf[warp * RP + r0 + i].w, O[r0 + i]);
+                for (int i = 0; i < kChunk; ++i) O[r0 + i] += join(d0[i], d1[i], d2[i]);
             }
         };
-        while (walk.next(c, s, group, RP, g)) {
+        while (walk.next(c, s, g)) {
             // q's rows as three signed digits: lanes of four components
             {
-                constexpr uint32_t kLanes = DIM / 4, kAtOnce = 128 / kLanes;
+                constexpr uint32_t kLanes = DIM / 4, kAtOnce = T::kSoft / kLanes;
                 const uint32_t sub = tid % kLanes, d = 4 * sub;
 #pragma unroll 1
                 for (uint32_t r = tid / kLanes; r < RP; r += kAtOnce) {
@@ -291,8 +363,8 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedView c, StepV
                     const float mult = e < 255 ? __uint_as_float((275u - e) << 23) : 0.0f;  // Q = rint(q 2^(22 - e)), |Q| <= 2^22
                     if (sub == 0) {
                         const float inv = e < 255 ? __uint_as_float((e - 21u) << 23) : __uint_as_float(0x7fc00000u);
-                        const int seen = r < g.rows ? (int)min(walk.r.len + token, walk.r.keys - 1) : -1;
-                        row_in[r] = make_float2(inv * scale, __int_as_float(seen));
+                        row_scale[r] = inv * scale;
+                        row_seen[r] = r < g.rows ? (int)min(walk.r.len + token, walk.r.keys - 1) : -1;
                     }
                     const float x[4] = {v.x, v.y, v.z, v.w};
                     uint32_t w0 = 0, w1 = 0, w2 = 0;
@@ -310,109 +382,137 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedView c, StepV
                     *reinterpret_cast<uint32_t*>(qd + key_at(DIM, 2 * RP + r, d)) = w2;
                 }
             }
-            named_barrier_sync(1, kKeys);  // row_in
+            named_barrier_sync(3, T::kSoft);  // row_scale, row_seen
             if (g.t0 < g.t1) {
                 fence_proxy_async_smem();
                 mbar_arrive(q_full);
             }
 #pragma unroll
-            for (int r = 0; r < RP; ++r) O[r] = l[r] = 0.0f;
-            float M = kNone;  // of row `lane`
+            for (int r = 0; r < R; ++r) O[r] = l[r] = 0.0f;
+            float M = kNone;  // the reference of row `lane`
             const int32_t* table = c.table + (size_t)g.b * c.max_blocks;
             auto entry = [&](uint32_t t) {
-                const uint32_t pos = t * kKeys + tid;
-                return t < g.t1 && pos < walk.r.keys ? table[pos >> c.shift] : -1;
+                const uint32_t pos = t * kKeys + key;
+                const int32_t e = t < g.t1 && pos < walk.r.keys ? table[pos >> c.shift] : -1;
+                return e >= 0 && (uint32_t)e < c.blocks ? e : -1;
             };
             auto scales = [&](int32_t e) {
-                if (e < 0 || (uint32_t)e >= c.blocks) return make_float2(0.0f, -1.0f);  // no such block
+                if (e < 0) return make_float2(0.0f, 0.0f);  // no such block
                 const size_t at = (size_t)e * c.kv_heads + g.head;
                 const float ks = c.kscale[at], vs = c.vscale[at];
-                return make_float2(ks + 0.0f * (ks + vs), fabsf(vs));  // a scale that is no number makes the key's score none
+                // what is no scale makes the key's score no number
+                return make_float2(vs >= 0.0f && vs <= 1.2676506e30f && fabsf(ks) <= 3.0e38f ? ks : __uint_as_float(0x7fc00000u), vs);
             };
-            float2 sc = scales(entry(g.t0));
-            int32_t e_next = entry(g.t0 + 1);
+            int32_t e = entry(g.t0), e_next = entry(g.t0 + 1);
+            float2 sc = scales(e);
             for (uint32_t t = g.t0; t < g.t1; ++t, ++tile) {
                 const float2 sc_next = scales(e_next);
-                e_next = entry(t + 2);
-                if (t > g.t0) drain(tile - 1);
-                const int pos = (int)(t * kKeys + tid);
-                const bool there = !(sc.y < 0.0f) && (uint32_t)pos < walk.r.keys;
-                const float lv = __log2f(sc.y);  // -inf for a block of zeros
+                const int32_t e_then = entry(t + 2);
+                const bool there = e >= 0;
+                // log2 of the value scale and a margin for its rounding, so that P stays below 2^23
+                const float lv = fmaxf(__log2f(sc.y), -100.0f) + 0.001f;
                 ok = ok && mbar_wait(s_full, tile & 1, failed, status, kStatusMmaWaitTimedOut);
                 tc_fence_after_sync();
-                float a[RP], mm = kNone, aa = kNone;
+                float a[R];
 #pragma unroll
-                for (int r0 = 0; r0 < RP; r0 += kChunk) {
+                for (int r0 = 0; r0 < R; r0 += kChunk) {
                     uint32_t d0[kChunk], d1[kChunk], d2[kChunk];
-                    const uint32_t at = tmem_addr(tmem, 32 * warp, r0);
-                    tmem_ld_cols(at, d0), tmem_ld_cols(at + RP, d1), tmem_ld_cols(at + 2 * RP, d2);
+                    const uint32_t at = tmem_addr(tmem, 32 * quarter, wrow + r0);
+                    tmem_ld8(at, d0), tmem_ld8(at + RP, d1), tmem_ld8(at + 2 * RP, d2);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < kChunk; ++i) {
-                        const float2 in = row_in[r0 + i];
-                        const float v = join(d0[i], d1[i], d2[i]) * (in.x * sc.x);
-                        a[r0 + i] = there && pos <= __float_as_int(in.y) ? v : kNone;
-                        const float m = warp_max(a[r0 + i]), n = warp_max(a[r0 + i] + lv);
-                        if (lane == (uint32_t)(r0 + i)) mm = m, aa = n;
+                    for (int i = 0; i < kChunk; i += 4) {
+                        const float4 rs = *reinterpret_cast<const float4*>(row_scale + wrow + r0 + i);
+                        a[r0 + i] = join(d0[i], d1[i], d2[i]) * (rs.x * sc.x);
+                        a[r0 + i + 1] = join(d0[i + 1], d1[i + 1], d2[i + 1]) * (rs.y * sc.x);
+                        a[r0 + i + 2] = join(d0[i + 2], d1[i + 2], d2[i + 2]) * (rs.z * sc.x);
+                        a[r0 + i + 3] = join(d0[i + 3], d1[i + 3], d2[i + 3]) * (rs.w * sc.x);
                     }
                 }
-                float2* ex = exchange + (tile & 1) * 4 * RP;
-                if (lane < (uint32_t)RP) ex[warp * RP + lane] = make_float2(mm, aa);
-                named_barrier_sync(1, kKeys);
-                bool moved = false;
-                if (lane < (uint32_t)RP) {
+                tc_fence_before_sync();
+                mbar_arrive(s_read);
+                if ((t + 1) * kKeys > g.clear || !__all_sync(0xffffffffu, there)) {  // some row does not see some key
+                    const int pos = (int)(t * kKeys + key);
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const float2 o = ex[w * RP + lane];
-                        mm = fmaxf(mm, o.x), aa = fmaxf(aa, o.y);
-                    }
-                    const float top = fmaxf(M, mm), at = top == kNone ? 0.0f : top, corr = exp2_fast(M - at);
-                    const int n = (int)fminf(fmaxf(ceilf(aa - at + 0.001f), -100.0f), 128.0f);
-                    rowbuf[warp * RP + lane] = make_float4(at, corr, pow2(24 - n), pow2(n - 24));
+                    for (int r = 0; r < R; ++r)
+                        if (!there || pos > row_seen[wrow + r]) a[r] = kNone;
+                }
+                float* ex = exchange + (tile & 1) * 4 * RP + wrow;
+#pragma unroll
+                for (int r = 0; r < R; r += 4) {
+                    const float4 m = make_float4(warp_max(a[r] + lv), warp_max(a[r + 1] + lv), warp_max(a[r + 2] + lv), warp_max(a[r + 3] + lv));
+                    if (lane == 0) *reinterpret_cast<float4*>(ex + quarter * RP + r) = m;
+                }
+                if (t > g.t0) drain(tile - 1);
+                named_barrier_sync(1 + wg, 128);
+                bool moved = false;
+                if (lane < (uint32_t)R) {
+                    const float top = fmaxf(fmaxf(fmaxf(M, ex[lane]), fmaxf(ex[RP + lane], ex[2 * RP + lane])), ex[3 * RP + lane]);
+                    const float ref = top == kNone ? 0.0f : top, corr = exp2_fast(M - ref);
+                    my_refs[lane] = ref, my_corrs[lane] = corr;
                     moved = corr != 1.0f;
                     M = top;
                 }
-                const bool rescale = __ballot_sync(0xffffffffu, moved) != 0;
-                uint8_t* pd = smem + T::kPAt + (tid >> 4) * 128 + (tid & 15);
+                __syncwarp();
+                if (__ballot_sync(0xffffffffu, moved)) {
 #pragma unroll
-                for (int r = 0; r < RP; ++r) {
-                    const float4 rb = rowbuf[warp * RP + r];
-                    const float p = exp2_fast(a[r] - rb.x);
-                    if (rescale) l[r] *= rb.y, O[r] *= rb.y;
-                    l[r] += p;
-                    const uint32_t P = min(__float2uint_rn(p * sc.y * rb.z), 0xffffffu);
-                    auto at = [](uint32_t n) { return (n >> 3) * 8 * kKeys + (n & 7) * 16; };
-                    pd[at(r)] = (uint8_t)P, pd[at(RP + r)] = (uint8_t)(P >> 8), pd[at(2 * RP + r)] = (uint8_t)(P >> 16);
+                    for (int r = 0; r < R; ++r) {
+                        const float corr = my_corrs[r];
+                        O[r] *= corr, l[r] *= corr;
+                    }
+                }
+                const float vz = sc.y * kMagic;
+#pragma unroll
+                for (int r = 0; r < R; r += 4) {
+                    const float4 rf = *reinterpret_cast<const float4*>(my_refs + r);
+                    const float p0 = exp2_fast(a[r] - rf.x), p1 = exp2_fast(a[r + 1] - rf.y), p2 = exp2_fast(a[r + 2] - rf.z),
+                                p3 = exp2_fast(a[r + 3] - rf.w);
+                    l[r] += p0, l[r + 1] += p1, l[r + 2] += p2, l[r + 3] += p3;
+                    // rint(p vscale 2^23) in the low 23 bits (one step of the magic number's last place is 1)
+                    const uint32_t x0 = __float_as_uint(fminf(__fmaf_rn(p0, vz, kMagic), 16777215.0f)),
+                                   x1 = __float_as_uint(fminf(__fmaf_rn(p1, vz, kMagic), 16777215.0f)),
+                                   x2 = __float_as_uint(fminf(__fmaf_rn(p2, vz, kMagic), 16777215.0f)),
+                                   x3 = __float_as_uint(fminf(__fmaf_rn(p3, vz, kMagic), 16777215.0f));
+                    // digit d of the four rows, one row to a byte
+                    const uint32_t t0 = __byte_perm(x0, x1, 0x5140), t1 = __byte_perm(x2, x3, 0x5140);
+                    uint32_t w[3] = {__byte_perm(t0, t1, 0x5410), __byte_perm(t0, t1, 0x7632),
+                                     __byte_perm(__byte_perm(x0, x1, 0x0062), __byte_perm(x2, x3, 0x0062), 0x5410)};
+#pragma unroll
+                    for (uint32_t d = 0; d < 3; ++d) {  // ... becomes row r + lane % 4 of four lanes' keys, one key to a byte
+                        w[d] = __byte_perm(w[d], __shfl_xor_sync(0xffffffffu, w[d], 1), sel1);
+                        w[d] = __byte_perm(w[d], __shfl_xor_sync(0xffffffffu, w[d], 2), sel2);
+                        const uint32_t n = d * RP + wrow + r;
+                        *reinterpret_cast<uint32_t*>(p_at + (n >> 3) * 8 * kKeys + (n & 7) * 16) = w[d];
+                    }
                 }
                 fence_proxy_async_smem();
                 tc_fence_before_sync();
                 mbar_arrive(p_full);
-                sc = sc_next;
+                sc = sc_next, e = e_next, e_next = e_then;
             }
             if (g.t0 < g.t1) drain(tile - 1);
             // the rows' sums over the keys, in a fixed order
 #pragma unroll
-            for (int r = 0; r < RP; ++r) {
+            for (int r = 0; r < R; ++r) {
                 float v = l[r];
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-                if (lane == (uint32_t)r) lsum[warp * RP + r] = v;
+                if (lane == (uint32_t)r) lsum[quarter * RP + wrow + r] = v;
             }
-            named_barrier_sync(1, kKeys);
+            named_barrier_sync(3, T::kSoft);
             auto sum_of = [&](uint32_t r) { return (lsum[r] + lsum[RP + r]) + (lsum[2 * RP + r] + lsum[3 * RP + r]); };
             auto out_at = [&](uint32_t r) {
                 const uint32_t row = g.row0 + r;
                 return out + ((size_t)(walk.r.start + row / group) * heads + g.head * group + row % group) * DIM;
             };
+            // (a row that saw no key has neither sum; one whose scores are no numbers keeps them)
+            auto quotient = [](float o, float sum) { return sum == 0.0f ? 0.0f : __fdiv_rn(o * (1.0f / kMagic), sum); };
             if (g.whole) {
                 if (owner)
 #pragma unroll
-                    for (int r = 0; r < RP; ++r)
-                        if ((uint32_t)r < g.rows) {
-                            const float sum = sum_of(r);
-                            out_at(r)[comp] = sum == 0.0f ? 0.0f : __fdiv_rn(O[r], sum);
-                        }
-                named_barrier_sync(1, kKeys);  // lsum and row_in are free
+                    for (int r = 0; r < R; ++r)
+                        if (wrow + r < g.rows) out_at(wrow + r)[comp] = quotient(O[r], sum_of(wrow + r));
+                named_barrier_sync(3, T::kSoft);  // lsum and the rows' arrays are free
                 continue;
             }
             // a part of an item: what this CTA has, and the last CTA to arrive adds the parts up
@@ -422,29 +522,29 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedView c, StepV
             float* part = part_of(blockIdx.x);
             if (owner)
 #pragma unroll
-                for (int r = 0; r < RP; ++r) part[r * DIM + comp] = O[r];
-            if (warp == 0 && lane < (uint32_t)RP) part[RP * DIM + lane] = M, part[RP * DIM + RP + lane] = sum_of(lane);
+                for (int r = 0; r < R; ++r) part[(wrow + r) * DIM + comp] = O[r];
+            if (quarter == 0 && lane < (uint32_t)R) part[RP * DIM + wrow + lane] = M, part[RP * DIM + RP + wrow + lane] = sum_of(wrow + lane);
             __threadfence();
-            named_barrier_sync(1, kKeys);
+            named_barrier_sync(3, T::kSoft);
             if (tid == 0) *arrived = atomicAdd(counters + c0, 1u);
-            named_barrier_sync(1, kKeys);
+            named_barrier_sync(3, T::kSoft);
             const uint32_t parts = (uint32_t)(c1 - c0) + 1;
             if (*arrived != parts - 1) continue;
             __threadfence();
             if (tid == 0) counters[c0] = 0;  // ready for the next call
             constexpr uint32_t kVec = DIM / 32;  // components of a lane
-            for (uint32_t r = warp; r < g.rows; r += 4) {
+            for (uint32_t r = warp; r < g.rows; r += 4 * WG) {
                 float top = kNone;
                 for (uint32_t i = lane; i < parts; i += 32) top = fmaxf(top, __ldcg(part_of(c0 + i) + RP * DIM + r));
                 top = warp_max(top);
-                const float at = top == kNone ? 0.0f : top;
+                const float ref = top == kNone ? 0.0f : top;
                 float sum = 0.0f, acc[kVec] = {};
                 for (uint32_t i0 = 0; i0 < parts; i0 += 32) {
                     const uint32_t i = i0 + lane, here = min(32u, parts - i0);
                     float wgt = 0.0f;
                     if (i < parts) {
                         const float* pp = part_of(c0 + i) + RP * DIM + r;
-                        wgt = exp2_fast(__ldcg(pp) - at);
+                        wgt = exp2_fast(__ldcg(pp) - ref);
                         sum = __fmaf_rn(wgt, __ldcg(pp + RP), sum);
                     }
 #pragma unroll 8
@@ -458,45 +558,45 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedView c, StepV
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
 #pragma unroll
-                for (uint32_t d = 0; d < kVec; ++d) out_at(r)[lane + 32 * d] = sum == 0.0f ? 0.0f : __fdiv_rn(acc[d], sum);
+                for (uint32_t d = 0; d < kVec; ++d) out_at(r)[lane + 32 * d] = quotient(acc[d], sum);
             }
         }
     }
     tc_fence_before_sync();
     __syncthreads();
-    if (warp == 4) tmem_dealloc(tmem, 2 * T::kCols);
+    if (warp == 4 * WG) tmem_dealloc(tmem, 2 * T::kCols);
 }
 
-template <int RP, int DIM>
+template <int RP, int WG, int DIM>
 void launch_split(cudaStream_t s, int sm_count, uint32_t* status, const PagedView& c, const StepView& st, const float* q, uint32_t heads, float scale,
                   float* out, void* state, void* scratch) {
-    using T = Split<RP, DIM>;
-    const uint32_t per_sm = (227 * 1024) / (T::kSmem + 1024), ctas = sm_count * (per_sm < kMostPerSm ? per_sm : kMostPerSm);
-    GQ_CUDA(cudaFuncSetAttribute(paged_attn_kernel<RP, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::kSmem));
-    launch_after(paged_attn_kernel<RP, DIM>, dim3(ctas), dim3(kThreads), T::kSmem, s, c, st, q, heads, scale * 1.4426950408889634f, out,
+    using T = Split<RP, WG, DIM>;
+    GQ_CUDA(cudaFuncSetAttribute(paged_attn_kernel<RP, WG, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::kSmem));
+    launch_after(paged_attn_kernel<RP, WG, DIM>, dim3(sm_count * T::kPerSm), dim3(T::kThreads), T::kSmem, s, c, st, q, heads, scale * 1.4426950408889634f, out,
                  reinterpret_cast<float*>(scratch), reinterpret_cast<uint32_t*>(state), status);
 }
 
-template <int RP>
+template <int RP, int WG>
 void launch_rows(cudaStream_t s, int sm_count, uint32_t* status, const PagedView& c, const StepView& st, const float* q, uint32_t heads, float scale,
                  float* out, void* state, void* scratch) {
-    if (c.dim == 128) launch_split<RP, 128>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
-    else if (c.dim == 64) launch_split<RP, 64>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
-    else launch_split<RP, 32>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+    if (c.dim == 128) launch_split<RP, WG, 128>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+    else if (c.dim == 64) launch_split<RP, WG, 64>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+    else launch_split<RP, WG, 32>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
 }
 
 }  // namespace
 
-// A counter per CTA; two parts per CTA of at most 32 rows.
+// A counter per CTA; two parts per CTA, of at most 32 rows with kMostPerSm CTAs an SM.
 uint64_t paged_attn_state_bytes() { return 1024 * kMostPerSm * 4; }
 uint64_t paged_attn_scratch_bytes(uint32_t dim, int sm_count) { return (uint64_t)sm_count * kMostPerSm * 2 * 32 * (dim + 2) * 4; }
 
 void launch_paged_attn(cudaStream_t s, int sm_count, uint32_t* status, const PagedView& c, const StepView& st, const float* q, uint32_t heads, float scale,
                        uint64_t max_count, float* out, void* state, void* scratch) {
     const uint64_t rows = max_count * (heads / c.kv_heads);
-    if (rows <= 8) launch_rows<8>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
-    else if (rows <= 16) launch_rows<16>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
-    else launch_rows<32>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+    if (rows <= 8) launch_rows<8, 1>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+    else if (rows <= 16) launch_rows<16, 1>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+    else if (rows <= 32) launch_rows<32, 2>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+    else launch_rows<64, 2>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
 }
 
 }  // namespace gq
