@@ -12,6 +12,8 @@
 //     so that P fits, the running maximum is the one of s + log2 vscale (the largest contribution, not the largest score) and
 //     P's steps are 2^-23 of the largest contribution so far, whatever the blocks' scales are. The denominator sums the w
 //     themselves in float32.
+// A warp's 32 keys share one block and so one scale (blocks of 32 and more): the maximum is taken over the joined integers
+// and scaled afterwards, and the exponent is one multiplication and addition of the integer.
 // Scales of values from 2^-100 to 2^100 (and 0) are exact; larger, negative or non-finite ones read as NaN.
 //
 // A CTA takes a contiguous range of all (request, row tile, KV head, 128-key tile) units, equal ranges for all CTAs: with ragged
@@ -51,11 +53,12 @@ struct Split {
     // (dim 32: the 64 lanes of D read 32 rows that are not there, up to 4 KB behind the last stage; nobody reads the sums)
     static constexpr uint32_t kQAt = kStages * kStageBytes + (DIM == 32 ? 4096 : 0);
     static constexpr uint32_t kPAt = kQAt + kN * DIM, kMiscAt = kPAt + kN * kKeys;
-    // rows' arrays: scale, last position seen, [4] sums, [2][4] maxima, [4] reference and correction of each warp
-    static constexpr uint32_t kSmem = kMiscAt + 1024 + RP * 4 * (1 + 1 + 4 + 8 + 8);
+    // rows' arrays: scale, last position seen, [4] sums, [2][4] maxima, [4] factor, reference and correction of each warp
+    static constexpr uint32_t kSmem = kMiscAt + 1024 + RP * 4 * (1 + 1 + 4 + 8 + 12);
     // CTAs of an SM: what shared memory and tensor memory hold
     static constexpr uint32_t kBySmem = (227 * 1024) / (kSmem + 1024), kByTmem = 512 / (2 * kCols), kHeld = kBySmem < kByTmem ? kBySmem : kByTmem;
-    static constexpr uint32_t kPerSm = kHeld < kMostPerSm ? kHeld : kMostPerSm;
+    static constexpr uint32_t kMost = RP == 16 ? 3 : kMostPerSm;  // (registers)
+    static constexpr uint32_t kPerSm = kHeld < kMost ? kHeld : kMost;
     static_assert(kPerSm >= 1 && kPerSm * RP <= kMostPerSm * 32, "the scratch holds the parts");
 };
 
@@ -64,10 +67,28 @@ __device__ __forceinline__ float warp_max(float v) {  // the largest that is a n
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
     return r;
 }
+// a barrier of the softmax threads that tells every one of them whether all say yes
+__device__ __forceinline__ bool all_of(bool mine, uint32_t threads) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, r;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.red.and.pred r, 9, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, r;\n\t}"
+        : "=r"(all)
+        : "r"((uint32_t)mine), "r"(threads)
+        : "memory");
+    return all != 0;
+}
 __device__ __forceinline__ float exp2_fast(float v) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
+}
+// A row's scale times a key's: what the joined integer is multiplied by. Never 0, so that the -inf of a key out of sight stays -inf.
+__device__ __forceinline__ float factor_of(float row, float key) {
+    const float f = row * key;
+    return f < 1e-37f ? 1e-37f : f;
 }
 // Three digit sums of up to 22 bits, joined with two roundings. The upper one becomes a float by an integer addition (it is
 // below 2^22), which spares the conversion pipe the exponentials go through.
@@ -76,19 +97,25 @@ __device__ __forceinline__ float join(uint32_t d0, uint32_t d1, uint32_t d2) {
     return __fmaf_rn(high, 65536.0f, (float)((int)d0 + ((int)d1 << 8)));
 }
 
-// sum of floor((a i + b) / m) for i < n, by Euclid's steps on (a, m)
-__device__ uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
+// sum of floor((a i + b) / m) for i < n, by Euclid's steps on (a, m); the divisions in 32 bits where the numbers allow (a
+// 64-bit one is a hundred instructions, and a range's start takes some twenty)
+template <class U>
+__device__ uint64_t floor_sum_in(U n, U m, U a, U b) {
     uint64_t sum = 0;
     while (n) {
-        if (a >= m) sum += n * (n - 1) / 2 * (a / m), a %= m;
-        if (b >= m) sum += n * (b / m), b %= m;
-        const uint64_t y = a * n + b;
+        if (a >= m) sum += (uint64_t)n * (n - 1) / 2 * (a / m), a %= m;
+        if (b >= m) sum += (uint64_t)n * (b / m), b %= m;
+        const U y = a * n + b;
         if (y < m) break;
         n = y / m, b = y % m;
-        const uint64_t t = m;
+        const U t = m;
         m = a, a = t;
     }
     return sum;
+}
+__device__ uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
+    return a * n + b < (1ull << 32) && m < (1ull << 32) ? floor_sum_in<uint32_t>((uint32_t)n, (uint32_t)m, (uint32_t)a, (uint32_t)b)
+                                                        : floor_sum_in<uint64_t>(n, m, a, b);
 }
 
 // One request's share of the units. A row tile's units are the 128-key tiles that its last row sees: all of the request's
@@ -112,22 +139,26 @@ __device__ __forceinline__ Request request_of(const PagedView& c, const StepView
     return r;
 }
 
-// What a stretch of one item's tiles is.
+// What a stretch of one item's tiles is. The warp that copies walks the CTA's units and hands the segments to the other roles
+// through a ring in shared memory.
 struct Segment {
     uint32_t b, t0, t1;          // tiles [t0, t1): those with a key that some row of the item sees
     uint32_t row0, rows, head;   // rows of the request's count * group, KV head
     uint32_t clear;              // keys that every row of the item sees
+    uint32_t start, len, keys;   // of the request
+    uint32_t whole, more;        // the item is this segment; 0: no segment, the end
     uint64_t first, last;        // the item's units [first, last)
-    bool whole;
 };
+constexpr uint32_t kSegments = 4;  // of the ring
 
-// Walks the units [u, hi) of this CTA, segment by segment; every role runs the same walk.
+// Walks the units [u, hi) of this CTA, segment by segment.
 struct Walk {
     uint64_t u, hi, base;  // base = the units before row tile qt of request b
     uint32_t b, qt;
     Request r;
     __device__ bool next(const PagedView& c, const StepView& s, Segment& g) {
-        if (u >= hi) return false;
+        g.more = u < hi;
+        if (!g.more) return false;
         uint32_t tiles;
         for (;;) {
             if (qt < r.row_tiles) {
@@ -139,7 +170,7 @@ struct Walk {
             }
         }
         const uint32_t v = (uint32_t)(u - base);
-        g.b = b, g.head = v / tiles, g.t0 = v - g.head * tiles;
+        g.b = b, g.start = r.start, g.len = r.len, g.keys = r.keys, g.head = v / tiles, g.t0 = v - g.head * tiles;
         g.first = base + (uint64_t)g.head * tiles, g.last = g.first + tiles;
         const uint64_t end = min(hi, g.last);
         g.whole = u == g.first && end == g.last;
@@ -152,10 +183,11 @@ struct Walk {
     }
 };
 
-template <int RP, int WG, int DIM>
-__global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG, DIM>::kPerSm)) paged_attn_kernel(PagedView c, StepView s, const float* __restrict__ q, uint32_t heads,
-                                                                                 float scale, float* __restrict__ out, float* __restrict__ partials,
-                                                                                 uint32_t* counters, uint32_t* status) {
+// ONE: the keys of a warp share a block (blocks of 32 tokens and more).
+template <int RP, int WG, int DIM, bool ONE>
+__global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG, DIM>::kPerSm))
+    paged_attn_kernel(PagedView c, StepView s, const float* __restrict__ q, uint32_t heads, float scale, float* __restrict__ out,
+                      float* __restrict__ partials, uint32_t* counters, uint32_t* status) {
     using T = Split<RP, WG, DIM>;
     constexpr int R = T::kRows;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -167,23 +199,29 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
     uint64_t* p_full = s_read + 1;                       // P is written, the D before is read
     uint64_t* d_full = p_full + 1;                       // D is complete
     uint64_t* q_full = d_full + 1;                       // Q is written
-    uint64_t* scan = q_full + 1;                         // [16]
-    uint64_t* found = scan + 16;                         // the units before the row tile that the range starts in
+    uint64_t* seg_full = q_full + 1;                     // [kSegments] a segment is written
+    uint64_t* seg_free = seg_full + kSegments;           // [kSegments] ... and done with
+    uint64_t* scan = seg_free + kSegments;               // [24]
+    uint64_t* found = scan + 24;                         // the units before the row tile that the range starts in
     uint32_t* found_b = reinterpret_cast<uint32_t*>(found + 1);
     uint32_t* found_qt = found_b + 1;
     uint32_t* tmem_slot = found_qt + 1;
     uint32_t* arrived = tmem_slot + 1;
     volatile uint32_t* failed = arrived + 1;
+    Segment* segments = reinterpret_cast<Segment*>(misc + 512);   // [kSegments]
+    float2* warp_scales = reinterpret_cast<float2*>(misc + 768);  // [2][WG][4] a warp's key scale and log2 of its value scale
     float* row_scale = reinterpret_cast<float*>(misc + 1024);   // [RP] scale of a row's Q, times log2 e
     int* row_seen = reinterpret_cast<int*>(row_scale + RP);     // [RP] the last position it sees
     float* lsum = reinterpret_cast<float*>(row_seen + RP);      // [4][RP]
     float* exchange = lsum + 4 * RP;                            // [2][4][RP] warps' maxima
-    float* refs = exchange + 8 * RP;                            // [4][RP] the rows' references, a copy per warp
+    float* refs = exchange + 8 * RP;                            // [4][RP] the rows' references (negative), a copy per warp
     float* corrs = refs + 4 * RP;                               // [4][RP] what older sums are multiplied by
+    float* factors = corrs + 4 * RP;                            // [4][RP] a row's scale times the warp's key scale
 
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = heads / c.kv_heads;
     if (tid == 0) {
         for (uint32_t i = 0; i < T::kStages; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
+        for (uint32_t i = 0; i < kSegments; ++i) mbar_init(seg_full + i, 1), mbar_init(seg_free + i, T::kSoft + 1);
         mbar_init(s_full, 1), mbar_init(s_read, T::kSoft), mbar_init(p_full, T::kSoft), mbar_init(d_full, 1), mbar_init(q_full, T::kSoft);
         *failed = 0;
         mbar_fence_init();
@@ -212,52 +250,67 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
         if (w < warp) before += scan[w];
         total += scan[w];
     }
-    const uint64_t ctas = min((uint64_t)gridDim.x, total);
-    auto range_at = [&](uint64_t i) { return total * i / ctas; };
-    Walk walk;
-    walk.u = walk.hi = 0;
+    // ranges of `share` units, the first `extra` ones of one more
+    const uint32_t ctas = (uint32_t)min((uint64_t)gridDim.x, total);
+    const uint64_t share = ctas ? (total >> 32 ? total / ctas : (uint32_t)total / ctas) : 0, extra = total - share * ctas;
+    auto range_at = [&](uint32_t i) { return i * share + min((uint64_t)i, extra); };
+    auto cta_of = [&](uint64_t u) {  // whose range holds unit u
+        const uint64_t longer = extra * (share + 1);
+        const uint64_t v = u < longer ? u : u - longer, by = u < longer ? share + 1 : share;
+        return (uint32_t)((u < longer ? 0 : extra) + (v >> 32 || by >> 32 ? v / by : (uint32_t)v / (uint32_t)by));
+    };
     if (blockIdx.x < ctas) {
-        walk.u = range_at(blockIdx.x), walk.hi = range_at(blockIdx.x + 1);
-        if (walk.u >= before && walk.u < before + mine) {
+        const uint64_t u = range_at(blockIdx.x);
+        if (u >= before && u < before + mine) {
             uint32_t b = b0;
             uint64_t base = before, units;
-            while (walk.u >= base + (units = request_of(c, s, b, group, RP).units())) base += units, ++b;
-            *found = base, *found_b = b, *found_qt = 0;
+            while (u >= base + (units = request_of(c, s, b, group, RP).units())) base += units, ++b;
+            *found = base, *found_b = b;
         }
     }
     __syncthreads();
-    if (walk.u < walk.hi) {
-        walk.b = *found_b, walk.base = *found;
-        walk.r = request_of(c, s, walk.b, group, RP);
-        if (walk.r.row_tiles > 1) {  // the same for all: the last row tile that begins at or before u, 32 candidates a round
-            const uint64_t v = walk.u - walk.base;
-            uint32_t lo = 0, hi = walk.r.row_tiles;
-            while (hi - lo > 1) {
-                const uint32_t step = (hi - lo + 31) / 32, k = lo + lane * step;
-                const uint32_t at = 31 - __clz(__ballot_sync(0xffffffffu, k < hi && walk.r.units_before(k) <= v));
-                lo += at * step, hi = min(hi, lo + step);
-            }
-            walk.base += walk.r.units_before(lo), walk.qt = lo;
-        } else {
-            walk.qt = 0;
-        }
-    }
-    Segment g;
     bool ok = true;
 
     if (warp == 4 * WG + 1) {
+        Walk walk;
+        walk.u = walk.hi = 0;
+        if (blockIdx.x < ctas) {
+            walk.u = range_at(blockIdx.x), walk.hi = range_at(blockIdx.x + 1);
+            walk.b = *found_b, walk.base = *found, walk.qt = 0;
+            walk.r = request_of(c, s, walk.b, group, RP);
+            if (walk.r.row_tiles > 1) {  // the last row tile that begins at or before u, 32 candidates a round
+                const uint64_t v = walk.u - walk.base;
+                uint32_t lo = 0, hi = walk.r.row_tiles;
+                while (hi - lo > 1) {
+                    const uint32_t step = (hi - lo + 31) / 32, k = lo + lane * step;
+                    const uint32_t at = 31 - __clz(__ballot_sync(0xffffffffu, k < hi && walk.r.units_before(k) <= v));
+                    lo += at * step, hi = min(hi, lo + step);
+                }
+                walk.base += walk.r.units_before(lo), walk.qt = lo;
+            }
+        }
         uint32_t st = 0, round = 0;
         const uint32_t per_tile = kKeys >> c.shift, bytes = c.block * DIM;
-        while (walk.next(c, s, g)) {
+        for (uint32_t seg = 0; ok; ++seg) {
+            Segment g;
+            const bool more = walk.next(c, s, g);
+            if (seg >= kSegments) ok = mbar_wait(seg_free + seg % kSegments, (seg / kSegments - 1) & 1, failed, status, kStatusEmptyWaitTimedOut);
+            if (__ballot_sync(0xffffffffu, !ok)) ok = false;
+            if (!ok) break;
+            if (lane == 0) {
+                segments[seg % kSegments] = g;
+                mbar_arrive(seg_full + seg % kSegments);
+            }
+            if (!more) break;
             const int32_t* table = c.table + (size_t)g.b * c.max_blocks;
             for (uint32_t t = g.t0; t < g.t1; ++t) {
                 const uint32_t j = t * per_tile + lane;  // one lane per block
-                int32_t e = lane < per_tile && j < c.max_blocks && (j << c.shift) < walk.r.keys ? table[j] : -1;
+                int32_t e = lane < per_tile && j < c.max_blocks && (j << c.shift) < g.keys ? table[j] : -1;
                 if (e < 0 || (uint32_t)e >= c.blocks) e = -1;
                 if (round) ok = ok && mbar_wait(empty + st, (round - 1) & 1, failed, status, kStatusEmptyWaitTimedOut);
                 const uint32_t held = __popc(__ballot_sync(0xffffffffu, e >= 0));
                 if (__ballot_sync(0xffffffffu, !ok)) ok = false;
-                if (!ok) continue;
+                if (!ok) break;
                 if (lane == 0) mbar_arrive_expect_tx(full + st, held * 2 * bytes);
                 __syncwarp();
                 if (e >= 0) {
@@ -282,7 +335,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
             constexpr uint32_t s_desc = umma_idesc(2, 1, 1, kKeys, T::kN);  // s32 sums, s8 codes x s8 digits of q
             constexpr uint32_t d_desc = umma_idesc(2, 1, 0, T::kM, T::kN);  // s32 sums, s8 codes x u8 digits of P
             const uint32_t q_addr = smem_u32(smem + T::kQAt), p_addr = smem_u32(smem + T::kPAt);
-            uint32_t st = 0, round = 0, tile = 0, seg = 0;
+            uint32_t st = 0, round = 0, tile = 0;
             auto score = [&](uint32_t stage, uint32_t parity) {  // S of the tile in `stage`
                 ok = ok && mbar_wait(full + stage, parity, failed, status, kStatusFullWaitTimedOut);
                 if (!ok) return;
@@ -293,15 +346,20 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                     umma_i8_ss(tmem, umma_desc_plain(k_addr + 256 * d, 128, 8 * DIM), umma_desc_plain(q_addr + 256 * d, 128, 8 * DIM), s_desc, d != 0);
                 umma_commit(s_full);
             };
-            while (ok && walk.next(c, s, g)) {
-                if (g.t0 == g.t1) continue;
-                ok = mbar_wait(q_full, seg++ & 1, failed, status, kStatusMmaWaitTimedOut);
+            for (uint32_t i = 0, turn = 0; ok; ++i) {
+                ok = mbar_wait(seg_full + i % kSegments, (i / kSegments) & 1, failed, status, kStatusMmaWaitTimedOut);
+                if (!ok) break;
+                const uint32_t more = segments[i % kSegments].more, tiles = segments[i % kSegments].t1 - segments[i % kSegments].t0;
+                mbar_arrive(seg_free + i % kSegments);
+                if (!more) break;
+                if (tiles == 0) continue;
+                ok = mbar_wait(q_full, turn++ & 1, failed, status, kStatusMmaWaitTimedOut);
                 score(st, round & 1);
-                for (uint32_t t = g.t0; t < g.t1 && ok; ++t, ++tile) {
+                for (uint32_t t = 0; t < tiles && ok; ++t, ++tile) {
                     const uint32_t here = st;
                     if (++st == T::kStages) st = 0, ++round;
                     ok = mbar_wait(s_read, tile & 1, failed, status, kStatusMmaWaitTimedOut);
-                    if (t + 1 < g.t1) score(st, round & 1);  // while the tile's weights are computed
+                    if (t + 1 < tiles) score(st, round & 1);  // while the tile's weights are computed
                     ok = ok && mbar_wait(p_full, tile & 1, failed, status, kStatusMmaWaitTimedOut);
                     if (!ok) break;
                     tc_fence_after_sync();
@@ -329,6 +387,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
         uint8_t* const p_at = smem + T::kPAt + (2 * quarter + (lane >> 4)) * 128 + (lane & 3) * 16 + ((lane >> 2) & 3) * 4;
         float* const my_refs = refs + quarter * RP + wrow;
         float* const my_corrs = corrs + quarter * RP + wrow;
+        float* const my_factors = factors + quarter * RP + wrow;
         uint32_t tile = 0;
         float O[R], l[R];
         auto drain = [&](uint32_t of_tile) {
@@ -344,37 +403,49 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                 for (int i = 0; i < kChunk; ++i) O[r0 + i] += join(d0[i], d1[i], d2[i]);
             }
         };
-        while (walk.next(c, s, g)) {
+        for (uint32_t seg = 0;; ++seg) {
+            ok = ok && mbar_wait(seg_full + seg % kSegments, (seg / kSegments) & 1, failed, status, kStatusMmaWaitTimedOut);
+            if (!all_of(ok, T::kSoft)) break;  // one verdict for all: they meet at barriers below
+            const Segment& g = segments[seg % kSegments];
+            if (!g.more) break;
+            const uint32_t t0 = g.t0, t1 = g.t1, clear_keys = g.clear;
             // q's rows as three signed digits: lanes of four components
             {
-                constexpr uint32_t kLanes = DIM / 4, kAtOnce = T::kSoft / kLanes;
+                constexpr uint32_t kLanes = DIM / 4, kAtOnce = T::kSoft / kLanes, kTurns = (RP + kAtOnce - 1) / kAtOnce;
                 const uint32_t sub = tid % kLanes, d = 4 * sub;
-#pragma unroll 1
-                for (uint32_t r = tid / kLanes; r < RP; r += kAtOnce) {
-                    const uint32_t row = g.row0 + r, token = row / group;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                float4 row_q[kTurns];  // all loads in flight together
+#pragma unroll
+                for (uint32_t i = 0; i < kTurns; ++i) {
+                    const uint32_t r = tid / kLanes + i * kAtOnce, row = g.row0 + r;
+                    row_q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (r < g.rows)
-                        v = *reinterpret_cast<const float4*>(q + ((size_t)(walk.r.start + token) * heads + g.head * group + row % group) * DIM + d);
+                        row_q[i] = *reinterpret_cast<const float4*>(q + ((size_t)(g.start + row / group) * heads + g.head * group + row % group) * DIM + d);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < kTurns; ++i) {
+                    const uint32_t r = tid / kLanes + i * kAtOnce, token = (g.row0 + r) / group;
+                    if (kTurns * kAtOnce > RP && r >= RP) break;
+                    const float4 v = row_q[i];
                     uint32_t m = max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
                                      max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
 #pragma unroll
                     for (uint32_t o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
                     const uint32_t e = max(m >> 23, 32u);  // 2^(e - 126) > max |q|
-                    const float mult = e < 255 ? __uint_as_float((275u - e) << 23) : 0.0f;  // Q = rint(q 2^(22 - e)), |Q| <= 2^22
+                    const float mult = e < 255 ? copysignf(__uint_as_float((275u - e) << 23), scale) : 0.0f;  // Q = rint(+-q 2^(22 - e)), |Q| <= 2^22
                     if (sub == 0) {
                         const float inv = e < 255 ? __uint_as_float((e - 21u) << 23) : __uint_as_float(0x7fc00000u);
-                        row_scale[r] = inv * scale;
-                        row_seen[r] = r < g.rows ? (int)min(walk.r.len + token, walk.r.keys - 1) : -1;
+                        row_scale[r] = inv * fabsf(scale);
+                        row_seen[r] = r < g.rows ? (int)min(g.len + token, g.keys - 1) : -1;
                     }
                     const float x[4] = {v.x, v.y, v.z, v.w};
                     uint32_t w0 = 0, w1 = 0, w2 = 0;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        int Q = __float2int_rn(x[i] * mult);
+                    for (int j = 0; j < 4; ++j) {
+                        int Q = __float2int_rn(x[j] * mult);
                         const int d0 = (int)(int8_t)Q;
                         Q = (Q - d0) >> 8;
                         const int d1 = (int)(int8_t)Q, d2 = (Q - d1) >> 8;
-                        w0 |= ((uint32_t)d0 & 0xffu) << (8 * i), w1 |= ((uint32_t)d1 & 0xffu) << (8 * i), w2 |= ((uint32_t)d2 & 0xffu) << (8 * i);
+                        w0 |= ((uint32_t)d0 & 0xffu) << (8 * j), w1 |= ((uint32_t)d1 & 0xffu) << (8 * j), w2 |= ((uint32_t)d2 & 0xffu) << (8 * j);
                     }
                     uint8_t* qd = smem + T::kQAt;
                     *reinterpret_cast<uint32_t*>(qd + key_at(DIM, r, d)) = w0;
@@ -382,8 +453,8 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                     *reinterpret_cast<uint32_t*>(qd + key_at(DIM, 2 * RP + r, d)) = w2;
                 }
             }
-            named_barrier_sync(3, T::kSoft);  // row_scale, row_seen
-            if (g.t0 < g.t1) {
+            named_barrier_sync(8, T::kSoft);  // row_scale, row_seen
+            if (t0 < t1) {
                 fence_proxy_async_smem();
                 mbar_arrive(q_full);
             }
@@ -392,8 +463,8 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
             float M = kNone;  // the reference of row `lane`
             const int32_t* table = c.table + (size_t)g.b * c.max_blocks;
             auto entry = [&](uint32_t t) {
-                const uint32_t pos = t * kKeys + key;
-                const int32_t e = t < g.t1 && pos < walk.r.keys ? table[pos >> c.shift] : -1;
+                const uint32_t j = (t * kKeys + key) >> c.shift;  // (a key behind the last one has its block's scale)
+                const int32_t e = t < t1 && (j << c.shift) < g.keys ? table[j] : -1;
                 return e >= 0 && (uint32_t)e < c.blocks ? e : -1;
             };
             auto scales = [&](int32_t e) {
@@ -401,19 +472,19 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                 const size_t at = (size_t)e * c.kv_heads + g.head;
                 const float ks = c.kscale[at], vs = c.vscale[at];
                 // what is no scale makes the key's score no number
-                return make_float2(vs >= 0.0f && vs <= 1.2676506e30f && fabsf(ks) <= 3.0e38f ? ks : __uint_as_float(0x7fc00000u), vs);
+                return make_float2(vs >= 0.0f && vs <= 1.2676506e30f && ks >= 0.0f && ks <= 3.0e38f ? ks : __uint_as_float(0x7fc00000u), vs);
             };
-            int32_t e = entry(g.t0), e_next = entry(g.t0 + 1);
+            int32_t e = entry(t0), e_next = entry(t0 + 1);
             float2 sc = scales(e);
-            for (uint32_t t = g.t0; t < g.t1; ++t, ++tile) {
+            const float my_scale = lane < (uint32_t)R ? row_scale[wrow + lane] : 0.0f;  // of row `lane`
+            for (uint32_t t = t0; t < t1; ++t, ++tile) {
                 const float2 sc_next = scales(e_next);
                 const int32_t e_then = entry(t + 2);
-                const bool there = e >= 0;
                 // log2 of the value scale and a margin for its rounding, so that P stays below 2^23
                 const float lv = fmaxf(__log2f(sc.y), -100.0f) + 0.001f;
                 ok = ok && mbar_wait(s_full, tile & 1, failed, status, kStatusMmaWaitTimedOut);
                 tc_fence_after_sync();
-                float a[R];
+                float a[R];  // q . k in units of the row's and the key's scales
 #pragma unroll
                 for (int r0 = 0; r0 < R; r0 += kChunk) {
                     uint32_t d0[kChunk], d1[kChunk], d2[kChunk];
@@ -421,62 +492,81 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                     tmem_ld8(at, d0), tmem_ld8(at + RP, d1), tmem_ld8(at + 2 * RP, d2);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < kChunk; i += 4) {
-                        const float4 rs = *reinterpret_cast<const float4*>(row_scale + wrow + r0 + i);
-                        a[r0 + i] = join(d0[i], d1[i], d2[i]) * (rs.x * sc.x);
-                        a[r0 + i + 1] = join(d0[i + 1], d1[i + 1], d2[i + 1]) * (rs.y * sc.x);
-                        a[r0 + i + 2] = join(d0[i + 2], d1[i + 2], d2[i + 2]) * (rs.z * sc.x);
-                        a[r0 + i + 3] = join(d0[i + 3], d1[i + 3], d2[i + 3]) * (rs.w * sc.x);
-                    }
+                    for (int i = 0; i < kChunk; ++i) a[r0 + i] = join(d0[i], d1[i], d2[i]);
                 }
                 tc_fence_before_sync();
                 mbar_arrive(s_read);
-                if ((t + 1) * kKeys > g.clear || !__all_sync(0xffffffffu, there)) {  // some row does not see some key
-                    const int pos = (int)(t * kKeys + key);
+                // Where some row does not see some key, or a scale is none: a key out of sight scores -inf, and a row that sees a
+                // key without a scale has no sum. (The scales themselves are then finite, so that -inf stays -inf.)
+                const bool bad = !(sc.x >= 0.0f);
+                if ((t + 1) * kKeys > clear_keys || __any_sync(0xffffffffu, e < 0 || bad)) {
+                    const int pos = e < 0 ? 0x7fffffff : (int)(t * kKeys + key);
 #pragma unroll
-                    for (int r = 0; r < R; ++r)
-                        if (!there || pos > row_seen[wrow + r]) a[r] = kNone;
+                    for (int r = 0; r < R; ++r) {
+                        const bool seen = pos <= row_seen[wrow + r];
+                        if (!seen) a[r] = kNone;
+                        else if (bad) l[r] = __uint_as_float(0x7fc00000u);
+                    }
                 }
+                const float ks = bad ? 1.0f : sc.x;
                 float* ex = exchange + (tile & 1) * 4 * RP + wrow;
+                float2* ws = warp_scales + (tile & 1) * 4 * WG + wg * 4;
 #pragma unroll
                 for (int r = 0; r < R; r += 4) {
-                    const float4 m = make_float4(warp_max(a[r] + lv), warp_max(a[r + 1] + lv), warp_max(a[r + 2] + lv), warp_max(a[r + 3] + lv));
-                    if (lane == 0) *reinterpret_cast<float4*>(ex + quarter * RP + r) = m;
+                    float m[4];
+                    float4 rs;
+                    if (!ONE) rs = *reinterpret_cast<const float4*>(row_scale + wrow + r);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        m[i] = warp_max(ONE ? a[r + i] : __fmaf_rn(a[r + i], factor_of(i == 0 ? rs.x : i == 1 ? rs.y : i == 2 ? rs.z : rs.w, ks), lv));
+                    if (lane == 0) *reinterpret_cast<float4*>(ex + quarter * RP + r) = make_float4(m[0], m[1], m[2], m[3]);
                 }
-                if (t > g.t0) drain(tile - 1);
+                if (ONE && lane == 0) ws[quarter] = make_float2(ks, lv);
+                if (t > t0) drain(tile - 1);
                 named_barrier_sync(1 + wg, 128);
                 bool moved = false;
                 if (lane < (uint32_t)R) {
-                    const float top = fmaxf(fmaxf(fmaxf(M, ex[lane]), fmaxf(ex[RP + lane], ex[2 * RP + lane])), ex[3 * RP + lane]);
+                    float top = M;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const float m = ex[w * RP + lane];
+                        top = fmaxf(top, ONE ? __fmaf_rn(m, factor_of(my_scale, ws[w].x), ws[w].y) : m);
+                    }
                     const float ref = top == kNone ? 0.0f : top, corr = exp2_fast(M - ref);
-                    my_refs[lane] = ref, my_corrs[lane] = corr;
+                    my_refs[lane] = -ref, my_corrs[lane] = corr;
+                    if (ONE) my_factors[lane] = factor_of(my_scale, ks);
                     moved = corr != 1.0f;
                     M = top;
                 }
                 __syncwarp();
-                if (__ballot_sync(0xffffffffu, moved)) {
+                const uint32_t rows_moved = __ballot_sync(0xffffffffu, moved);
+                if (rows_moved) {
 #pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        const float corr = my_corrs[r];
-                        O[r] *= corr, l[r] *= corr;
-                    }
+                    for (int r = 0; r < R; r += 4)
+                        if (rows_moved >> r & 15u) {
+                            const float4 cr = *reinterpret_cast<const float4*>(my_corrs + r);
+                            O[r] *= cr.x, O[r + 1] *= cr.y, O[r + 2] *= cr.z, O[r + 3] *= cr.w;
+                            l[r] *= cr.x, l[r + 1] *= cr.y, l[r + 2] *= cr.z, l[r + 3] *= cr.w;
+                        }
                 }
                 const float vz = sc.y * kMagic;
 #pragma unroll
                 for (int r = 0; r < R; r += 4) {
                     const float4 rf = *reinterpret_cast<const float4*>(my_refs + r);
-                    const float p0 = exp2_fast(a[r] - rf.x), p1 = exp2_fast(a[r + 1] - rf.y), p2 = exp2_fast(a[r + 2] - rf.z),
-                                p3 = exp2_fast(a[r + 3] - rf.w);
-                    l[r] += p0, l[r + 1] += p1, l[r + 2] += p2, l[r + 3] += p3;
-                    // rint(p vscale 2^23) in the low 23 bits (one step of the magic number's last place is 1)
-                    const uint32_t x0 = __float_as_uint(fminf(__fmaf_rn(p0, vz, kMagic), 16777215.0f)),
-                                   x1 = __float_as_uint(fminf(__fmaf_rn(p1, vz, kMagic), 16777215.0f)),
-                                   x2 = __float_as_uint(fminf(__fmaf_rn(p2, vz, kMagic), 16777215.0f)),
-                                   x3 = __float_as_uint(fminf(__fmaf_rn(p3, vz, kMagic), 16777215.0f));
+                    const float4 fc = *reinterpret_cast<const float4*>((ONE ? my_factors : row_scale + wrow) + r);
+                    uint32_t x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float f = i == 0 ? fc.x : i == 1 ? fc.y : i == 2 ? fc.z : fc.w, ref = i == 0 ? rf.x : i == 1 ? rf.y : i == 2 ? rf.z : rf.w;
+                        const float p = exp2_fast(__fmaf_rn(a[r + i], ONE ? f : factor_of(f, ks), ref));
+                        l[r + i] += p;
+                        // rint(p vscale 2^23) in the low 23 bits (the last place of 2^23 is 1)
+                        x[i] = __float_as_uint(fminf(__fmaf_rn(p, vz, kMagic), 16777215.0f));
+                    }
                     // digit d of the four rows, one row to a byte
-                    const uint32_t t0 = __byte_perm(x0, x1, 0x5140), t1 = __byte_perm(x2, x3, 0x5140);
-                    uint32_t w[3] = {__byte_perm(t0, t1, 0x5410), __byte_perm(t0, t1, 0x7632),
-                                     __byte_perm(__byte_perm(x0, x1, 0x0062), __byte_perm(x2, x3, 0x0062), 0x5410)};
+                    const uint32_t y0 = __byte_perm(x[0], x[1], 0x5140), y1 = __byte_perm(x[2], x[3], 0x5140);
+                    uint32_t w[3] = {__byte_perm(y0, y1, 0x5410), __byte_perm(y0, y1, 0x7632),
+                                     __byte_perm(__byte_perm(x[0], x[1], 0x0062), __byte_perm(x[2], x[3], 0x0062), 0x5410)};
 #pragma unroll
                     for (uint32_t d = 0; d < 3; ++d) {  // ... becomes row r + lane % 4 of four lanes' keys, one key to a byte
                         w[d] = __byte_perm(w[d], __shfl_xor_sync(0xffffffffu, w[d], 1), sel1);
@@ -490,7 +580,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                 mbar_arrive(p_full);
                 sc = sc_next, e = e_next, e_next = e_then;
             }
-            if (g.t0 < g.t1) drain(tile - 1);
+            if (t0 < t1) drain(tile - 1);
             // the rows' sums over the keys, in a fixed order
 #pragma unroll
             for (int r = 0; r < R; ++r) {
@@ -499,39 +589,52 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                 for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
                 if (lane == (uint32_t)r) lsum[quarter * RP + wrow + r] = v;
             }
-            named_barrier_sync(3, T::kSoft);
+            named_barrier_sync(8, T::kSoft);
             auto sum_of = [&](uint32_t r) { return (lsum[r] + lsum[RP + r]) + (lsum[2 * RP + r] + lsum[3 * RP + r]); };
-            auto out_at = [&](uint32_t r) {
-                const uint32_t row = g.row0 + r;
-                return out + ((size_t)(walk.r.start + row / group) * heads + g.head * group + row % group) * DIM;
-            };
-            // (a row that saw no key has neither sum; one whose scores are no numbers keeps them)
-            auto quotient = [](float o, float sum) { return sum == 0.0f ? 0.0f : __fdiv_rn(o * (1.0f / kMagic), sum); };
+            // a row that saw no key has neither sum and gives zeros
+            auto share_of = [](float sum) { return sum == 0.0f ? 0.0f : __fdiv_rn(1.0f / kMagic, sum); };
             if (g.whole) {
+                // the rows' factors and places, once each (the arrays of the tile loop are free)
+                if (tid < RP) {
+                    row_scale[tid] = share_of(sum_of(tid));
+                    row_seen[tid] = tid < g.rows ? (int)((g.row0 + tid) / group * heads + (g.row0 + tid) % group) : -1;
+                }
+                named_barrier_sync(8, T::kSoft);
+                float* at = out + ((size_t)g.start * heads + g.head * group) * DIM + comp;
                 if (owner)
 #pragma unroll
-                    for (int r = 0; r < R; ++r)
-                        if (wrow + r < g.rows) out_at(wrow + r)[comp] = quotient(O[r], sum_of(wrow + r));
-                named_barrier_sync(3, T::kSoft);  // lsum and the rows' arrays are free
+                    for (int r = 0; r < R; ++r) {
+                        const int row = row_seen[wrow + r];
+                        if (row >= 0) at[(size_t)row * DIM] = O[r] * row_scale[wrow + r];
+                    }
+                named_barrier_sync(8, T::kSoft);  // lsum and the rows' arrays are free
+                mbar_arrive(seg_free + seg % kSegments);
                 continue;
             }
             // a part of an item: what this CTA has, and the last CTA to arrive adds the parts up
             constexpr uint32_t kPart = RP * (DIM + 2);
-            const uint64_t c0 = ((g.first + 1) * ctas - 1) / total, c1 = (g.last * ctas - 1) / total;
-            auto part_of = [&](uint64_t cta) { return partials + (cta * 2 + (cta == c0 && range_at(c0) != g.first ? 1 : 0)) * kPart; };
+            const uint32_t c0 = cta_of(g.first), parts = cta_of(g.last - 1) - c0 + 1;
+            const uint32_t second = range_at(c0) != g.first;  // the first CTA's range began with another item
+            auto part_of = [&](uint32_t cta) { return partials + (size_t)(cta * 2 + (cta == c0 ? second : 0)) * kPart; };
             float* part = part_of(blockIdx.x);
             if (owner)
 #pragma unroll
                 for (int r = 0; r < R; ++r) part[(wrow + r) * DIM + comp] = O[r];
             if (quarter == 0 && lane < (uint32_t)R) part[RP * DIM + wrow + lane] = M, part[RP * DIM + RP + wrow + lane] = sum_of(wrow + lane);
             __threadfence();
-            named_barrier_sync(3, T::kSoft);
+            named_barrier_sync(8, T::kSoft);
             if (tid == 0) *arrived = atomicAdd(counters + c0, 1u);
-            named_barrier_sync(3, T::kSoft);
-            const uint32_t parts = (uint32_t)(c1 - c0) + 1;
-            if (*arrived != parts - 1) continue;
+            named_barrier_sync(8, T::kSoft);
+            if (*arrived != parts - 1) {
+                mbar_arrive(seg_free + seg % kSegments);
+                continue;
+            }
             __threadfence();
             if (tid == 0) counters[c0] = 0;  // ready for the next call
+            auto out_at = [&](uint32_t r) {
+                const uint32_t row = g.row0 + r;
+                return out + ((size_t)(g.start + row / group) * heads + g.head * group + row % group) * DIM;
+            };
             constexpr uint32_t kVec = DIM / 32;  // components of a lane
             for (uint32_t r = warp; r < g.rows; r += 4 * WG) {
                 float top = kNone;
@@ -557,9 +660,11 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                 }
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                const float factor = share_of(sum);
 #pragma unroll
-                for (uint32_t d = 0; d < kVec; ++d) out_at(r)[lane + 32 * d] = quotient(acc[d], sum);
+                for (uint32_t d = 0; d < kVec; ++d) out_at(r)[lane + 32 * d] = acc[d] * factor;
             }
+            mbar_arrive(seg_free + seg % kSegments);
         }
     }
     tc_fence_before_sync();
@@ -567,21 +672,29 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
     if (warp == 4 * WG) tmem_dealloc(tmem, 2 * T::kCols);
 }
 
-template <int RP, int WG, int DIM>
+template <int RP, int WG, int DIM, bool ONE>
 void launch_split(cudaStream_t s, int sm_count, uint32_t* status, const PagedView& c, const StepView& st, const float* q, uint32_t heads, float scale,
                   float* out, void* state, void* scratch) {
     using T = Split<RP, WG, DIM>;
-    GQ_CUDA(cudaFuncSetAttribute(paged_attn_kernel<RP, WG, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::kSmem));
-    launch_after(paged_attn_kernel<RP, WG, DIM>, dim3(sm_count * T::kPerSm), dim3(T::kThreads), T::kSmem, s, c, st, q, heads, scale * 1.4426950408889634f, out,
+    GQ_CUDA(cudaFuncSetAttribute(paged_attn_kernel<RP, WG, DIM, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::kSmem));
+    launch_after(paged_attn_kernel<RP, WG, DIM, ONE>, dim3(sm_count * T::kPerSm), dim3(T::kThreads), T::kSmem, s, c, st, q, heads, scale * 1.4426950408889634f, out,
                  reinterpret_cast<float*>(scratch), reinterpret_cast<uint32_t*>(state), status);
 }
 
-template <int RP, int WG>
+template <int RP, int WG, bool ONE>
 void launch_rows(cudaStream_t s, int sm_count, uint32_t* status, const PagedView& c, const StepView& st, const float* q, uint32_t heads, float scale,
                  float* out, void* state, void* scratch) {
-    if (c.dim == 128) launch_split<RP, WG, 128>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
-    else if (c.dim == 64) launch_split<RP, WG, 64>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
-    else launch_split<RP, WG, 32>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+    if (c.dim == 128) launch_split<RP, WG, 128, ONE>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+    else if (c.dim == 64) launch_split<RP, WG, 64, ONE>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+    else launch_split<RP, WG, 32, ONE>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+}
+template <bool ONE>
+void launch_blocks(cudaStream_t s, int sm_count, uint32_t* status, const PagedView& c, const StepView& st, const float* q, uint32_t heads, float scale,
+                   uint64_t rows, float* out, void* state, void* scratch) {
+    if (rows <= 8) launch_rows<8, 1, ONE>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+    else if (rows <= 16) launch_rows<16, 1, ONE>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+    else if (rows <= 32) launch_rows<32, 2, ONE>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+    else launch_rows<64, 4, ONE>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
 }
 
 }  // namespace
@@ -593,10 +706,8 @@ uint64_t paged_attn_scratch_bytes(uint32_t dim, int sm_count) { return (uint64_t
 void launch_paged_attn(cudaStream_t s, int sm_count, uint32_t* status, const PagedView& c, const StepView& st, const float* q, uint32_t heads, float scale,
                        uint64_t max_count, float* out, void* state, void* scratch) {
     const uint64_t rows = max_count * (heads / c.kv_heads);
-    if (rows <= 8) launch_rows<8, 1>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
-    else if (rows <= 16) launch_rows<16, 1>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
-    else if (rows <= 32) launch_rows<32, 2>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
-    else launch_rows<64, 2>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+    if (c.block >= 32) launch_blocks<true>(s, sm_count, status, c, st, q, heads, scale, rows, out, state, scratch);
+    else launch_blocks<false>(s, sm_count, status, c, st, q, heads, scale, rows, out, state, scratch);
 }
 
 }  // namespace gq
