@@ -20,9 +20,10 @@ from dataclasses import dataclass, fields, replace
 import numpy as np
 
 from .. import _C
-from .sampling import Generator, Sampler
+from .paged import PagedKvCache, PagedStep
+from .sampling import Generator, Sampler, _default_generator, sample_rows
 
-__all__ = ["GenerationConfig", "generate"]
+__all__ = ["GenerationConfig", "generate", "generate_batch"]
 
 
 @dataclass
@@ -102,3 +103,99 @@ def generate(model, inputs=None, generation_config: GenerationConfig | None = No
             break
     out = sampler.history.numpy()[0, :prompt + done]
     return out[None].astype(np.int64)
+
+
+def _per_request(name: str, value, n: int, off, dtype):
+    """A setting for every request: one value for all (None: ``off``), or a sequence of n."""
+    values = list(value) if isinstance(value, (list, tuple, np.ndarray)) else [value] * n
+    if len(values) != n:
+        raise ValueError(f"`{name}` must be one value or one per prompt ({n}), got {len(values)}")
+    return np.array([off if v is None else v for v in values], dtype=dtype)
+
+
+def generate_batch(model, prompts, generation_config: GenerationConfig | None = None, *, min_p=0.0, block_size: int = 64, blocks: int | None = None,
+                   generator: Generator | None = None, graphed: bool = True, **kwargs) -> list:
+    """``generate()`` for several prompts at once over a paged int8 cache: the prompts run as one ragged step, then every
+    step decodes one token of each request still running; the step, block tables and sampler included, is one captured
+    graph. ``do_sample``, ``temperature``, ``top_k``, ``top_p`` and ``min_p`` may be sequences with a setting for each prompt. A request
+    that ends at ``eos_token_id`` gives its blocks back. ``blocks``: the pool's size (the default holds all requests to the end); a
+    pool that runs out raises. Returns a list of int64 arrays, prompt first. No counterpart in the reference (batch 1)."""
+    rows = [np.asarray(p).reshape(-1) for p in prompts]
+    n = len(rows)
+    if n == 0 or any(r.size == 0 or not np.issubdtype(r.dtype, np.integer) for r in rows):
+        raise ValueError("`prompts` must be non-empty sequences of integer token ids")
+    config = replace(generation_config or GenerationConfig())
+    unused = [k for k in kwargs if k not in _FIELDS]
+    if unused:
+        raise ValueError(f"The following `model_kwargs` are not used by the model: {unused}")
+    for k, v in kwargs.items():
+        setattr(config, k, v)
+    if config.num_beams != 1:
+        raise NotImplementedError("grilly: generate_batch() with num_beams > 1 (beam search) is not implemented yet")
+    if config.repetition_penalty not in (None, 1.0):
+        raise NotImplementedError("grilly: generate_batch() with a repetition penalty is not implemented yet")
+    cfg = model.cfg
+    new = [(config.max_new_tokens if config.max_new_tokens is not None else config.max_length - r.size) for r in rows]
+    new = [max(v, 0) for v in new]
+    steps = max(new)
+    if any(r.size + v > cfg.max_cache_len + 1 for r, v in zip(rows, new)):
+        raise RuntimeError(f"a request may hold {cfg.max_cache_len} cached positions; prompt + new tokens = "
+                           f"{max(r.size + v for r, v in zip(rows, new))}")
+    if steps == 0:
+        return [r.astype(np.int64) for r in rows]
+    sampled = _per_request("do_sample", config.do_sample, n, False, bool)
+    heat = _per_request("temperature", config.temperature, n, 1.0, np.float32)
+    if (sampled & ~(heat > 0)).any():
+        raise ValueError("`temperature` has to be a strictly positive float, otherwise your next token scores will be invalid. If you're "
+                         "looking for greedy decoding strategies, set `do_sample=False`.")
+    T = _C.Tensor.from_numpy
+    settings = {"temperature": T(np.where(sampled, heat, 0.0).astype(np.float32)),
+                "top_k": T(_per_request("top_k", config.top_k, n, 0, np.int32)), "top_p": T(_per_request("top_p", config.top_p, n, 1.0, np.float32)),
+                "min_p": T(_per_request("min_p", min_p, n, 0.0, np.float32))}
+    eos = config.eos_token_id
+    eos = set() if eos is None else {int(eos)} if isinstance(eos, (int, np.integer)) else {int(e) for e in eos}
+    if blocks is None:  # the last token is never cached
+        blocks = sum(-(-max(r.size + v - 1, 1) // block_size) for r, v in zip(rows, new))
+    cache = PagedKvCache.for_model(cfg, seqs=n, blocks=blocks, block_size=block_size)
+    uniforms = T((generator or _default_generator).uniform((steps, n)))
+    draws, chosen = T(np.zeros(1, dtype=np.int32)), _C.Tensor.empty((n,), "int32")
+    counts, tokens = T(np.array([r.size for r in rows], dtype=np.int32)), T(np.concatenate(rows).astype(np.int32))
+
+    def run(tokens, counts, step, max_count):
+        cache.plan(counts, step)
+        sample_rows(model.step_paged(tokens, cache, step, max_count=max_count), uniforms, draws=draws, tokens=chosen, **settings)
+
+    prompt_step = PagedStep(cache, tokens.numel())
+    run(tokens, counts, prompt_step, max(r.size for r in rows))
+    if prompt_step.shortfall():
+        raise RuntimeError(f"the pool of {blocks} blocks cannot hold the prompts: {prompt_step.shortfall()} more are needed")
+    step = PagedStep(cache, n)
+    tokens, counts = _C.Tensor.empty((n,), "int32"), _C.Tensor.empty((n,), "int32")  # the decode step's inputs
+
+    def decode():
+        run(tokens, counts, step, 1)
+
+    import grilly2_b200 as g
+    decode = g.graphed(decode) if graphed else decode
+    out, running = [list(map(int, r)) for r in rows], [v > 0 for v in new]
+    gone = [False] * n
+    while True:
+        for b, t in enumerate(chosen.numpy()):
+            if running[b]:
+                out[b].append(int(t))
+                running[b] = len(out[b]) < rows[b].size + new[b] and int(t) not in eos and t >= 0
+        over = [not r and not x for r, x in zip(running, gone)]
+        if any(over):
+            cache.release(T(np.array(over, dtype=np.int32)))
+            gone = [not r for r in running]
+        live = [b for b in range(n) if running[b]]
+        if not live:
+            return [np.array(o, dtype=np.int64) for o in out]
+        # a request's row in the step: the running ones in order
+        row = np.zeros(n, dtype=np.int32)
+        row[:len(live)] = [out[b][-1] for b in live]
+        tokens.copy_(T(row))
+        counts.copy_(T(np.array(running, dtype=np.int32)))
+        decode()
+        if step.shortfall():
+            raise RuntimeError(f"the pool of {blocks} blocks has run out: {len(live)} requests are running")

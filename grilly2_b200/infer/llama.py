@@ -214,6 +214,43 @@ class LlamaDecoder:
         check(lib.gq_kv_advance_by(ctx, self.cache.lens.storage.handle, c.num_hidden_layers, c.max_cache_len, T))
         return logits
 
+    def step_paged(self, tokens: "_C.Tensor", cache, step, max_count: int | None = None):
+        """One step of several requests over a ``PagedKvCache``: tokens int32 [step.max_tokens], the step's rows as
+        ``cache.plan(counts, step)`` has laid them out (prompts, single tokens, or both; rows behind the last request's are ignored).
+        Returns the logits of every request's last row, [seqs, vocab], NaN where a request has no row, and advances the
+        cache. Nothing reads a host integer, so a captured step replays. ``max_count``: the largest count expected (1 for a decode
+        step). No counterpart in the reference, which runs one request."""
+        c, lib, ctx = self.cfg, _lib.load(), _C.context()
+        T = step.max_tokens
+        if tokens.dtype != "int32" or tokens.numel() != T or tokens.offset:
+            raise RuntimeError(f"step_paged takes {T} int32 tokens at offset 0, got {list(tokens.shape)} {tokens.dtype} at {tokens.offset}")
+        if (cache.layers, cache.kv_heads, cache.head_dim) != (c.num_hidden_layers, c.num_key_value_heads, c.head_dim):
+            raise RuntimeError(f"the cache is for {cache.layers} layers of {cache.kv_heads} x {cache.head_dim}, the model has "
+                               f"{c.num_hidden_layers} of {c.num_key_value_heads} x {c.head_dim}")
+        hidden = _C.Tensor.empty((T, c.hidden_size), "float32")
+        check(lib.gq_embedding(ctx, self.embed.storage.handle, tokens.storage.handle, T, c.hidden_size, c.vocab_size, hidden.storage.handle))
+        delta = None
+        for li, lw in enumerate(self.layers):
+            x, summed = self._norm(hidden, delta, lw["input_norm"], delta is not None, T)
+            if summed is not None:
+                hidden = summed
+            q = cache.append(li, lw["qkv"].linear(x, lw["qkv_bias"]), c.num_attention_heads, self.cos, self.sin, step)
+            o = lw["o"].linear(cache.attend(li, q, c.num_attention_heads, step, max_count=max_count))
+            x, hidden = self._norm(hidden, o, lw["post_norm"], True, T)
+            gu = lw["gate_up"].linear(x)
+            act = _C.Tensor.empty((T, c.intermediate_size), "float32")
+            check(lib.gq_swiglu(ctx, gu.storage.handle, T, c.intermediate_size, act.storage.handle))
+            delta = lw["down"].linear(act)
+        last = []
+        for rows in (hidden, delta):  # the last row of every request
+            out = _C.Tensor.empty((cache.seqs, c.hidden_size), "float32")
+            check(lib.gq_embedding(ctx, rows.storage.handle, step.last.storage.handle, cache.seqs, c.hidden_size, T, out.storage.handle))
+            last.append(out)
+        x, _ = self._norm(last[0], last[1], self.norm, False, cache.seqs)
+        logits = self.lm_head.linear(x)
+        cache.advance(step)
+        return logits
+
     def _make_plan(self):
         c, lib = self.cfg, _lib.load()
         layers = (_lib.DecodeLayer * c.num_hidden_layers)()

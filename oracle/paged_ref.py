@@ -156,3 +156,46 @@ def sample(x, temperature, top_k, top_p, min_p, u):
     hit = np.nonzero((c > np.float64(u) * c[-1]) & (w > 0))[0]
     i = int(hit[0]) if len(hit) else int(np.nonzero(w > 0)[0][-1])
     return i, w[i] / c[-1]
+
+
+class PagedDecoderRef:
+    """float64 model of a decoder whose requests share a paged int8 cache: oracle.llama_ref's arithmetic with the cached rows as
+    the codes and block scales that ``append`` leaves. ``step`` takes the new tokens of every request and returns the logits
+    of each one's last token (None where it has none)."""
+
+    def __init__(self, cfg, weights, cos, sin, seqs, block):
+        from .llama_ref import DecoderRef
+        self.m, self.cfg, self.block, self.seqs = DecoderRef(cfg, weights, cos, sin), cfg, block, seqs
+        per = -(-cfg.max_cache_len // block)
+        shape = (cfg.num_hidden_layers, seqs * per, cfg.num_key_value_heads)
+        self.codes = {n: np.zeros(shape + (block, cfg.head_dim), np.int8) for n in "kv"}
+        self.scales = {n: np.zeros(shape, np.float32) for n in "kv"}
+        self.table = np.arange(seqs * per, dtype=np.int32).reshape(seqs, per)  # which block holds what does not matter here
+        self.lens = np.zeros(seqs, np.int64)
+
+    def step(self, new):
+        c, m, D = self.cfg, self.m, self.cfg.head_dim
+        counts = [len(t) for t in new]
+        steps, _ = plan(self.lens, counts, self.table, [], 0, self.block, self.table.size, max(sum(counts), 1))
+        pos = steps["positions"][:sum(counts)]
+        h = m.embed[[t for r in new for t in r]].copy()
+        norm = lambda x, w: x / np.sqrt((x * x).mean(-1, keepdims=True) + c.rms_norm_eps) * w  # noqa: E731
+
+        def turn(x):
+            x = x.reshape(len(pos), -1, D)
+            return x * m.cos[pos][:, None] + np.concatenate([-x[..., D // 2:], x[..., :D // 2]], -1) * m.sin[pos][:, None]
+
+        for li, lw in enumerate(m.layers):
+            x = norm(h, lw["input_norm"])
+            q = turn(x @ lw["q"].T + lw["q_bias"])
+            k, v = turn(x @ lw["k"].T + lw["k_bias"]), (x @ lw["v"].T + lw["v_bias"]).reshape(len(pos), -1, D)
+            append(self.codes["k"][li], self.scales["k"][li], k.astype(np.float32), steps, self.block)
+            append(self.codes["v"][li], self.scales["v"][li], v.astype(np.float32), steps, self.block)
+            out, _ = attend(q, self.codes["k"][li], self.codes["v"][li], self.scales["k"][li], self.scales["v"][li], self.table, self.lens, steps,
+                            D ** -0.5)
+            h = h + out.reshape(len(pos), -1) @ lw["o"].T
+            x = norm(h, lw["post_norm"])
+            g, u = x @ lw["gate"].T, x @ lw["up"].T
+            h = h + (g / (1.0 + np.exp(-g)) * u) @ lw["down"].T
+        self.lens = self.lens + counts
+        return [m.head @ norm(h[r], m.norm) if r >= 0 else None for r in steps["last"]]
