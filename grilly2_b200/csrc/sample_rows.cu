@@ -1,17 +1,20 @@
 // The next token of every row with settings of its own: temperature, top-k, top-p, min-p, and the draw by the inverse CDF in
 // token order (include/gq.h, gq_sample_rows). Beside gq_sample (sample.cu), which has one setting for all rows.
 //
-// w_i = exp((x_i - M) / T), M the row's maximum, in float64; top-p's masses as 64-bit integers w 2^40, so that
-// histograms do not depend on the order of their additions. A row is a cluster of up to eight CTAs that keep its logits in
-// shared memory: they are read from memory once, and a row's work is spread where there are few rows.
-//   1 the maximum
-//   2 top-k: a histogram of counts over 2048 bins that are linear in x (the top 64 T nats, or the row's range where
-//     that is less: what lies below weighs under e^-64 and is dropped), its crossing bin, and that bin's tokens as a list
-//     that the cluster's first CTA ranks by comparing all pairs
-//   3 top-p: the same with masses
-//   4 every warp's kept mass, in token order; the warp that holds the target walks its tokens
+// w_i = exp((x_i - M) / T), M the row's maximum, in float64; where masses are added by atomics they are whole numbers w 2^40, so
+// that no result depends on their order. A row is a cluster of up to eight CTAs that keep its logits in shared memory: they
+// are read from memory once, and a row's work is spread where there are few rows. "Bins" are 2048 steps linear in x over
+// the top 64 T nats, or over the row's range where that is less; what lies below weighs under e^-64 and is dropped.
+//   1 every thread's maximum, the row's maximum
+//   2 top-k, as long as there are k threads: the threads' maxima alone go into a histogram; at least k tokens lie in or above the
+//     bin where it reaches k. Those are listed in the first CTA's shared memory, and it finishes the row alone: it
+//     counts for every listed token how many and how much lie above, and for the kept ones how much lies before.
+//   3 otherwise, for top-k and then top-p: a histogram of all tokens (counts or masses), its crossing bin, and that bin's
+//     tokens as a list that is ranked the same way
+//   4 every thread's kept mass, a thread owning consecutive tokens; the thread that holds the target walks its own
 // A bin of more tokens than the list holds (ties, a flat row) falls back to bisecting the float's bits with a pass over the
-// row per step. Bound: latency (some ten cluster barriers); of large batches the float64 pipe, ~14 operations a token.
+// row per step. Bound: latency (4 to 12 cluster barriers); of large batches without top-k the arithmetic of a float64
+// exponential a token.
 #include <cooperative_groups.h>
 
 #include "gq_internal.h"
@@ -22,20 +25,29 @@ namespace gq {
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 1024, kWarps = kThreads / 32;
 constexpr uint32_t kBins = 2048, kList = 2048, kMostCtas = 8;
 constexpr double kFixed = 1099511627776.0;  // 2^40
-constexpr uint32_t kStaged = 44 * 1024;     // logits of a row that a CTA keeps at most
+constexpr uint32_t kStaged = 46 * 1024;     // logits of a row that a CTA keeps at most
 
-__device__ __forceinline__ uint32_t key_of(float f) {  // a < b as floats <=> key_of(a) < key_of(b); NaN as -inf
-    const uint32_t b = f == f ? __float_as_uint(f) : 0xff800000u;
+__device__ __forceinline__ uint32_t key_of(float f) {  // a < b as floats <=> key_of(a) < key_of(b)
+    const uint32_t b = __float_as_uint(f);
     return (b >> 31) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k); }
+// a logit as it is compared: NaN counts as -inf, -0 is 0
+__device__ __forceinline__ float clean(float v) { return v == v ? v + 0.0f : -INFINITY; }
+
+// A float as a double without the conversion pipe: the exponent moved over, the mantissa shifted. (A zero or a denormal becomes
+// a number of 2^-127, which is as good beside a logit.)
+__device__ __forceinline__ double widen(float v) {
+    const uint32_t b = __float_as_uint(v);
+    return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
+}
 
 struct Control {
     uint32_t top[2];             // this CTA's largest key, smallest above -inf
-    uint32_t border, listed, low, range_lo, range_hi, owner_warp;
+    uint32_t border, listed, low, range_lo, range_hi, owner_warp, pick, last;
     unsigned long long above, target, part[2];
     double before, goal, total;
     double warp_sum[kWarps];
@@ -50,7 +62,7 @@ struct alignas(16) Shared {  // the logits behind it are stored four at a time
         } hist;
         struct {
             unsigned long long mass[kList];
-            uint32_t key[kList];
+            uint32_t key[kList], at[kList];  // the token's index
         } list;
     };
 };
@@ -73,7 +85,7 @@ __device__ __forceinline__ double exp_of(double y, const double* pow2) {
     return __hiloint2double(__double2hiint(v) + ((n >> 6) << 20), __double2loint(v));
 }
 
-__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* __restrict__ logits, uint32_t vocab, uint32_t slice, uint32_t staged,
+__global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* __restrict__ logits, uint32_t vocab, uint32_t slice, uint32_t staged,
                                                                  const float* __restrict__ temperature, const int32_t* __restrict__ top_k,
                                                                  const float* __restrict__ top_p, const float* __restrict__ min_p,
                                                                  const float* __restrict__ uniforms, uint32_t uniform_rows, uint32_t* draws, int32_t* tokens,
@@ -100,39 +112,46 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* _
     }
 
     // 1: the row into shared memory, its largest and smallest values
-    const uint32_t none = key_of(__uint_as_float(0xff800000u));
-    uint32_t mk = 0, lk = 0xffffffffu;
+    float most = -INFINITY, least_seen = INFINITY;
     auto see = [&](float v) {
-        const uint32_t k = key_of(v);
-        mk = max(mk, k);
-        if (k != none) lk = min(lk, k);
+        most = fmaxf(most, v);
+        if (v != -INFINITY) least_seen = fminf(least_seen, v);
     };
-    uint32_t i0 = 0;
-    if (staged && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
-        i0 = n & ~3u;
+    const uint32_t lead_in = min(n, (uint32_t)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / 4), quads = (n - lead_in) / 4;
+    if (staged) {
+        // (the part on 16-byte boundaries four at a time; in shared memory the logits lie one behind the other from 0 on)
+        const float4* x4 = reinterpret_cast<const float4*>(x + lead_in);
 #pragma unroll 4
-        for (uint32_t i = 4 * tid; i < i0; i += 4 * kThreads) {
-            const float4 v = __ldcs(reinterpret_cast<const float4*>(x + i));
-            *reinterpret_cast<float4*>(stage + i) = v;
+        for (uint32_t i = tid; i < quads; i += kThreads) {
+            float4 v = __ldcs(x4 + i);
+            v = make_float4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
+            float* at = stage + lead_in + 4 * i;
+            if (lead_in == 0) *reinterpret_cast<float4*>(at) = v;
+            else at[0] = v.x, at[1] = v.y, at[2] = v.z, at[3] = v.w;
             see(v.x), see(v.y), see(v.z), see(v.w);
         }
+        for (uint32_t i = tid; i < n - 4 * quads; i += kThreads) {  // the few before and behind
+            const uint32_t at = i < lead_in ? i : 4 * quads + i;
+            const float v = clean(x[at]);
+            stage[at] = v;
+            see(v);
+        }
+    } else {
+        for (uint32_t i = tid; i < n; i += kThreads) see(clean(x[i]));
     }
-#pragma unroll 4
-    for (uint32_t i = i0 + tid; i < n; i += kThreads) {
-        const float v = x[i];
-        if (staged) stage[i] = v;
-        see(v);
+    auto logit = [&](uint32_t i) { return staged ? stage[i] : clean(x[i]); };
+    {
+        const uint32_t mk = __reduce_max_sync(0xffffffffu, key_of(most)), lk = __reduce_min_sync(0xffffffffu, key_of(least_seen));
+        if (lane == 0) atomicMax(&sh.ctl.top[0], mk), atomicMin(&sh.ctl.top[1], lk);
     }
-    const float* xs = staged ? stage : x;
-    mk = __reduce_max_sync(0xffffffffu, mk), lk = __reduce_min_sync(0xffffffffu, lk);
-    if (lane == 0) atomicMax(&sh.ctl.top[0], mk), atomicMin(&sh.ctl.top[1], lk);
     cluster.sync();
+    uint32_t mk = 0, lk = 0xffffffffu;
     for (uint32_t c = 0; c < ctas; ++c) {
         const Control& o = cluster.map_shared_rank(&sh, c)->ctl;
         mk = max(mk, o.top[0]), lk = min(lk, o.top[1]);
     }
-
-    if (mk == none) {  // every logit is -inf
+    const float M = value_of(mk), tf = temperature[row];
+    if (M == -INFINITY) {  // every logit is -inf
         if (rank == 0 && tid == 0) {
             tokens[row] = -1;
             if (probs) probs[row] = 0.0f;
@@ -140,34 +159,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* _
         cluster.sync();  // nobody leaves while its shared memory may be read
         return;
     }
-    const float M = value_of(mk), tf = temperature[row];
     const bool greedy = !(tf > 0.0f);
     const double Md = (double)M, inv_t = greedy ? 0.0 : 1.0 / (double)tf;
     const float per_x = fmaxf(32.0f / tf, (float)(kBins - 1) / (M - value_of(lk)));
-    auto weight = [&](uint32_t key, float v) { return key == mk ? 1.0 : exp_of(((double)v - Md) * inv_t, sh.pow2); };
-    auto fixed = [&](uint32_t key) { return (unsigned long long)(weight(key, value_of(key)) * kFixed + 0.5); };
-    auto bin_of = [&](uint32_t key, float v) {  // monotone in the key
-        const float f = key == mk ? 0.0f : (M - v) * per_x;
-        return f < (float)kBins ? (int)f : -1;
+    auto weight = [&](float v) { return v == M ? 1.0 : exp_of((widen(v) - Md) * inv_t, sh.pow2); };
+    auto fixed = [&](float v) {  // w 2^40 as a whole number, by the last place of 2^52
+        return (unsigned long long)__double_as_longlong(__fma_rn(weight(v), kFixed, 4503599627370496.0)) & 0xfffffffffffffull;
     };
-    uint32_t low = greedy ? mk : none + 1;  // keys below are dropped
+    // falls as v rises; rounded by the last place of 2^23
+    auto bin_of = [&](float v) { return v == M ? 0 : (int)(__float_as_uint(fminf((M - v) * per_x, (float)(kBins - 1)) + 8388608.0f) & (kBins - 1)); };
+    // tokens below are dropped: at first what weighs less than e^-64 (in a bin behind the last, too)
+    float low = greedy ? M : fmaxf(M - 64.0f * tf, -3.402823466e+38f);
 
-    // the smallest key above which there is less than the target: of tokens (by_mass false) or of mass
-    auto select = [&](bool by_mass, double share, unsigned long long count) {
-        for (uint32_t i = tid; i < n; i += kThreads) {
-            const float v = xs[i];
-            const uint32_t key = key_of(v);
-            const int b = bin_of(key, v);
-            if (b < 0 || key < low) continue;
-            if (!by_mass) {
-                atomicAdd(&sh.hist.lo[b], 1u);
-            } else {
-                const unsigned long long m = fixed(key);
-                const uint32_t l = (uint32_t)m, was = atomicAdd(&sh.hist.lo[b], l);
-                const uint32_t h = (uint32_t)(m >> 32) + (was + l < was);
-                if (h) atomicAdd(&sh.hist.hi[b], h);
-            }
-        }
+    // adds the other CTAs' histograms to the first one's
+    auto gather = [&]() {
         __syncthreads();
         if (rank != 0)
             for (uint32_t b = tid; b < kBins; b += kThreads) {
@@ -180,7 +185,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* _
                 if (h) atomicAdd(&lead->hist.hi[b], h);
             }
         cluster.sync();
-        if (rank == 0) {  // the crossing bin: a scan, four bins a thread
+    };
+    // The bin where the first CTA's histogram reaches the target (the count, or a share of the whole); kBins: nowhere.
+    auto cross = [&](bool by_mass, double share, unsigned long long count) {
+        if (rank == 0) {  // a scan, some bins a thread
             constexpr uint32_t kPer = kBins / kThreads;
             unsigned long long m[kPer], mine = 0;
 #pragma unroll
@@ -198,11 +206,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* _
             if (lane == 31) sh.ctl.scan[warp] = upto;
             if (tid == 0) sh.ctl.border = kBins;
             __syncthreads();
-            unsigned long long above = upto - mine, all = 0;
-            for (uint32_t w = 0; w < (uint32_t)kWarps; ++w) {
-                if (w < warp) above += sh.ctl.scan[w];
-                all += sh.ctl.scan[w];
+            unsigned long long sums = sh.ctl.scan[lane], upto_warp = sums;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned long long y = __shfl_up_sync(0xffffffffu, upto_warp, o);
+                if (lane >= (uint32_t)o) upto_warp += y;
             }
+            const unsigned long long all = __shfl_sync(0xffffffffu, upto_warp, 31);
+            unsigned long long above = upto - mine + __shfl_sync(0xffffffffu, upto_warp - sums, warp);
             // less than the target <=> below this whole number; the largest token always stays
             const unsigned long long target = by_mass ? (unsigned long long)fmax(ceil(share * (double)all), 1.0) : count;
 #pragma unroll
@@ -212,49 +223,95 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* _
             }
         }
         cluster.sync();
-        const int border = (int)lead->ctl.border;
+        return (int)lead->ctl.border;
+    };
+    // Over the list of the first CTA, for a token each: what `other(j, i)` adds over all j. A token is shared by as many lanes
+    // of a warp as the list leaves.
+    auto each_listed = [&](uint32_t listed, auto other, auto done) {
+        uint32_t parts = 32;
+        while (parts > 1 && listed * parts > kThreads) parts /= 2;
+        const uint32_t step = kThreads / parts;
+        for (uint32_t i0 = 0; i0 < listed; i0 += step) {  // the same turns for every thread of a warp
+            const uint32_t i = i0 + tid / parts;
+            unsigned long long count = 0, mass = 0;
+            if (i < listed)
+                for (uint32_t j = tid % parts; j < listed; j += parts) other(i, j, count, mass);
+            for (uint32_t o = parts / 2; o > 0; o /= 2) count += __shfl_xor_sync(0xffffffffu, count, o), mass += __shfl_xor_sync(0xffffffffu, mass, o);
+            if (i < listed && tid % parts == 0) done(i, count, mass);
+        }
+    };
+    auto clear_lists = [&]() {  // the histogram and the list share their memory
+        cluster.sync();
+        for (uint32_t i = tid; i < kBins; i += kThreads) sh.hist.lo[i] = sh.hist.hi[i] = 0;
+        if (tid == 0) sh.ctl.listed = 0, sh.ctl.range_lo = 0xffffffffu, sh.ctl.range_hi = 0;
+        cluster.sync();
+    };
+    // calls `take` with every logit of at least `bound`, four loads in flight
+    auto every = [&](float bound, auto take) {
+        uint32_t i = tid;
+        for (; i + 3 * kThreads < n; i += 4 * kThreads) {
+            const float v[4] = {logit(i), logit(i + kThreads), logit(i + 2 * kThreads), logit(i + 3 * kThreads)};
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+                if (v[j] >= bound) take(v[j], i + j * kThreads);
+        }
+        for (; i < n; i += kThreads) {
+            const float v = logit(i);
+            if (v >= bound) take(v, i);
+        }
+    };
+
+    // raises `low` to the smallest value above which there is less than the target: of tokens (by_mass false) or of mass
+    auto select = [&](bool by_mass, double share, unsigned long long count) {
+        every(low, [&](float v, uint32_t) {
+            const int b = bin_of(v);
+            if (!by_mass) {
+                atomicAdd(&sh.hist.lo[b], 1u);
+            } else {
+                const unsigned long long m = fixed(v);
+                const uint32_t l = (uint32_t)m, was = atomicAdd(&sh.hist.lo[b], l);
+                const uint32_t h = (uint32_t)(m >> 32) + (was + l < was);
+                if (h) atomicAdd(&sh.hist.hi[b], h);
+            }
+        });
+        gather();
+        const int border = cross(by_mass, share, count);
         if (border == (int)kBins) return;  // everything stays
         const unsigned long long above = lead->ctl.above, target = lead->ctl.target;
         uint32_t lo = 0xffffffffu, hi = 0;
-        for (uint32_t i = tid; i < n; i += kThreads) {
-            const float v = xs[i];
-            const uint32_t key = key_of(v);
-            if (key < low || bin_of(key, v) != border) continue;
+        every(low, [&](float v, uint32_t) {
+            if (bin_of(v) != border) return;
+            const uint32_t key = key_of(v), at = atomicAdd(&lead->ctl.listed, 1u);
             lo = min(lo, key), hi = max(hi, key);
-            const uint32_t at = atomicAdd(&lead->ctl.listed, 1u);
-            if (at < kList) lead->list.key[at] = key, lead->list.mass[at] = by_mass ? fixed(key) : 1ull;
-        }
+            if (at < kList) lead->list.key[at] = key, lead->list.mass[at] = by_mass ? fixed(v) : 1ull;
+        });
         lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi);
-        if (lane == 0) atomicMin(&lead->ctl.range_lo, lo), atomicMax(&lead->ctl.range_hi, hi);
+        if (lane == 0 && lo <= hi) atomicMin(&lead->ctl.range_lo, lo), atomicMax(&lead->ctl.range_hi, hi);
         cluster.sync();
         const uint32_t listed = lead->ctl.listed;
         lo = lead->ctl.range_lo, hi = lead->ctl.range_hi;
         if (listed <= kList) {
             if (rank == 0) {
-                uint32_t least = hi;
-                for (uint32_t i = tid; i < listed; i += kThreads) {
-                    const uint32_t key = sh.list.key[i];
-                    unsigned long long over = above;
-                    for (uint32_t j = 0; j < listed; ++j)
-                        if (sh.list.key[j] > key) over += sh.list.mass[j];
-                    if (over < target) least = min(least, key);
-                }
-                least = __reduce_min_sync(0xffffffffu, least);
                 if (tid == 0) sh.ctl.low = hi;
                 __syncthreads();
-                if (lane == 0) atomicMin(&sh.ctl.low, least);
+                each_listed(
+                    listed,
+                    [&](uint32_t i, uint32_t j, unsigned long long&, unsigned long long& mass) {
+                        if (sh.list.key[j] > sh.list.key[i]) mass += sh.list.mass[j];
+                    },
+                    [&](uint32_t i, unsigned long long, unsigned long long mass) {
+                        if (above + mass < target) atomicMin(&sh.ctl.low, sh.list.key[i]);
+                    });
             }
             cluster.sync();
-            low = lead->ctl.low;
+            low = value_of(lead->ctl.low);
         } else {
             for (uint32_t round = 0; lo < hi; ++round) {  // the same bounds in every thread of the cluster
                 const uint32_t mid = lo + (hi - lo) / 2;
                 unsigned long long over = 0;
-                for (uint32_t i = tid; i < n; i += kThreads) {
-                    const float v = xs[i];
-                    const uint32_t key = key_of(v);
-                    if (key > mid && key >= low && bin_of(key, v) == border) over += by_mass ? fixed(key) : 1ull;
-                }
+                every(low, [&](float v, uint32_t) {
+                    if (key_of(v) > mid && bin_of(v) == border) over += by_mass ? fixed(v) : 1ull;
+                });
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) over += __shfl_xor_sync(0xffffffffu, over, o);
                 if (lane == 0) sh.ctl.scan[warp] = over;
@@ -271,39 +328,113 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* _
                 else lo = mid + 1;
             }
             cluster.sync();  // the sums may still be read
-            low = lo;
+            low = value_of(lo);
         }
     };
-    if (!greedy) {
-        const int32_t k = top_k[row];
-        const float p = top_p[row];
-        const bool by_k = k > 0 && (uint32_t)k < vocab, by_p = p < 1.0f;
-        if (by_k) select(false, 0.0, (unsigned long long)k);
-        if (by_k && by_p) {  // the histogram and the list share their memory
-            cluster.sync();
-            for (uint32_t i = tid; i < kBins; i += kThreads) sh.hist.lo[i] = sh.hist.hi[i] = 0;
-            if (tid == 0) sh.ctl.listed = 0, sh.ctl.range_lo = 0xffffffffu, sh.ctl.range_hi = 0;
-            cluster.sync();
-        }
-        if (by_p) select(true, (double)p, 0);
-    }
-
-    // 4: the draw. A warp owns consecutive tokens.
     const double least = greedy ? 0.0 : (double)min_p[row];
+    const float p = greedy ? 1.0f : top_p[row];
+    const int32_t k = greedy ? 0 : top_k[row];
+    const bool by_k = k > 0 && (uint32_t)k < vocab, by_p = p < 1.0f;
+    if (by_k) {
+        // 2: at least k tokens lie in or above the bin where the threads' maxima reach k
+        if (most >= low) atomicAdd(&sh.hist.lo[bin_of(most)], 1u);
+        gather();
+        const int border = cross(false, 0.0, (unsigned long long)k);
+        if (border != (int)kBins) {
+            every(low, [&](float v, uint32_t i) {
+                if (bin_of(v) > border) return;
+                const uint32_t at = atomicAdd(&lead->ctl.listed, 1u);
+                if (at < kList) lead->list.key[at] = key_of(v), lead->list.at[at] = first + i, lead->list.mass[at] = fixed(v);
+            });
+            cluster.sync();
+            const uint32_t listed = lead->ctl.listed;
+            if (listed <= kList) {
+                if (rank == 0) {
+                    // what lies above a token, of all (counted) and of those top-k keeps
+                    if (tid == 0) sh.ctl.low = mk, sh.ctl.part[0] = sh.ctl.part[1] = 0, sh.ctl.pick = 0xffffffffu, sh.ctl.last = 0;
+                    __syncthreads();
+                    each_listed(
+                        listed, [&](uint32_t i, uint32_t j, unsigned long long& count, unsigned long long&) { count += sh.list.key[j] > sh.list.key[i]; },
+                        [&](uint32_t i, unsigned long long count, unsigned long long) {
+                            if (count < (unsigned long long)k) atomicMin(&sh.ctl.low, sh.list.key[i]), atomicAdd(&sh.ctl.part[0], sh.list.mass[i]);
+                        });
+                    __syncthreads();
+                    const uint32_t kth = sh.ctl.low;
+                    const unsigned long long target = by_p ? (unsigned long long)fmax(ceil((double)p * (double)sh.ctl.part[0]), 1.0) : ~0ull;
+                    // out of the list goes what top-k, top-p or min-p drop: its mass becomes 0 (no other's mass above it counts it)
+                    each_listed(
+                        listed,
+                        [&](uint32_t i, uint32_t j, unsigned long long&, unsigned long long& mass) {
+                            if (sh.list.key[j] > sh.list.key[i]) mass += sh.list.mass[j];
+                        },
+                        [&](uint32_t i, unsigned long long, unsigned long long mass) {
+                            const uint32_t key = sh.list.key[i];
+                            const bool keep = key == mk || (key >= kth && mass < target && weight(value_of(key)) >= least);
+                            if (keep) atomicAdd(&sh.ctl.part[1], sh.list.mass[i]);
+                            else sh.list.at[i] |= 0x80000000u;
+                        });
+                    __syncthreads();
+                    const unsigned long long total = sh.ctl.part[1];
+                    const double goal = (double)u * (double)total;
+                    each_listed(
+                        listed,
+                        [&](uint32_t i, uint32_t j, unsigned long long&, unsigned long long& mass) {  // (a dropped token's index is beyond all)
+                            if (sh.list.at[j] <= sh.list.at[i]) mass += sh.list.mass[j];
+                        },
+                        [&](uint32_t i, unsigned long long, unsigned long long mass) {
+                            const uint32_t at = sh.list.at[i];
+                            if (at >> 31 || sh.list.mass[i] == 0) return;
+                            if ((double)mass > goal) atomicMin(&sh.ctl.pick, at);
+                            atomicMax(&sh.ctl.last, at);
+                        });
+                    __syncthreads();
+                    const uint32_t chosen = sh.ctl.pick != 0xffffffffu ? sh.ctl.pick : sh.ctl.last;
+                    for (uint32_t i = tid; i < listed; i += kThreads)
+                        if (sh.list.at[i] == chosen) {
+                            tokens[row] = (int32_t)chosen;
+                            if (probs) probs[row] = (float)(weight(value_of(sh.list.key[i])) * kFixed / (double)total);
+                        }
+                }
+                cluster.sync();  // nobody leaves while its shared memory may be read
+                return;
+            }
+        }
+        // 3: more than k threads' worth, or more tokens beside the k-th than the list holds
+        clear_lists();
+        select(false, 0.0, (unsigned long long)k);
+        if (by_p) clear_lists();
+    }
+    if (by_p) select(true, (double)p, 0);
+
+    // 4: the draw. A thread owns `per` consecutive tokens, an odd number so that its warp's loads meet no bank conflicts.
+    // (min_p's own test is in float64; below `near` the weight is under it for certain)
+    const float near = least > 0.0 ? fmaxf(low, fminf(M + tf * (__logf((float)least) * 1.0001f - 0.001f) - fabsf(M) * 1e-6f, M)) : low;
     auto kept = [&](float v) -> double {
-        const uint32_t key = key_of(v);
-        if (key < low || bin_of(key, v) < 0) return 0.0;
-        const double w = weight(key, v);
-        return w >= least || key == mk ? w : 0.0;
+        const double w = weight(v);
+        return w >= least || v == M ? w : 0.0;
     };
-    const uint32_t span = (n + kThreads - 1) / kThreads * 32, w0 = min(warp * span, n), w1 = min(w0 + span, n);
+    const uint32_t per = ((n + kThreads - 1) / kThreads) | 1, t0 = min(tid * per, n), t1 = min(t0 + per, n);
     double sum = 0.0;
-    for (uint32_t i = w0 + lane; i < w1; i += 32) sum += kept(xs[i]);
+    {
+        uint32_t i = t0;
+        for (; i + 3 < t1; i += 4) {
+            const float v[4] = {logit(i), logit(i + 1), logit(i + 2), logit(i + 3)};
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) sh.ctl.warp_sum[warp] = sum;
+            for (int j = 0; j < 4; ++j)
+                if (v[j] >= near) sum += kept(v[j]);
+        }
+        for (; i < t1; ++i)
+            if (logit(i) >= near) sum += kept(logit(i));
+    }
+    double upto = sum;  // of the warp's threads, in order
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= (uint32_t)o) upto += y;
+    }
+    if (lane == 31) sh.ctl.warp_sum[warp] = upto;
     cluster.sync();
-    if (warp == 0) {  // every CTA finds the warp that holds the target: lane = four of the cluster's warps, in order
+    if (warp == 0) {  // every CTA finds the warp that holds the target: lane = some of the cluster's warps, in order
         constexpr uint32_t kPer = kMostCtas * kWarps / 32;
         double s[kPer], mine = 0.0;
 #pragma unroll
@@ -312,14 +443,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* _
             s[j] = w < ctas * kWarps ? cluster.map_shared_rank(&sh, w / kWarps)->ctl.warp_sum[w % kWarps] : 0.0;
             mine += s[j];
         }
-        double upto = mine;
+        double through = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const double y = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= (uint32_t)o) upto += y;
+            const double y = __shfl_up_sync(0xffffffffu, through, o);
+            if (lane >= (uint32_t)o) through += y;
         }
-        const double total = __shfl_sync(0xffffffffu, upto, 31), goal = greedy ? 0.0 : (double)u * total;
-        double before = __shfl_up_sync(0xffffffffu, upto, 1);
+        const double total = __shfl_sync(0xffffffffu, through, 31), goal = greedy ? 0.0 : (double)u * total;
+        double before = __shfl_up_sync(0xffffffffu, through, 1);
         if (lane == 0) before = 0.0;
         uint32_t hit = 0xffffffffu, last = 0;
         double hit_before = 0.0, last_before = 0.0;
@@ -338,27 +469,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* _
     }
     __syncthreads();
     if (sh.ctl.owner_warp == rank * kWarps + warp) {
-        const double goal = sh.ctl.goal;
-        double run = sh.ctl.before;
-        uint32_t chosen = 0;
-        double share = 0.0;
-        for (uint32_t i = w0; i < w1; i += 32) {
-            const double w = i + lane < w1 ? kept(xs[i + lane]) : 0.0;
-            const uint32_t some = __ballot_sync(0xffffffffu, w > 0.0);
-            if (!some) continue;
-            double upto = w;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= (uint32_t)o) upto += y;
+        // the first thread that passes the target, else the last that keeps anything; it walks its tokens
+        const double goal = sh.ctl.goal, before = sh.ctl.before;
+        const uint32_t over = __ballot_sync(0xffffffffu, sum > 0.0 && before + upto > goal), some = __ballot_sync(0xffffffffu, sum > 0.0);
+        const uint32_t owner = over ? __ffs(over) - 1 : 31 - __clz(some);
+        if (lane == owner) {
+            double run = before + (upto - sum), share = 0.0;
+            uint32_t chosen = 0;
+            for (uint32_t i = t0; i < t1; ++i) {
+                const float v = logit(i);
+                if (v < near) continue;
+                const double w = kept(v);
+                if (w == 0.0) continue;
+                chosen = i, share = w, run += w;  // the last one, should no more come
+                if (run > goal) break;
             }
-            const uint32_t over = __ballot_sync(0xffffffffu, w > 0.0 && run + upto > goal);
-            const int pick = over ? __ffs(over) - 1 : 31 - __clz(some);  // else the last one, should no more come
-            chosen = i + pick, share = __shfl_sync(0xffffffffu, w, pick);
-            if (over) break;
-            run += __shfl_sync(0xffffffffu, upto, 31);
-        }
-        if (lane == 0) {
             tokens[row] = (int32_t)(first + chosen);
             if (probs) probs[row] = (float)(share / sh.ctl.total);
         }
@@ -371,9 +496,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* _
 void launch_sample_rows(cudaStream_t s, int sm_count, const float* logits, uint32_t rows, uint32_t vocab, const float* temperature, const int32_t* top_k,
                         const float* top_p, const float* min_p, const float* uniforms, uint32_t uniform_rows, uint32_t* draws, int32_t* tokens, float* probs,
                         uint32_t* ticket) {
-    // CTAs of a row: as many as give each 4096 tokens while two CTAs an SM hold all rows, and what its shared memory needs
+    // CTAs of a row: as many as leave each some thousands of tokens while one CTA an SM holds all rows, and what its shared
+    // memory needs
     uint32_t ctas = 1;
-    while (ctas < kMostCtas && ((vocab / ctas >= 8192 && rows * ctas * 2 <= 2u * (uint32_t)sm_count) || (vocab + ctas - 1) / ctas > kStaged)) ctas *= 2;
+    while (ctas < kMostCtas && ((vocab / ctas >= 8192 && rows * ctas * 2 <= (uint32_t)sm_count) || (vocab + ctas - 1) / ctas > kStaged)) ctas *= 2;
     const uint32_t slice = ((vocab + ctas - 1) / ctas + 3) / 4 * 4, staged = slice <= kStaged;
     const size_t smem = sizeof(Shared) + (staged ? slice * 4 : 0);
     GQ_CUDA(cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
