@@ -54,7 +54,7 @@ struct Control {
     unsigned long long scan[kWarps];
 };
 struct alignas(16) Shared {  // the logits behind it are stored four at a time
-    double pow2[64];  // 2^(i / 64)
+    double pow2[8];  // 2^(i / 8)
     Control ctl;
     union {
         struct {
@@ -67,25 +67,26 @@ struct alignas(16) Shared {  // the logits behind it are stored four at a time
     };
 };
 
-// exp(y) for y <= 0: 2^(n / 64) from a table times the Taylor polynomial of the rest, |r| <= ln 2 / 128: r^6 / 720 < 2^-54
-__device__ __forceinline__ double exp_of(double y, const double* pow2) {
-    if (!(y > -700.0)) return 0.0;
-    const double t = __fma_rn(y, 92.332482616893656, 6755399441055744.0);  // 64 / ln 2; 1.5 * 2^52 rounds to a whole number
+// exp(d ln 2 / 8 step) for d <= 0, step = 8 / (T ln 2): 2^(n / 8) from a table of eight (small enough that the lanes' loads meet
+// no bank conflicts) times the Taylor polynomial of 2^(f / 8), |f| <= 1/2, whose next term is below 6e-14. The result keeps an
+// exponent above 2^-1022 for all that weighs more than e^-64.
+__device__ __forceinline__ double exp_of(double d, double step, const double* pow2) {
+    const double t = __fma_rn(d, step, 6755399441055744.0);  // 1.5 * 2^52 rounds to a whole number
     const int n = __double2loint(t);
-    const double nf = t - 6755399441055744.0;
-    // ln 2 / 64 in two parts, the first of 32 bits so that its product with n is exact
-    double r = __fma_rn(nf, -0x1.62e42feep-7, y);
-    r = __fma_rn(nf, -0x1.a39ef35793c76p-39, r);
-    double p = __fma_rn(r, 1.0 / 120.0, 1.0 / 24.0);
-    p = __fma_rn(p, r, 1.0 / 6.0);
-    p = __fma_rn(p, r, 0.5);
-    p = __fma_rn(p, r, 1.0);
-    p = __fma_rn(p, r, 1.0);
-    const double v = p * pow2[n & 63];
-    return __hiloint2double(__double2hiint(v) + ((n >> 6) << 20), __double2loint(v));
+    const double f = __fma_rn(d, step, -(t - 6755399441055744.0));
+    double p = __fma_rn(f, 5.87598052726044e-10, 4.069079024178602e-08);  // (ln 2 / 8)^k / k!
+    p = __fma_rn(p, f, 2.3481760516671086e-06);
+    p = __fma_rn(p, f, 0.00010840646223597965);
+    p = __fma_rn(p, f, 0.0037535391712359488);
+    p = __fma_rn(p, f, 0.08664339756999316);
+    p = __fma_rn(p, f, 1.0);
+    const double v = p * pow2[n & 7];
+    return __hiloint2double(__double2hiint(v) + ((n >> 3) << 20), __double2loint(v));
 }
 
-__global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* __restrict__ logits, uint32_t vocab, uint32_t slice, uint32_t staged,
+// STAGED: a CTA's logits fit its shared memory.
+template <bool STAGED>
+__global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* __restrict__ logits, uint32_t vocab, uint32_t slice,
                                                                  const float* __restrict__ temperature, const int32_t* __restrict__ top_k,
                                                                  const float* __restrict__ top_p, const float* __restrict__ min_p,
                                                                  const float* __restrict__ uniforms, uint32_t uniform_rows, uint32_t* draws, int32_t* tokens,
@@ -101,7 +102,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* _
     const float* x = logits + (size_t)row * vocab + first;
     Shared* lead = cluster.map_shared_rank(&sh, 0);
 
-    if (tid < 64) sh.pow2[tid] = exp2((double)tid / 64.0);
+    if (tid < 8) sh.pow2[tid] = exp2((double)tid / 8.0);
     for (uint32_t i = tid; i < kBins; i += kThreads) sh.hist.lo[i] = sh.hist.hi[i] = 0;
     const float u = uniforms[(size_t)(draws ? *draws % uniform_rows : 0u) * rows + row];
     if (tid == 0) sh.ctl.top[0] = 0, sh.ctl.top[1] = 0xffffffffu, sh.ctl.listed = 0, sh.ctl.range_lo = 0xffffffffu, sh.ctl.range_hi = 0;
@@ -118,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* _
         if (v != -INFINITY) least_seen = fminf(least_seen, v);
     };
     const uint32_t lead_in = min(n, (uint32_t)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / 4), quads = (n - lead_in) / 4;
-    if (staged) {
+    if (STAGED) {
         // (the part on 16-byte boundaries four at a time; in shared memory the logits lie one behind the other from 0 on)
         const float4* x4 = reinterpret_cast<const float4*>(x + lead_in);
 #pragma unroll 4
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* _
     } else {
         for (uint32_t i = tid; i < n; i += kThreads) see(clean(x[i]));
     }
-    auto logit = [&](uint32_t i) { return staged ? stage[i] : clean(x[i]); };
+    auto logit = [&](uint32_t i) { return STAGED ? stage[i] : clean(x[i]); };
     {
         const uint32_t mk = __reduce_max_sync(0xffffffffu, key_of(most)), lk = __reduce_min_sync(0xffffffffu, key_of(least_seen));
         if (lane == 0) atomicMax(&sh.ctl.top[0], mk), atomicMin(&sh.ctl.top[1], lk);
@@ -160,9 +161,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* _
         return;
     }
     const bool greedy = !(tf > 0.0f);
-    const double Md = (double)M, inv_t = greedy ? 0.0 : 1.0 / (double)tf;
+    const double Md = (double)M, step = greedy ? 0.0 : 11.541560327111707 / (double)tf;  // 8 / ln 2
     const float per_x = fmaxf(32.0f / tf, (float)(kBins - 1) / (M - value_of(lk)));
-    auto weight = [&](float v) { return v == M ? 1.0 : exp_of((widen(v) - Md) * inv_t, sh.pow2); };
+    auto weight = [&](float v) { return v == M ? 1.0 : exp_of(widen(v) - Md, step, sh.pow2); };  // of what is not below `low`
     auto fixed = [&](float v) {  // w 2^40 as a whole number, by the last place of 2^52
         return (unsigned long long)__double_as_longlong(__fma_rn(weight(v), kFixed, 4503599627370496.0)) & 0xfffffffffffffull;
     };
@@ -225,20 +226,34 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* _
         cluster.sync();
         return (int)lead->ctl.border;
     };
-    // Over the list of the first CTA, for a token each: what `other(j, i)` adds over all j. A token is shared by as many lanes
-    // of a warp as the list leaves.
+    // Over the list of the first CTA, for a token each: the sum of what `other(i, j)` gives over all j. A token is shared by a
+    // few lanes of a warp, so that each has some eight others to look at and few warps take part.
     auto each_listed = [&](uint32_t listed, auto other, auto done) {
-        uint32_t parts = 32;
-        while (parts > 1 && listed * parts > kThreads) parts /= 2;
-        const uint32_t step = kThreads / parts;
-        for (uint32_t i0 = 0; i0 < listed; i0 += step) {  // the same turns for every thread of a warp
-            const uint32_t i = i0 + tid / parts;
-            unsigned long long count = 0, mass = 0;
-            if (i < listed)
-                for (uint32_t j = tid % parts; j < listed; j += parts) other(i, j, count, mass);
-            for (uint32_t o = parts / 2; o > 0; o /= 2) count += __shfl_xor_sync(0xffffffffu, count, o), mass += __shfl_xor_sync(0xffffffffu, mass, o);
-            if (i < listed && tid % parts == 0) done(i, count, mass);
+        uint32_t bits = 0;
+        while (bits < 5 && (16u << bits) <= listed && (listed << (bits + 1)) <= (uint32_t)kThreads) ++bits;
+        const uint32_t part = tid & ((1u << bits) - 1);
+        for (uint32_t i0 = 0; i0 < listed; i0 += kThreads >> bits) {
+            const uint32_t i = i0 + (tid >> bits);
+            if (i - lane / (1u << bits) >= listed) break;  // the whole warp is behind the list
+            unsigned long long sum = 0;
+            if (i < listed) {
+#pragma unroll 4
+                for (uint32_t j = part; j < listed; j += 1u << bits) sum += other(i, j);
+            }
+            for (uint32_t o = 1u << bits >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (i < listed && part == 0) done(i, sum);
         }
+    };
+    auto block_sum = [&](unsigned long long v) {  // of the CTA's threads, the same for all
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == 0) sh.ctl.scan[warp] = v;
+        __syncthreads();
+        v = sh.ctl.scan[lane];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        __syncthreads();
+        return v;
     };
     auto clear_lists = [&]() {  // the histogram and the list share their memory
         cluster.sync();
@@ -246,40 +261,49 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* _
         if (tid == 0) sh.ctl.listed = 0, sh.ctl.range_lo = 0xffffffffu, sh.ctl.range_hi = 0;
         cluster.sync();
     };
-    // calls `take` with every logit of at least `bound`, four loads in flight
+    // calls `take` with every logit of at least `bound`, eight loads in flight
     auto every = [&](float bound, auto take) {
-        uint32_t i = tid;
-        for (; i + 3 * kThreads < n; i += 4 * kThreads) {
-            const float v[4] = {logit(i), logit(i + kThreads), logit(i + 2 * kThreads), logit(i + 3 * kThreads)};
+        constexpr uint32_t kAtOnce = 8;
+        for (uint32_t i = tid; i < n; i += kAtOnce * kThreads) {
+            float v[kAtOnce];
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j)
+            for (uint32_t j = 0; j < kAtOnce; ++j) v[j] = i + j * kThreads < n ? logit(i + j * kThreads) : -INFINITY;
+#pragma unroll
+            for (uint32_t j = 0; j < kAtOnce; ++j)
                 if (v[j] >= bound) take(v[j], i + j * kThreads);
-        }
-        for (; i < n; i += kThreads) {
-            const float v = logit(i);
-            if (v >= bound) take(v, i);
         }
     };
 
     // raises `low` to the smallest value above which there is less than the target: of tokens (by_mass false) or of mass
     auto select = [&](bool by_mass, double share, unsigned long long count) {
-        every(low, [&](float v, uint32_t) {
-            const int b = bin_of(v);
-            if (!by_mass) {
-                atomicAdd(&sh.hist.lo[b], 1u);
-            } else {
-                const unsigned long long m = fixed(v);
-                const uint32_t l = (uint32_t)m, was = atomicAdd(&sh.hist.lo[b], l);
-                const uint32_t h = (uint32_t)(m >> 32) + (was + l < was);
-                if (h) atomicAdd(&sh.hist.hi[b], h);
+        if (!by_mass) {
+            every(low, [&](float v, uint32_t) { atomicAdd(&sh.hist.lo[bin_of(v)], 1u); });
+        } else {
+            // (the exponentials of four tokens side by side: one is a chain of fourteen float64 operations)
+            constexpr uint32_t kAtOnce = 4;
+            for (uint32_t i = tid; i < n; i += kAtOnce * kThreads) {
+                float v[kAtOnce];
+                unsigned long long m[kAtOnce];
+#pragma unroll
+                for (uint32_t j = 0; j < kAtOnce; ++j) v[j] = i + j * kThreads < n ? logit(i + j * kThreads) : -INFINITY;
+#pragma unroll
+                for (uint32_t j = 0; j < kAtOnce; ++j) m[j] = fixed(v[j]);
+#pragma unroll
+                for (uint32_t j = 0; j < kAtOnce; ++j) {
+                    if (v[j] < low) continue;
+                    const int b = bin_of(v[j]);
+                    const uint32_t l = (uint32_t)m[j], was = atomicAdd(&sh.hist.lo[b], l);
+                    const uint32_t h = (uint32_t)(m[j] >> 32) + (was + l < was);
+                    if (h) atomicAdd(&sh.hist.hi[b], h);
+                }
             }
-        });
+        }
         gather();
         const int border = cross(by_mass, share, count);
         if (border == (int)kBins) return;  // everything stays
         const unsigned long long above = lead->ctl.above, target = lead->ctl.target;
         uint32_t lo = 0xffffffffu, hi = 0;
-        every(low, [&](float v, uint32_t) {
+        every(fmaxf(low, M - ((float)border + 1.0f) / per_x), [&](float v, uint32_t) {
             if (bin_of(v) != border) return;
             const uint32_t key = key_of(v), at = atomicAdd(&lead->ctl.listed, 1u);
             lo = min(lo, key), hi = max(hi, key);
@@ -296,10 +320,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* _
                 __syncthreads();
                 each_listed(
                     listed,
-                    [&](uint32_t i, uint32_t j, unsigned long long&, unsigned long long& mass) {
-                        if (sh.list.key[j] > sh.list.key[i]) mass += sh.list.mass[j];
-                    },
-                    [&](uint32_t i, unsigned long long, unsigned long long mass) {
+                    [&](uint32_t i, uint32_t j) { return sh.list.key[j] > sh.list.key[i] ? sh.list.mass[j] : 0ull; },
+                    [&](uint32_t i, unsigned long long mass) {
                         if (above + mass < target) atomicMin(&sh.ctl.low, sh.list.key[i]);
                     });
             }
@@ -312,15 +334,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* _
                 every(low, [&](float v, uint32_t) {
                     if (key_of(v) > mid && bin_of(v) == border) over += by_mass ? fixed(v) : 1ull;
                 });
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) over += __shfl_xor_sync(0xffffffffu, over, o);
-                if (lane == 0) sh.ctl.scan[warp] = over;
-                __syncthreads();
-                if (tid == 0) {
-                    unsigned long long sum = 0;
-                    for (int w = 0; w < kWarps; ++w) sum += sh.ctl.scan[w];
-                    sh.ctl.part[round & 1] = sum;
-                }
+                over = block_sum(over);
+                if (tid == 0) sh.ctl.part[round & 1] = over;
                 cluster.sync();
                 unsigned long long sum = above;
                 for (uint32_t c = 0; c < ctas; ++c) sum += cluster.map_shared_rank(&sh, c)->ctl.part[round & 1];
@@ -341,7 +356,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* _
         gather();
         const int border = cross(false, 0.0, (unsigned long long)k);
         if (border != (int)kBins) {
-            every(low, [&](float v, uint32_t i) {
+            // (no value below this is in such a bin, whatever its rounding)
+            every(fmaxf(low, M - ((float)border + 1.0f) / per_x), [&](float v, uint32_t i) {
                 if (bin_of(v) > border) return;
                 const uint32_t at = atomicAdd(&lead->ctl.listed, 1u);
                 if (at < kList) lead->list.key[at] = key_of(v), lead->list.at[at] = first + i, lead->list.mass[at] = fixed(v);
@@ -351,37 +367,36 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* _
             if (listed <= kList) {
                 if (rank == 0) {
                     // what lies above a token, of all (counted) and of those top-k keeps
-                    if (tid == 0) sh.ctl.low = mk, sh.ctl.part[0] = sh.ctl.part[1] = 0, sh.ctl.pick = 0xffffffffu, sh.ctl.last = 0;
+                    if (tid == 0) sh.ctl.low = mk, sh.ctl.pick = 0xffffffffu, sh.ctl.last = 0;
                     __syncthreads();
+                    unsigned long long kept_mass = 0;  // of this thread's tokens
                     each_listed(
-                        listed, [&](uint32_t i, uint32_t j, unsigned long long& count, unsigned long long&) { count += sh.list.key[j] > sh.list.key[i]; },
-                        [&](uint32_t i, unsigned long long count, unsigned long long) {
-                            if (count < (unsigned long long)k) atomicMin(&sh.ctl.low, sh.list.key[i]), atomicAdd(&sh.ctl.part[0], sh.list.mass[i]);
+                        listed, [&](uint32_t i, uint32_t j) { return sh.list.key[j] > sh.list.key[i] ? 1ull : 0ull; },
+                        [&](uint32_t i, unsigned long long count) {
+                            if (count < (unsigned long long)k) atomicMin(&sh.ctl.low, sh.list.key[i]), kept_mass += sh.list.mass[i];
                         });
-                    __syncthreads();
+                    const unsigned long long of_k = block_sum(kept_mass);
                     const uint32_t kth = sh.ctl.low;
-                    const unsigned long long target = by_p ? (unsigned long long)fmax(ceil((double)p * (double)sh.ctl.part[0]), 1.0) : ~0ull;
+                    const unsigned long long target = by_p ? (unsigned long long)fmax(ceil((double)p * (double)of_k), 1.0) : ~0ull;
+                    kept_mass = 0;
                     // out of the list goes what top-k, top-p or min-p drop: its mass becomes 0 (no other's mass above it counts it)
                     each_listed(
                         listed,
-                        [&](uint32_t i, uint32_t j, unsigned long long&, unsigned long long& mass) {
-                            if (sh.list.key[j] > sh.list.key[i]) mass += sh.list.mass[j];
-                        },
-                        [&](uint32_t i, unsigned long long, unsigned long long mass) {
+                        [&](uint32_t i, uint32_t j) { return sh.list.key[j] > sh.list.key[i] ? sh.list.mass[j] : 0ull; },
+                        [&](uint32_t i, unsigned long long mass) {
                             const uint32_t key = sh.list.key[i];
                             const bool keep = key == mk || (key >= kth && mass < target && weight(value_of(key)) >= least);
-                            if (keep) atomicAdd(&sh.ctl.part[1], sh.list.mass[i]);
+                            if (keep) kept_mass += sh.list.mass[i];
                             else sh.list.at[i] |= 0x80000000u;
                         });
-                    __syncthreads();
-                    const unsigned long long total = sh.ctl.part[1];
+                    const unsigned long long total = block_sum(kept_mass);
                     const double goal = (double)u * (double)total;
                     each_listed(
                         listed,
-                        [&](uint32_t i, uint32_t j, unsigned long long&, unsigned long long& mass) {  // (a dropped token's index is beyond all)
-                            if (sh.list.at[j] <= sh.list.at[i]) mass += sh.list.mass[j];
+                        [&](uint32_t i, uint32_t j) {  // (a dropped token's index is beyond all)
+                            return sh.list.at[j] <= sh.list.at[i] ? sh.list.mass[j] : 0ull;
                         },
-                        [&](uint32_t i, unsigned long long, unsigned long long mass) {
+                        [&](uint32_t i, unsigned long long mass) {
                             const uint32_t at = sh.list.at[i];
                             if (at >> 31 || sh.list.mass[i] == 0) return;
                             if ((double)mass > goal) atomicMin(&sh.ctl.pick, at);
@@ -415,16 +430,13 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* _
     };
     const uint32_t per = ((n + kThreads - 1) / kThreads) | 1, t0 = min(tid * per, n), t1 = min(t0 + per, n);
     double sum = 0.0;
-    {
-        uint32_t i = t0;
-        for (; i + 3 < t1; i += 4) {
-            const float v[4] = {logit(i), logit(i + 1), logit(i + 2), logit(i + 3)};
+    for (uint32_t i = t0; i < t1; i += 8) {
+        float v[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (v[j] >= near) sum += kept(v[j]);
-        }
-        for (; i < t1; ++i)
-            if (logit(i) >= near) sum += kept(logit(i));
+        for (uint32_t j = 0; j < 8; ++j) v[j] = i + j < t1 ? logit(i + j) : -INFINITY;
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j)
+            if (v[j] >= near) sum += kept(v[j]);
     }
     double upto = sum;  // of the warp's threads, in order
 #pragma unroll
@@ -502,7 +514,8 @@ void launch_sample_rows(cudaStream_t s, int sm_count, const float* logits, uint3
     while (ctas < kMostCtas && ((vocab / ctas >= 8192 && rows * ctas * 2 <= (uint32_t)sm_count) || (vocab + ctas - 1) / ctas > kStaged)) ctas *= 2;
     const uint32_t slice = ((vocab + ctas - 1) / ctas + 3) / 4 * 4, staged = slice <= kStaged;
     const size_t smem = sizeof(Shared) + (staged ? slice * 4 : 0);
-    GQ_CUDA(cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    auto kernel = staged ? sample_rows_kernel<true> : sample_rows_kernel<false>;
+    GQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(rows * ctas), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem, cfg.stream = s;
     cudaLaunchAttribute attr[2]{};
@@ -511,7 +524,7 @@ void launch_sample_rows(cudaStream_t s, int sm_count, const float* logits, uint3
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = ctas, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr, cfg.numAttrs = 2;
-    GQ_CUDA(cudaLaunchKernelEx(&cfg, sample_rows_kernel, logits, vocab, slice, staged, temperature, top_k, top_p, min_p, uniforms, uniform_rows, draws,
+    GQ_CUDA(cudaLaunchKernelEx(&cfg, kernel, logits, vocab, slice, temperature, top_k, top_p, min_p, uniforms, uniform_rows, draws,
                                tokens, probs, ticket));
 }
 
