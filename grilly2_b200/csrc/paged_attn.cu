@@ -45,16 +45,17 @@ template <int RP, int WG, int DIM>
 struct Split {
     static constexpr int kRows = RP / WG;                                        // rows of a thread
     static constexpr int kSoft = 128 * WG, kThreads = kSoft + 64;                // softmax threads; all
-    static constexpr uint32_t kN = RP == 8 ? 32 : 3 * RP;                        // columns: a multiple of 16; digit d of row r in column d RP + r
-    static constexpr uint32_t kCols = RP == 8 ? 32 : RP == 16 ? 64 : RP == 32 ? 128 : 256;  // S at column 0, D at kCols
+    static constexpr uint32_t kN = (3 * RP + 15) / 16 * 16;                      // columns: digit d of row r in column d RP + r
+    static constexpr uint32_t kCols = kN <= 32 ? 32 : kN <= 64 ? 64 : 128;       // S at column 0, D at kCols
     static constexpr uint32_t kM = DIM == 128 ? 128 : 64;                        // lanes of D: dim, at least 64
     static constexpr uint32_t kTileBytes = kKeys * DIM, kStageBytes = 2 * kTileBytes;
-    static constexpr uint32_t kStages = DIM == 128 ? (RP == 64 ? 3 : 2) : DIM == 64 ? 3 : 4;
+    static constexpr uint32_t kStages = DIM == 128 ? 2 : DIM == 64 ? 3 : 4;
     // (dim 32: the 64 lanes of D read 32 rows that are not there, up to 4 KB behind the last stage; nobody reads the sums)
     static constexpr uint32_t kQAt = kStages * kStageBytes + (DIM == 32 ? 4096 : 0);
     static constexpr uint32_t kPAt = kQAt + kN * DIM, kMiscAt = kPAt + kN * kKeys;
-    // rows' arrays: scale, last position seen, [4] sums, [2][4] maxima, [4] factor, reference and correction of each warp
-    static constexpr uint32_t kSmem = kMiscAt + 1024 + RP * 4 * (1 + 1 + 4 + 8 + 12);
+    // blocks' scales of each stage; rows' arrays: scale, last position seen, [4] sums, [2][4] maxima, [4] raw maximum or factor,
+    // reference and correction of each warp
+    static constexpr uint32_t kSmem = kMiscAt + 1024 + kStages * 128 + RP * 4 * (1 + 1 + 4 + 8 + 12);
     // CTAs of an SM: what shared memory and tensor memory hold
     static constexpr uint32_t kBySmem = (227 * 1024) / (kSmem + 1024), kByTmem = 512 / (2 * kCols), kHeld = kBySmem < kByTmem ? kBySmem : kByTmem;
     static constexpr uint32_t kMost = RP == 16 ? 3 : kMostPerSm;  // (registers)
@@ -95,6 +96,17 @@ __device__ __forceinline__ float factor_of(float row, float key) {
 __device__ __forceinline__ float join(uint32_t d0, uint32_t d1, uint32_t d2) {
     const float high = __int_as_float((int)d2 + 0x4b400000) - 12582912.0f;
     return __fmaf_rn(high, 65536.0f, (float)((int)d0 + ((int)d1 << 8)));
+}
+
+__device__ __forceinline__ void tmem_ld4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// What the softmax needs to know of a block: x = its key scale; y = log2 of its value scale (of at least 2^-100) and a margin for the
+// rounding, so that P stays below 2^23; z = the value scale times 2^23; w = 0, 1 where a scale is none (negative, beyond 2^100 or
+// no number; x is 1 then), 2 where there is no block.
+__device__ __forceinline__ float4 block_scale(float ks, float vs) {
+    const bool good = vs >= 0.0f && vs <= 1.2676506e30f && ks >= 0.0f && ks <= 3.0e38f;
+    return make_float4(good ? ks : 1.0f, fmaxf(__log2f(vs), -100.0f) + 0.001f, vs * kMagic, good ? 0.0f : 1.0f);
 }
 
 // sum of floor((a i + b) / m) for i < n, by Euclid's steps on (a, m); the divisions in 32 bits where the numbers allow (a
@@ -209,18 +221,18 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
     uint32_t* arrived = tmem_slot + 1;
     volatile uint32_t* failed = arrived + 1;
     Segment* segments = reinterpret_cast<Segment*>(misc + 512);   // [kSegments]
-    float2* warp_scales = reinterpret_cast<float2*>(misc + 768);  // [2][WG][4] a warp's key scale and log2 of its value scale
-    float* row_scale = reinterpret_cast<float*>(misc + 1024);   // [RP] scale of a row's Q, times log2 e
+    float4* block_scales = reinterpret_cast<float4*>(misc + 1024);  // [kStages][8] what block_scale() gives
+    float* row_scale = reinterpret_cast<float*>(misc + 1024 + T::kStages * 128);  // [RP] scale of a row's Q, times log2 e
     int* row_seen = reinterpret_cast<int*>(row_scale + RP);     // [RP] the last position it sees
     float* lsum = reinterpret_cast<float*>(row_seen + RP);      // [4][RP]
-    float* exchange = lsum + 4 * RP;                            // [2][4][RP] warps' maxima
+    float* exchange = lsum + 4 * RP;                            // [2][RP][4] warps' maxima
     float* refs = exchange + 8 * RP;                            // [4][RP] the rows' references (negative), a copy per warp
     float* corrs = refs + 4 * RP;                               // [4][RP] what older sums are multiplied by
-    float* factors = corrs + 4 * RP;                            // [4][RP] a row's scale times the warp's key scale
+    float* factors = corrs + 4 * RP;                            // [4][RP] a warp's raw maxima, then the row's scale times the warp's key scale
 
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = heads / c.kv_heads;
     if (tid == 0) {
-        for (uint32_t i = 0; i < T::kStages; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
+        for (uint32_t i = 0; i < T::kStages; ++i) mbar_init(full + i, 2), mbar_init(empty + i, 1);
         for (uint32_t i = 0; i < kSegments; ++i) mbar_init(seg_full + i, 1), mbar_init(seg_free + i, T::kSoft + 1);
         mbar_init(s_full, 1), mbar_init(s_read, T::kSoft), mbar_init(p_full, T::kSoft), mbar_init(d_full, 1), mbar_init(q_full, T::kSoft);
         *failed = 0;
@@ -290,7 +302,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
             }
         }
         uint32_t st = 0, round = 0;
-        const uint32_t per_tile = kKeys >> c.shift, bytes = c.block * DIM;
+        const uint32_t per_tile = kKeys >> c.shift, bytes = c.block * DIM;  // (at most max_blocks blocks hold the keys)
         for (uint32_t seg = 0; ok; ++seg) {
             Segment g;
             const bool more = walk.next(c, s, g);
@@ -303,10 +315,16 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
             }
             if (!more) break;
             const int32_t* table = c.table + (size_t)g.b * c.max_blocks;
+            auto entry = [&](uint32_t t) {  // one lane per block
+                const uint32_t j = t * per_tile + lane;
+                const int32_t e = t < g.t1 && lane < per_tile && (j << c.shift) < g.keys ? table[j] : -1;
+                return e >= 0 && (uint32_t)e < c.blocks ? e : -1;
+            };
+            int32_t e = entry(g.t0);
             for (uint32_t t = g.t0; t < g.t1; ++t) {
-                const uint32_t j = t * per_tile + lane;  // one lane per block
-                int32_t e = lane < per_tile && j < c.max_blocks && (j << c.shift) < g.keys ? table[j] : -1;
-                if (e < 0 || (uint32_t)e >= c.blocks) e = -1;
+                const int32_t e_next = entry(t + 1);
+                const size_t at = ((size_t)max(e, 0) * c.kv_heads + g.head);
+                const float ks = e >= 0 ? c.kscale[at] : 0.0f, vs = e >= 0 ? c.vscale[at] : 0.0f;
                 if (round) ok = ok && mbar_wait(empty + st, (round - 1) & 1, failed, status, kStatusEmptyWaitTimedOut);
                 const uint32_t held = __popc(__ballot_sync(0xffffffffu, e >= 0));
                 if (__ballot_sync(0xffffffffu, !ok)) ok = false;
@@ -314,11 +332,14 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                 if (lane == 0) mbar_arrive_expect_tx(full + st, held * 2 * bytes);
                 __syncwarp();
                 if (e >= 0) {
-                    const size_t at = ((size_t)e * c.kv_heads + g.head) * bytes;
                     uint8_t* dst = smem + st * T::kStageBytes + lane * bytes;
-                    bulk_load(dst, c.k + at, bytes, full + st);
-                    bulk_load(dst + T::kTileBytes, c.v + at, bytes, full + st);
+                    bulk_load(dst, c.k + at * bytes, bytes, full + st);
+                    bulk_load(dst + T::kTileBytes, c.v + at * bytes, bytes, full + st);
                 }
+                if (lane < per_tile) block_scales[st * 8 + lane] = e >= 0 ? block_scale(ks, vs) : make_float4(1.0f, -100.0f, 0.0f, 2.0f);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full + st);
+                e = e_next;
                 if (++st == T::kStages) st = 0, ++round;
             }
         }
@@ -378,7 +399,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
             }
         }
     } else {
-        constexpr int kChunk = 8;
+        constexpr int kChunk = 8;  // (and a last one of four, for 20 rows)
         const uint32_t quarter = warp & 3, wg = warp >> 2, key = tid & 127, wrow = wg * R;  // this thread's key, its first row
         const uint32_t comp = T::kM == 128 ? key : 16 * quarter + lane;                    // the component of D on its lane
         const bool owner = T::kM == 128 || (lane < 16 && comp < (uint32_t)DIM);
@@ -388,19 +409,29 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
         float* const my_refs = refs + quarter * RP + wrow;
         float* const my_corrs = corrs + quarter * RP + wrow;
         float* const my_factors = factors + quarter * RP + wrow;
-        uint32_t tile = 0;
+        uint32_t tile = 0, st = 0, round = 0;
         float O[R], l[R];
         auto drain = [&](uint32_t of_tile) {
             ok = ok && mbar_wait(d_full, of_tile & 1, failed, status, kStatusMmaWaitTimedOut);
             tc_fence_after_sync();
 #pragma unroll
             for (int r0 = 0; r0 < R; r0 += kChunk) {
-                uint32_t d0[kChunk], d1[kChunk], d2[kChunk];
                 const uint32_t at = tmem_addr(tmem, 32 * quarter, T::kCols + wrow + r0);
-                tmem_ld8(at, d0), tmem_ld8(at + RP, d1), tmem_ld8(at + 2 * RP, d2);
-                tmem_wait_ld();
+                if (R - r0 >= kChunk) {
+                    uint32_t d0[8], d1[8], d2[8];
+                    tmem_ld8(at, d0), tmem_ld8(at + RP, d1), tmem_ld8(at + 2 * RP, d2);
+                    tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < kChunk; ++i) O[r0 + i] += join(d0[i], d1[i], d2[i]);
+                    for (int i = 0; i < 8; ++i)
+                        if (r0 + i < R) O[r0 + i] += join(d0[i], d1[i], d2[i]);
+                } else {
+                    uint32_t d0[4], d1[4], d2[4];
+                    tmem_ld4(at, d0), tmem_ld4(at + RP, d1), tmem_ld4(at + 2 * RP, d2);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (r0 + i < R) O[r0 + i] += join(d0[i], d1[i], d2[i]);
+                }
             }
         };
         for (uint32_t seg = 0;; ++seg) {
@@ -461,56 +492,47 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
 #pragma unroll
             for (int r = 0; r < R; ++r) O[r] = l[r] = 0.0f;
             float M = kNone;  // the reference of row `lane`
-            const int32_t* table = c.table + (size_t)g.b * c.max_blocks;
-            auto entry = [&](uint32_t t) {
-                const uint32_t j = (t * kKeys + key) >> c.shift;  // (a key behind the last one has its block's scale)
-                const int32_t e = t < t1 && (j << c.shift) < g.keys ? table[j] : -1;
-                return e >= 0 && (uint32_t)e < c.blocks ? e : -1;
-            };
-            auto scales = [&](int32_t e) {
-                if (e < 0) return make_float2(0.0f, 0.0f);  // no such block
-                const size_t at = (size_t)e * c.kv_heads + g.head;
-                const float ks = c.kscale[at], vs = c.vscale[at];
-                // what is no scale makes the key's score no number
-                return make_float2(vs >= 0.0f && vs <= 1.2676506e30f && ks >= 0.0f && ks <= 3.0e38f ? ks : __uint_as_float(0x7fc00000u), vs);
-            };
-            int32_t e = entry(t0), e_next = entry(t0 + 1);
-            float2 sc = scales(e);
             const float my_scale = lane < (uint32_t)R ? row_scale[wrow + lane] : 0.0f;  // of row `lane`
             for (uint32_t t = t0; t < t1; ++t, ++tile) {
-                const float2 sc_next = scales(e_next);
-                const int32_t e_then = entry(t + 2);
-                // log2 of the value scale and a margin for its rounding, so that P stays below 2^23
-                const float lv = fmaxf(__log2f(sc.y), -100.0f) + 0.001f;
+                ok = ok && mbar_wait(full + st, round & 1, failed, status, kStatusFullWaitTimedOut);
+                const float4 sc = block_scales[st * 8 + (key >> c.shift)];
+                if (++st == T::kStages) st = 0, ++round;
                 ok = ok && mbar_wait(s_full, tile & 1, failed, status, kStatusMmaWaitTimedOut);
                 tc_fence_after_sync();
                 float a[R];  // q . k in units of the row's and the key's scales
 #pragma unroll
                 for (int r0 = 0; r0 < R; r0 += kChunk) {
-                    uint32_t d0[kChunk], d1[kChunk], d2[kChunk];
                     const uint32_t at = tmem_addr(tmem, 32 * quarter, wrow + r0);
-                    tmem_ld8(at, d0), tmem_ld8(at + RP, d1), tmem_ld8(at + 2 * RP, d2);
-                    tmem_wait_ld();
+                    if (R - r0 >= kChunk) {
+                        uint32_t d0[8], d1[8], d2[8];
+                        tmem_ld8(at, d0), tmem_ld8(at + RP, d1), tmem_ld8(at + 2 * RP, d2);
+                        tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < kChunk; ++i) a[r0 + i] = join(d0[i], d1[i], d2[i]);
+                        for (int i = 0; i < 8; ++i)
+                            if (r0 + i < R) a[r0 + i] = join(d0[i], d1[i], d2[i]);
+                    } else {
+                        uint32_t d0[4], d1[4], d2[4];
+                        tmem_ld4(at, d0), tmem_ld4(at + RP, d1), tmem_ld4(at + 2 * RP, d2);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (r0 + i < R) a[r0 + i] = join(d0[i], d1[i], d2[i]);
+                    }
                 }
                 tc_fence_before_sync();
                 mbar_arrive(s_read);
                 // Where some row does not see some key, or a scale is none: a key out of sight scores -inf, and a row that sees a
-                // key without a scale has no sum. (The scales themselves are then finite, so that -inf stays -inf.)
-                const bool bad = !(sc.x >= 0.0f);
-                if ((t + 1) * kKeys > clear_keys || __any_sync(0xffffffffu, e < 0 || bad)) {
-                    const int pos = e < 0 ? 0x7fffffff : (int)(t * kKeys + key);
+                // key without a scale has no sum. (The factors are finite and not 0, so that -inf stays -inf.)
+                if ((t + 1) * kKeys > clear_keys || __any_sync(0xffffffffu, sc.w != 0.0f)) {
+                    const int pos = sc.w == 2.0f ? 0x7fffffff : (int)(t * kKeys + key);
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
                         const bool seen = pos <= row_seen[wrow + r];
                         if (!seen) a[r] = kNone;
-                        else if (bad) l[r] = __uint_as_float(0x7fc00000u);
+                        else if (sc.w != 0.0f) l[r] = __uint_as_float(0x7fc00000u);
                     }
                 }
-                const float ks = bad ? 1.0f : sc.x;
-                float* ex = exchange + (tile & 1) * 4 * RP + wrow;
-                float2* ws = warp_scales + (tile & 1) * 4 * WG + wg * 4;
+                float* ex = exchange + ((tile & 1) * RP + wrow) * 4;
 #pragma unroll
                 for (int r = 0; r < R; r += 4) {
                     float m[4];
@@ -518,23 +540,22 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                     if (!ONE) rs = *reinterpret_cast<const float4*>(row_scale + wrow + r);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        m[i] = warp_max(ONE ? a[r + i] : __fmaf_rn(a[r + i], factor_of(i == 0 ? rs.x : i == 1 ? rs.y : i == 2 ? rs.z : rs.w, ks), lv));
-                    if (lane == 0) *reinterpret_cast<float4*>(ex + quarter * RP + r) = make_float4(m[0], m[1], m[2], m[3]);
+                        m[i] = warp_max(ONE ? a[r + i] : __fmaf_rn(a[r + i], factor_of(i == 0 ? rs.x : i == 1 ? rs.y : i == 2 ? rs.z : rs.w, sc.x), sc.y));
+                    if (lane == 0) *reinterpret_cast<float4*>(my_factors + r) = make_float4(m[0], m[1], m[2], m[3]);
                 }
-                if (ONE && lane == 0) ws[quarter] = make_float2(ks, lv);
+                __syncwarp();
+                if (lane < (uint32_t)R) {
+                    const float raw = my_factors[lane], f = factor_of(my_scale, sc.x);
+                    ex[lane * 4 + quarter] = ONE ? __fmaf_rn(raw, f, sc.y) : raw;
+                    if (ONE) my_factors[lane] = f;
+                }
                 if (t > t0) drain(tile - 1);
                 named_barrier_sync(1 + wg, 128);
                 bool moved = false;
                 if (lane < (uint32_t)R) {
-                    float top = M;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const float m = ex[w * RP + lane];
-                        top = fmaxf(top, ONE ? __fmaf_rn(m, factor_of(my_scale, ws[w].x), ws[w].y) : m);
-                    }
-                    const float ref = top == kNone ? 0.0f : top, corr = exp2_fast(M - ref);
+                    const float4 m = *reinterpret_cast<const float4*>(ex + lane * 4);
+                    const float top = fmaxf(fmaxf(fmaxf(M, m.x), fmaxf(m.y, m.z)), m.w), ref = top == kNone ? 0.0f : top, corr = exp2_fast(M - ref);
                     my_refs[lane] = -ref, my_corrs[lane] = corr;
-                    if (ONE) my_factors[lane] = factor_of(my_scale, ks);
                     moved = corr != 1.0f;
                     M = top;
                 }
@@ -549,7 +570,6 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                             l[r] *= cr.x, l[r + 1] *= cr.y, l[r + 2] *= cr.z, l[r + 3] *= cr.w;
                         }
                 }
-                const float vz = sc.y * kMagic;
 #pragma unroll
                 for (int r = 0; r < R; r += 4) {
                     const float4 rf = *reinterpret_cast<const float4*>(my_refs + r);
@@ -558,10 +578,10 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float f = i == 0 ? fc.x : i == 1 ? fc.y : i == 2 ? fc.z : fc.w, ref = i == 0 ? rf.x : i == 1 ? rf.y : i == 2 ? rf.z : rf.w;
-                        const float p = exp2_fast(__fmaf_rn(a[r + i], ONE ? f : factor_of(f, ks), ref));
+                        const float p = exp2_fast(__fmaf_rn(a[r + i], ONE ? f : factor_of(f, sc.x), ref));
                         l[r + i] += p;
                         // rint(p vscale 2^23) in the low 23 bits (the last place of 2^23 is 1)
-                        x[i] = __float_as_uint(fminf(__fmaf_rn(p, vz, kMagic), 16777215.0f));
+                        x[i] = __float_as_uint(fminf(__fmaf_rn(p, sc.z, kMagic), 16777215.0f));
                     }
                     // digit d of the four rows, one row to a byte
                     const uint32_t y0 = __byte_perm(x[0], x[1], 0x5140), y1 = __byte_perm(x[2], x[3], 0x5140);
@@ -578,7 +598,6 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                 fence_proxy_async_smem();
                 tc_fence_before_sync();
                 mbar_arrive(p_full);
-                sc = sc_next, e = e_next, e_next = e_then;
             }
             if (t0 < t1) drain(tile - 1);
             // the rows' sums over the keys, in a fixed order
@@ -693,8 +712,7 @@ void launch_blocks(cudaStream_t s, int sm_count, uint32_t* status, const PagedVi
                    uint64_t rows, float* out, void* state, void* scratch) {
     if (rows <= 8) launch_rows<8, 1, ONE>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
     else if (rows <= 16) launch_rows<16, 1, ONE>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
-    else if (rows <= 32) launch_rows<32, 2, ONE>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
-    else launch_rows<64, 4, ONE>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+    else launch_rows<40, 2, ONE>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
 }
 
 }  // namespace

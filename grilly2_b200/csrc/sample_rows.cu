@@ -25,10 +25,10 @@ namespace gq {
 
 namespace {
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr uint32_t kBins = 2048, kList = 2048, kMostCtas = 8;
 constexpr double kFixed = 1099511627776.0;  // 2^40
-constexpr uint32_t kStaged = 46 * 1024;     // logits of a row that a CTA keeps at most
+constexpr uint32_t kStaged = 19 * 1024;     // logits of a row that a CTA keeps at most: two CTAs an SM
 
 __device__ __forceinline__ uint32_t key_of(float f) {  // a < b as floats <=> key_of(a) < key_of(b)
     const uint32_t b = __float_as_uint(f);
@@ -86,7 +86,7 @@ __device__ __forceinline__ double exp_of(double d, double step, const double* po
 
 // STAGED: a CTA's logits fit its shared memory.
 template <bool STAGED>
-__global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* __restrict__ logits, uint32_t vocab, uint32_t slice,
+__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* __restrict__ logits, uint32_t vocab, uint32_t slice,
                                                                  const float* __restrict__ temperature, const int32_t* __restrict__ top_k,
                                                                  const float* __restrict__ top_p, const float* __restrict__ min_p,
                                                                  const float* __restrict__ uniforms, uint32_t uniform_rows, uint32_t* draws, int32_t* tokens,
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* _
             if (lane == 31) sh.ctl.scan[warp] = upto;
             if (tid == 0) sh.ctl.border = kBins;
             __syncthreads();
-            unsigned long long sums = sh.ctl.scan[lane], upto_warp = sums;
+            unsigned long long sums = lane < kWarps ? sh.ctl.scan[lane] : 0ull, upto_warp = sums;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const unsigned long long y = __shfl_up_sync(0xffffffffu, upto_warp, o);
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* _
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         if (lane == 0) sh.ctl.scan[warp] = v;
         __syncthreads();
-        v = sh.ctl.scan[lane];
+        v = lane < kWarps ? sh.ctl.scan[lane] : 0ull;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         __syncthreads();
@@ -508,10 +508,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const float* _
 void launch_sample_rows(cudaStream_t s, int sm_count, const float* logits, uint32_t rows, uint32_t vocab, const float* temperature, const int32_t* top_k,
                         const float* top_p, const float* min_p, const float* uniforms, uint32_t uniform_rows, uint32_t* draws, int32_t* tokens, float* probs,
                         uint32_t* ticket) {
-    // CTAs of a row: as many as leave each some thousands of tokens while one CTA an SM holds all rows, and what its shared
-    // memory needs
+    // CTAs of a row: as many as leave each some thousands of tokens while the CTAs an SM holds (two) hold all rows, and as
+    // many as keep the row in shared memory. (1024 threads and one CTA an SM: 14.6 us for one row of 151936 against 13.6, 49 for
+    // 200 rows of 32003 against 43, 77 for 64 rows of 151936 against 84.)
     uint32_t ctas = 1;
-    while (ctas < kMostCtas && ((vocab / ctas >= 8192 && rows * ctas * 2 <= (uint32_t)sm_count) || (vocab + ctas - 1) / ctas > kStaged)) ctas *= 2;
+    while (ctas < kMostCtas && ((vocab / ctas >= 8192 && rows * ctas <= (uint32_t)sm_count) || (vocab + ctas - 1) / ctas > kStaged)) ctas *= 2;
     const uint32_t slice = ((vocab + ctas - 1) / ctas + 3) / 4 * 4, staged = slice <= kStaged;
     const size_t smem = sizeof(Shared) + (staged ? slice * 4 : 0);
     auto kernel = staged ? sample_rows_kernel<true> : sample_rows_kernel<false>;
