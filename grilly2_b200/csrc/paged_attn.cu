@@ -8,10 +8,12 @@
 // meets them is held as an exact fixed-point integer in three base-256 digits, so three products in int32 and one join
 // give a float32 result:
 //   q_r = 2^(e_r - 22) Q, Q in signed digits; kscale_j is a factor of a lane;
-//   w vscale = 2^-23 P, P in unsigned digits. The value scales are folded into P because the sum over j runs across blocks;
-//     so that P fits, the running maximum is the one of s + log2 vscale (the largest contribution, not the largest score) and
-//     P's steps are 2^-23 of the largest contribution so far, whatever the blocks' scales are. The denominator sums the w
-//     themselves in float32.
+//   w vscale = 2^-22 P, P in unsigned digits. The value scales are folded into P because the sum over j runs across blocks;
+//     so that P fits, the reference of a row is the running maximum of s + log2 vscale (the largest contribution, not the largest
+//     score) and P's steps are 2^-22 of the largest contribution so far, whatever the blocks' scales are. The denominator
+//     sums the w themselves in float32. The reference stays until it is passed by a factor of 2: as long as no row of a warpgroup
+//     passes it D goes on adding up in int32, and is read, joined and added to the float32 sums only when one does (or
+//     after 256 tiles, before a sum could leave 32 bits).
 // A warp's 32 keys share one block and so one scale (blocks of 32 and more): the maximum is taken over the joined integers
 // and scaled afterwards, and the exponent is one multiplication and addition of the integer.
 // Scales of values from 2^-100 to 2^100 (and 0) are exact; larger, negative or non-finite ones read as NaN.
@@ -40,12 +42,13 @@ constexpr uint32_t kKeys = 128;    // keys of a tile
 constexpr float kNone = -INFINITY;
 constexpr uint32_t kMostPerSm = 4;  // CTAs of an SM
 constexpr float kMagic = 8388608.0f;  // 2^23: x + 2^23 has rint(x) in its low 23 bits
+constexpr float kUnit = 4194304.0f;   // 2^22: P's steps of the reference
 
 template <int RP, int WG, int DIM>
 struct Split {
     static constexpr int kRows = RP / WG;                                        // rows of a thread
     static constexpr int kSoft = 128 * WG, kThreads = kSoft + 64;                // softmax threads; all
-    static constexpr uint32_t kN = (3 * RP + 15) / 16 * 16;                      // columns: digit d of row r in column d RP + r
+    static constexpr uint32_t kNw = (3 * kRows + 15) / 16 * 16, kN = WG * kNw;   // columns: digit d of a warpgroup's row r in its column d kRows + r
     static constexpr uint32_t kCols = kN <= 32 ? 32 : kN <= 64 ? 64 : 128;       // S at column 0, D at kCols
     static constexpr uint32_t kM = DIM == 128 ? 128 : 64;                        // lanes of D: dim, at least 64
     static constexpr uint32_t kTileBytes = kKeys * DIM, kStageBytes = 2 * kTileBytes;
@@ -98,15 +101,12 @@ __device__ __forceinline__ float join(uint32_t d0, uint32_t d1, uint32_t d2) {
     return __fmaf_rn(high, 65536.0f, (float)((int)d0 + ((int)d1 << 8)));
 }
 
-__device__ __forceinline__ void tmem_ld4(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
 // What the softmax needs to know of a block: x = its key scale; y = log2 of its value scale (of at least 2^-100) and a margin for the
-// rounding, so that P stays below 2^23; z = the value scale times 2^23; w = 0, 1 where a scale is none (negative, beyond 2^100 or
+// rounding, so that P stays below 2^23; z = the value scale times 2^22; w = 0, 1 where a scale is none (negative, beyond 2^100 or
 // no number; x is 1 then), 2 where there is no block.
 __device__ __forceinline__ float4 block_scale(float ks, float vs) {
     const bool good = vs >= 0.0f && vs <= 1.2676506e30f && ks >= 0.0f && ks <= 3.0e38f;
-    return make_float4(good ? ks : 1.0f, fmaxf(__log2f(vs), -100.0f) + 0.001f, vs * kMagic, good ? 0.0f : 1.0f);
+    return make_float4(good ? ks : 1.0f, fmaxf(__log2f(vs), -100.0f) + 0.001f, vs * kUnit, good ? 0.0f : 1.0f);
 }
 
 // sum of floor((a i + b) / m) for i < n, by Euclid's steps on (a, m); the divisions in 32 bits where the numbers allow (a
@@ -208,9 +208,9 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
     uint64_t* empty = full + 4;                          // [kStages] its products are complete
     uint64_t* s_full = empty + 4;                        // S is complete
     uint64_t* s_read = s_full + 1;                       // S is read
-    uint64_t* p_full = s_read + 1;                       // P is written, the D before is read
-    uint64_t* d_full = p_full + 1;                       // D is complete
-    uint64_t* q_full = d_full + 1;                       // Q is written
+    uint64_t* p_full = s_read + 1;                       // [2] a warpgroup's P is written
+    uint64_t* d_full = p_full + 2;                       // [2] its D is complete
+    uint64_t* q_full = d_full + 2;                       // Q is written
     uint64_t* seg_full = q_full + 1;                     // [kSegments] a segment is written
     uint64_t* seg_free = seg_full + kSegments;           // [kSegments] ... and done with
     uint64_t* scan = seg_free + kSegments;               // [24]
@@ -220,6 +220,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
     uint32_t* tmem_slot = found_qt + 1;
     uint32_t* arrived = tmem_slot + 1;
     volatile uint32_t* failed = arrived + 1;
+    volatile uint32_t* go_on = arrived + 2;              // [2] whether a warpgroup's D goes on adding up
     Segment* segments = reinterpret_cast<Segment*>(misc + 512);   // [kSegments]
     float4* block_scales = reinterpret_cast<float4*>(misc + 1024);  // [kStages][8] what block_scale() gives
     float* row_scale = reinterpret_cast<float*>(misc + 1024 + T::kStages * 128);  // [RP] scale of a row's Q, times log2 e
@@ -234,7 +235,8 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
     if (tid == 0) {
         for (uint32_t i = 0; i < T::kStages; ++i) mbar_init(full + i, 2), mbar_init(empty + i, 1);
         for (uint32_t i = 0; i < kSegments; ++i) mbar_init(seg_full + i, 1), mbar_init(seg_free + i, T::kSoft + 1);
-        mbar_init(s_full, 1), mbar_init(s_read, T::kSoft), mbar_init(p_full, T::kSoft), mbar_init(d_full, 1), mbar_init(q_full, T::kSoft);
+        for (uint32_t i = 0; i < WG; ++i) mbar_init(p_full + i, 128), mbar_init(d_full + i, 1);
+        mbar_init(s_full, 1), mbar_init(s_read, T::kSoft), mbar_init(q_full, T::kSoft);
         *failed = 0;
         mbar_fence_init();
     }
@@ -354,7 +356,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
     } else if (warp == 4 * WG) {
         if (lane == 0) {
             constexpr uint32_t s_desc = umma_idesc(2, 1, 1, kKeys, T::kN);  // s32 sums, s8 codes x s8 digits of q
-            constexpr uint32_t d_desc = umma_idesc(2, 1, 0, T::kM, T::kN);  // s32 sums, s8 codes x u8 digits of P
+            constexpr uint32_t d_desc = umma_idesc(2, 1, 0, T::kM, T::kNw);  // s32 sums, s8 codes x u8 digits of P
             const uint32_t q_addr = smem_u32(smem + T::kQAt), p_addr = smem_u32(smem + T::kPAt);
             uint32_t st = 0, round = 0, tile = 0;
             auto score = [&](uint32_t stage, uint32_t parity) {  // S of the tile in `stage`
@@ -381,58 +383,55 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                     if (++st == T::kStages) st = 0, ++round;
                     ok = mbar_wait(s_read, tile & 1, failed, status, kStatusMmaWaitTimedOut);
                     if (t + 1 < tiles) score(st, round & 1);  // while the tile's weights are computed
-                    ok = ok && mbar_wait(p_full, tile & 1, failed, status, kStatusMmaWaitTimedOut);
-                    if (!ok) break;
-                    tc_fence_after_sync();
                     const uint32_t v_addr = smem_u32(smem + here * T::kStageBytes) + T::kTileBytes;
 #pragma unroll
-                    for (uint32_t i = 0; i < kKeys / 32; ++i) {
-                        // keys 32 i ..: two core matrices of one block, or (blocks of 16) of two
-                        const uint32_t k0 = 32 * i, at = (k0 >> c.shift) * c.block * DIM + (k0 & (c.block - 1)) * 8;
-                        const uint32_t step = c.shift == 4 ? 16 * DIM : 128;
-                        umma_i8_ss(tmem + T::kCols, umma_desc_plain(v_addr + at, step, 8 * c.block), umma_desc_plain(p_addr + 256 * i, 128, 8 * kKeys),
-                                   d_desc, i != 0);
+                    for (uint32_t w = 0; w < WG; ++w) {
+                        ok = ok && mbar_wait(p_full + w, tile & 1, failed, status, kStatusMmaWaitTimedOut);
+                        if (!ok) break;
+                        tc_fence_after_sync();
+                        const bool more = go_on[w] != 0;
+#pragma unroll
+                        for (uint32_t i = 0; i < kKeys / 32; ++i) {
+                            // keys 32 i ..: two core matrices of one block, or (blocks of 16) of two
+                            const uint32_t k0 = 32 * i, at = (k0 >> c.shift) * c.block * DIM + (k0 & (c.block - 1)) * 8;
+                            const uint32_t step = c.shift == 4 ? 16 * DIM : 128;
+                            umma_i8_ss(tmem + T::kCols + w * T::kNw, umma_desc_plain(v_addr + at, step, 8 * c.block),
+                                       umma_desc_plain(p_addr + w * T::kNw * kKeys + 256 * i, 128, 8 * kKeys), d_desc, i != 0 || more);
+                        }
+                        umma_commit(d_full + w);
                     }
-                    umma_commit(d_full);
+                    if (!ok) break;
                     umma_commit(empty + here);
                 }
             }
         }
     } else {
-        constexpr int kChunk = 8;  // (and a last one of four, for 20 rows)
         const uint32_t quarter = warp & 3, wg = warp >> 2, key = tid & 127, wrow = wg * R;  // this thread's key, its first row
         const uint32_t comp = T::kM == 128 ? key : 16 * quarter + lane;                    // the component of D on its lane
         const bool owner = T::kM == 128 || (lane < 16 && comp < (uint32_t)DIM);
         // a 4 x 4 transposition of bytes between lanes: which bytes a lane keeps in its two steps
         const uint32_t sel1 = lane & 1 ? 0x3715u : 0x6240u, sel2 = lane & 2 ? 0x3276u : 0x5410u;
-        uint8_t* const p_at = smem + T::kPAt + (2 * quarter + (lane >> 4)) * 128 + (lane & 3) * 16 + ((lane >> 2) & 3) * 4;
+        uint8_t* const p_at = smem + T::kPAt + wg * T::kNw * kKeys + (2 * quarter + (lane >> 4)) * 128 + (lane & 3) * 16 + ((lane >> 2) & 3) * 4;
         float* const my_refs = refs + quarter * RP + wrow;
         float* const my_corrs = corrs + quarter * RP + wrow;
         float* const my_factors = factors + quarter * RP + wrow;
         uint32_t tile = 0, st = 0, round = 0;
         float O[R], l[R];
-        auto drain = [&](uint32_t of_tile) {
-            ok = ok && mbar_wait(d_full, of_tile & 1, failed, status, kStatusMmaWaitTimedOut);
+        auto products = [&](uint32_t of_tile) {  // D of the tile is complete, P may be written
+            ok = ok && mbar_wait(d_full + wg, of_tile & 1, failed, status, kStatusMmaWaitTimedOut);
+        };
+        auto drain = [&]() {  // adds D to the float32 sums
             tc_fence_after_sync();
 #pragma unroll
-            for (int r0 = 0; r0 < R; r0 += kChunk) {
-                const uint32_t at = tmem_addr(tmem, 32 * quarter, T::kCols + wrow + r0);
-                if (R - r0 >= kChunk) {
-                    uint32_t d0[8], d1[8], d2[8];
-                    tmem_ld8(at, d0), tmem_ld8(at + RP, d1), tmem_ld8(at + 2 * RP, d2);
-                    tmem_wait_ld();
+            for (int r0 = 0; r0 < R; r0 += 8) {
+                uint32_t d0[8], d1[8], d2[8];
+                const uint32_t at = tmem_addr(tmem, 32 * quarter, T::kCols + wg * T::kNw + r0);
+                tmem_ld8(at, d0), tmem_ld8(at + R, d1), tmem_ld8(at + 2 * R, d2);
+                tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (r0 + i < R) O[r0 + i] += join(d0[i], d1[i], d2[i]);
-                } else {
-                    uint32_t d0[4], d1[4], d2[4];
-                    tmem_ld4(at, d0), tmem_ld4(at + RP, d1), tmem_ld4(at + 2 * RP, d2);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (r0 + i < R) O[r0 + i] += join(d0[i], d1[i], d2[i]);
-                }
+                for (int i = 0; i < 8; ++i) O[r0 + i] = __fmaf_rn((float)(int)d2[i], 65536.0f, __fmaf_rn((float)(int)d1[i], 256.0f, O[r0 + i] + (float)(int)d0[i]));
             }
+            tc_fence_before_sync();
         };
         for (uint32_t seg = 0;; ++seg) {
             ok = ok && mbar_wait(seg_full + seg % kSegments, (seg / kSegments) & 1, failed, status, kStatusMmaWaitTimedOut);
@@ -479,9 +478,10 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                         w0 |= ((uint32_t)d0 & 0xffu) << (8 * j), w1 |= ((uint32_t)d1 & 0xffu) << (8 * j), w2 |= ((uint32_t)d2 & 0xffu) << (8 * j);
                     }
                     uint8_t* qd = smem + T::kQAt;
-                    *reinterpret_cast<uint32_t*>(qd + key_at(DIM, r, d)) = w0;
-                    *reinterpret_cast<uint32_t*>(qd + key_at(DIM, RP + r, d)) = w1;
-                    *reinterpret_cast<uint32_t*>(qd + key_at(DIM, 2 * RP + r, d)) = w2;
+                    const uint32_t n = r / R * T::kNw + r % R;
+                    *reinterpret_cast<uint32_t*>(qd + key_at(DIM, n, d)) = w0;
+                    *reinterpret_cast<uint32_t*>(qd + key_at(DIM, n + R, d)) = w1;
+                    *reinterpret_cast<uint32_t*>(qd + key_at(DIM, n + 2 * R, d)) = w2;
                 }
             }
             named_barrier_sync(8, T::kSoft);  // row_scale, row_seen
@@ -492,6 +492,9 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
 #pragma unroll
             for (int r = 0; r < R; ++r) O[r] = l[r] = 0.0f;
             float M = kNone;  // the reference of row `lane`
+            uint32_t since = 0;  // tiles in D
+            if (lane < (uint32_t)R) my_refs[lane] = 0.0f;  // (of a row that sees no key)
+            __syncwarp();
             const float my_scale = lane < (uint32_t)R ? row_scale[wrow + lane] : 0.0f;  // of row `lane`
             for (uint32_t t = t0; t < t1; ++t, ++tile) {
                 ok = ok && mbar_wait(full + st, round & 1, failed, status, kStatusFullWaitTimedOut);
@@ -501,23 +504,13 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                 tc_fence_after_sync();
                 float a[R];  // q . k in units of the row's and the key's scales
 #pragma unroll
-                for (int r0 = 0; r0 < R; r0 += kChunk) {
-                    const uint32_t at = tmem_addr(tmem, 32 * quarter, wrow + r0);
-                    if (R - r0 >= kChunk) {
-                        uint32_t d0[8], d1[8], d2[8];
-                        tmem_ld8(at, d0), tmem_ld8(at + RP, d1), tmem_ld8(at + 2 * RP, d2);
-                        tmem_wait_ld();
+                for (int r0 = 0; r0 < R; r0 += 8) {
+                    uint32_t d0[8], d1[8], d2[8];
+                    const uint32_t at = tmem_addr(tmem, 32 * quarter, wg * T::kNw + r0);
+                    tmem_ld8(at, d0), tmem_ld8(at + R, d1), tmem_ld8(at + 2 * R, d2);
+                    tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (r0 + i < R) a[r0 + i] = join(d0[i], d1[i], d2[i]);
-                    } else {
-                        uint32_t d0[4], d1[4], d2[4];
-                        tmem_ld4(at, d0), tmem_ld4(at + RP, d1), tmem_ld4(at + 2 * RP, d2);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (r0 + i < R) a[r0 + i] = join(d0[i], d1[i], d2[i]);
-                    }
+                    for (int i = 0; i < 8; ++i) a[r0 + i] = join(d0[i], d1[i], d2[i]);
                 }
                 tc_fence_before_sync();
                 mbar_arrive(s_read);
@@ -549,18 +542,27 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                     ex[lane * 4 + quarter] = ONE ? __fmaf_rn(raw, f, sc.y) : raw;
                     if (ONE) my_factors[lane] = f;
                 }
-                if (t > t0) drain(tile - 1);
                 named_barrier_sync(1 + wg, 128);
                 bool moved = false;
                 if (lane < (uint32_t)R) {
                     const float4 m = *reinterpret_cast<const float4*>(ex + lane * 4);
-                    const float top = fmaxf(fmaxf(fmaxf(M, m.x), fmaxf(m.y, m.z)), m.w), ref = top == kNone ? 0.0f : top, corr = exp2_fast(M - ref);
-                    my_refs[lane] = -ref, my_corrs[lane] = corr;
-                    moved = corr != 1.0f;
-                    M = top;
+                    const float top = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));
+                    moved = top > M + 1.0f;  // (-inf passes nothing, anything passes -inf)
+                    if (moved) {
+                        my_refs[lane] = -top, my_corrs[lane] = exp2_fast(M - top);
+                        M = top;
+                    } else {
+                        my_corrs[lane] = 1.0f;
+                    }
                 }
                 __syncwarp();
+                // the same in all four warps of the warpgroup
                 const uint32_t rows_moved = __ballot_sync(0xffffffffu, moved);
+                const bool more = t > t0 && !rows_moved && since < 255;
+                if (t > t0) products(tile - 1);
+                if (t > t0 && !more) drain();
+                since = more ? since + 1 : 0;
+                if (key == 0) go_on[wg] = more;
                 if (rows_moved) {
 #pragma unroll
                     for (int r = 0; r < R; r += 4)
@@ -580,7 +582,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                         const float f = i == 0 ? fc.x : i == 1 ? fc.y : i == 2 ? fc.z : fc.w, ref = i == 0 ? rf.x : i == 1 ? rf.y : i == 2 ? rf.z : rf.w;
                         const float p = exp2_fast(__fmaf_rn(a[r + i], ONE ? f : factor_of(f, sc.x), ref));
                         l[r + i] += p;
-                        // rint(p vscale 2^23) in the low 23 bits (the last place of 2^23 is 1)
+                        // rint(p vscale 2^22) in the low 23 bits (the last place of 2^23 is 1)
                         x[i] = __float_as_uint(fminf(__fmaf_rn(p, sc.z, kMagic), 16777215.0f));
                     }
                     // digit d of the four rows, one row to a byte
@@ -591,15 +593,15 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                     for (uint32_t d = 0; d < 3; ++d) {  // ... becomes row r + lane % 4 of four lanes' keys, one key to a byte
                         w[d] = __byte_perm(w[d], __shfl_xor_sync(0xffffffffu, w[d], 1), sel1);
                         w[d] = __byte_perm(w[d], __shfl_xor_sync(0xffffffffu, w[d], 2), sel2);
-                        const uint32_t n = d * RP + wrow + r;
+                        const uint32_t n = d * R + r;
                         *reinterpret_cast<uint32_t*>(p_at + (n >> 3) * 8 * kKeys + (n & 7) * 16) = w[d];
                     }
                 }
                 fence_proxy_async_smem();
                 tc_fence_before_sync();
-                mbar_arrive(p_full);
+                mbar_arrive(p_full + wg);
             }
-            if (t0 < t1) drain(tile - 1);
+            if (t0 < t1) products(tile - 1), drain();
             // the rows' sums over the keys, in a fixed order
 #pragma unroll
             for (int r = 0; r < R; ++r) {
@@ -611,7 +613,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
             named_barrier_sync(8, T::kSoft);
             auto sum_of = [&](uint32_t r) { return (lsum[r] + lsum[RP + r]) + (lsum[2 * RP + r] + lsum[3 * RP + r]); };
             // a row that saw no key has neither sum and gives zeros
-            auto share_of = [](float sum) { return sum == 0.0f ? 0.0f : __fdiv_rn(1.0f / kMagic, sum); };
+            auto share_of = [](float sum) { return sum == 0.0f ? 0.0f : __fdiv_rn(1.0f / kUnit, sum); };
             if (g.whole) {
                 // the rows' factors and places, once each (the arrays of the tile loop are free)
                 if (tid < RP) {
@@ -712,7 +714,7 @@ void launch_blocks(cudaStream_t s, int sm_count, uint32_t* status, const PagedVi
                    uint64_t rows, float* out, void* state, void* scratch) {
     if (rows <= 8) launch_rows<8, 1, ONE>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
     else if (rows <= 16) launch_rows<16, 1, ONE>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
-    else launch_rows<40, 2, ONE>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
+    else launch_rows<32, 2, ONE>(s, sm_count, status, c, st, q, heads, scale, out, state, scratch);
 }
 
 }  // namespace
