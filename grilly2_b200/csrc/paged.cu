@@ -20,8 +20,9 @@ namespace gq {
 
 namespace {
 
-constexpr int kPlanThreads = 1024;
+constexpr uint32_t kPlanThreads = 1024, kPlanFew = 256;  // of a CTA; where requests and rows are few (its barriers cost less)
 constexpr uint32_t kPlanCluster = 8;
+constexpr uint32_t kAtOnce = 4;  // runs of a thread whose loads are in flight together
 
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -29,6 +30,7 @@ __device__ __forceinline__ void cluster_barrier() {
 }
 
 // Exclusive scan of one value per thread of the CTA, sums saturating at `cap` (which keeps them in 32 bits); *total is the sum.
+template <uint32_t NT>
 __device__ uint32_t block_scan(uint32_t v, uint32_t cap, uint32_t* warp_sums, uint32_t* total) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t x = v;
@@ -41,7 +43,7 @@ __device__ uint32_t block_scan(uint32_t v, uint32_t cap, uint32_t* warp_sums, ui
     if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
     if (warp == 0) {
-        uint32_t s = lane < kPlanThreads / 32 ? warp_sums[lane] : 0u;
+        uint32_t s = lane < NT / 32 ? warp_sums[lane] : 0u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t y = __shfl_up_sync(0xffffffffu, s, o);
@@ -50,24 +52,22 @@ __device__ uint32_t block_scan(uint32_t v, uint32_t cap, uint32_t* warp_sums, ui
         warp_sums[lane] = s;
     }
     __syncthreads();
-    *total = warp_sums[kPlanThreads / 32 - 1];
+    *total = warp_sums[NT / 32 - 1];
     const uint32_t before = warp ? warp_sums[warp - 1] : 0u;
     const uint32_t left = __shfl_up_sync(0xffffffffu, x, 1);
     return lane ? min(before + left, cap) : before;
 }
 
-// the request that owns item i: the last b with at[b] <= i, at ascending
-__device__ __forceinline__ uint32_t owner_of(const uint32_t* at, uint32_t n, uint32_t i) {
-    uint32_t lo = 0, hi = n;  // at[lo] <= i < at[hi]
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (at[mid] <= i) lo = mid;
-        else hi = mid;
-    }
-    return lo;
+// The request that owns an item: the last b >= from with at[b] <= item, at ascending and at[from] <= item.
+__device__ __forceinline__ uint32_t owner_of(const uint32_t* at, uint32_t n, uint32_t item, uint32_t from = 0) {
+    uint32_t b = from;
+    for (uint32_t step = n - from > 1 ? 1u << (31 - __clz(n - from - 1)) : 0; step > 0; step >>= 1)
+        if (b + step < n && at[b + step] <= item) b += step;
+    return b;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedView c, StepView s, const int32_t* __restrict__ counts,
+template <uint32_t NT>
+__global__ void __launch_bounds__(NT) paged_plan_kernel(PagedView c, StepView s, const int32_t* __restrict__ counts,
                                                                  const int32_t* __restrict__ free_list, int32_t* free_count) {
     GQ_GRID_DEP_SYNC();
     extern __shared__ uint32_t smem[];
@@ -75,10 +75,10 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedView c, S
     uint32_t* start = smem;                  // [seqs + 1]
     uint32_t* run = start + c.seqs + 1;      // [seqs + 1]
     uint32_t* len = run + c.seqs + 1;        // [seqs]
-    const uint32_t tid = threadIdx.x, per = (c.seqs + kPlanThreads - 1) / kPlanThreads, b0 = tid * per, b1 = min(b0 + per, c.seqs);
+    const uint32_t tid = threadIdx.x, per = (c.seqs + NT - 1) / NT, b0 = tid * per, b1 = min(b0 + per, c.seqs);
     uint32_t total, runs, sum = 0;
     for (uint32_t b = b0; b < b1; ++b) sum = min(sum + min((uint32_t)max(counts[b], 0), s.tokens), s.tokens);
-    uint32_t at = block_scan(sum, s.tokens, warp_sums, &total);
+    uint32_t at = block_scan<NT>(sum, s.tokens, warp_sums, &total);
     sum = 0;
     for (uint32_t b = b0; b < b1; ++b) {
         const uint32_t next = min(at + min((uint32_t)max(counts[b], 0), s.tokens), s.tokens), n = paged_len(c, b);
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedView c, S
         at = next;
     }
     if (tid == 0) start[c.seqs] = total;
-    at = block_scan(sum, s.runs_cap, warp_sums, &runs);  // (its barriers publish start and len)
+    at = block_scan<NT>(sum, s.runs_cap, warp_sums, &runs);  // (its barriers publish start and len)
     for (uint32_t b = b0; b < b1; ++b) {
         run[b] = at;
         const uint32_t rows = start[b + 1] - start[b];
@@ -100,22 +100,37 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedView c, S
         // the runs, and a block for every touched entry that has none
         const uint32_t have = (uint32_t)min(max(*free_count, 0), (int32_t)c.blocks);
         uint32_t wanted = 0;
-        for (uint32_t r0 = 0; r0 < runs; r0 += kPlanThreads) {
-            const uint32_t r = r0 + tid;
-            int32_t* entry = nullptr;
-            bool need = false;
-            if (r < runs) {
-                const uint32_t b = owner_of(run, c.seqs, r), j = (len[b] >> c.shift) + (r - run[b]);
-                s.runs[r] = (int32_t)(r == run[b] ? start[b] : start[b] + ((j << c.shift) - len[b]));
-                if (j < c.max_blocks) entry = c.table + (size_t)b * c.max_blocks + j, need = *entry < 0;
+        for (uint32_t r0 = 0; r0 < runs; r0 += kAtOnce * NT) {
+            int32_t* entry[kAtOnce];
+            uint32_t need = 0, packed_lo = 0, packed_hi = 0;  // four counts of 16 bits, one for each slab of NT runs
+#pragma unroll
+            for (uint32_t k = 0; k < kAtOnce; ++k) {
+                const uint32_t r = r0 + k * NT + tid;
+                entry[k] = nullptr;
+                if (r < runs) {
+                    const uint32_t b = owner_of(run, c.seqs, r), j = (len[b] >> c.shift) + (r - run[b]);
+                    s.runs[r] = (int32_t)(r == run[b] ? start[b] : start[b] + ((j << c.shift) - len[b]));
+                    if (j < c.max_blocks) entry[k] = c.table + (size_t)b * c.max_blocks + j;
+                }
             }
-            uint32_t here;
-            const uint32_t rank = wanted + block_scan(need ? 1u : 0u, 0x7fffffffu, warp_sums, &here);
-            if (need && rank < have) *entry = free_list[have - 1 - rank];
-            wanted += here;
+#pragma unroll
+            for (uint32_t k = 0; k < kAtOnce; ++k)
+                if (entry[k] && *entry[k] < 0) need |= 1u << k;
+            packed_lo = (need & 1) | (need & 2) << 15, packed_hi = (need >> 2 & 1) | (need & 8) << 13;
+            uint32_t all_lo, all_hi = 0, before_hi = 0;
+            const uint32_t before_lo = block_scan<NT>(packed_lo, 0xffffffffu, warp_sums, &all_lo);
+            if (r0 + 2 * NT < runs) before_hi = block_scan<NT>(packed_hi, 0xffffffffu, warp_sums, &all_hi);
+            const uint32_t before[kAtOnce] = {before_lo & 0xffffu, before_lo >> 16, before_hi & 0xffffu, before_hi >> 16};
+            const uint32_t all[kAtOnce] = {all_lo & 0xffffu, all_lo >> 16, all_hi & 0xffffu, all_hi >> 16};
+#pragma unroll
+            for (uint32_t k = 0; k < kAtOnce; ++k) {
+                const uint32_t rank = wanted + before[k];
+                if ((need >> k & 1) && rank < have) *entry[k] = free_list[have - 1 - rank];
+                wanted += all[k];
+            }
         }
-        for (uint32_t r = runs + tid; r <= s.runs_cap; r += kPlanThreads) s.runs[r] = (int32_t)total;
-        for (uint32_t b = tid; b <= c.seqs; b += kPlanThreads) {
+        for (uint32_t r = runs + tid; r <= s.runs_cap; r += NT) s.runs[r] = (int32_t)total;
+        for (uint32_t b = tid; b <= c.seqs; b += NT) {
             s.starts[b] = (int32_t)start[b];
             if (b < c.seqs) s.last[b] = start[b + 1] > start[b] ? (int32_t)start[b + 1] - 1 : -1;
         }
@@ -126,17 +141,35 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedView c, S
     }
     if (gridDim.x > 1) cluster_barrier();
     else __syncthreads();
-    for (uint32_t t = blockIdx.x * kPlanThreads + tid; t < s.tokens; t += gridDim.x * kPlanThreads) {
-        int32_t slot = -1, pos = -1;
-        if (t < total) {
-            const uint32_t b = owner_of(start, c.seqs, t), p = len[b] + (t - start[b]), j = p >> c.shift;
-            pos = (int32_t)p;
-            if (j < c.max_blocks) {
-                const int32_t e = __ldcg(c.table + (size_t)b * c.max_blocks + j);
-                if (e >= 0 && (uint32_t)e < c.blocks) slot = (int32_t)(((uint32_t)e << c.shift) + (p & (c.block - 1)));
-            }
+    // four rows a thread, one behind the other: one search, and another only where a request ends among them
+    const bool wide = ((reinterpret_cast<uintptr_t>(s.slots) | reinterpret_cast<uintptr_t>(s.positions)) & 15) == 0;
+    for (uint32_t t0 = 4 * (blockIdx.x * NT + tid); t0 < s.tokens; t0 += 4 * gridDim.x * NT) {
+        int32_t pos[4], slot[4];
+        uint32_t entry[4], b = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            const uint32_t t = t0 + k;
+            pos[k] = slot[k] = -1, entry[k] = 0xffffffffu;
+            if (t >= total) continue;
+            if (k == 0 || start[b + 1] <= t) b = owner_of(start, c.seqs, t, b);
+            const uint32_t p = len[b] + (t - start[b]), j = p >> c.shift;
+            pos[k] = (int32_t)p;
+            if (j < c.max_blocks) entry[k] = b * c.max_blocks + j;
         }
-        s.slots[t] = slot, s.positions[t] = pos;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k)
+            if (entry[k] != 0xffffffffu) slot[k] = __ldcg(c.table + entry[k]);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k)
+            slot[k] = slot[k] >= 0 && (uint32_t)slot[k] < c.blocks ? (int32_t)(((uint32_t)slot[k] << c.shift) + ((uint32_t)pos[k] & (c.block - 1))) : -1;
+        if (wide && t0 + 4 <= s.tokens) {
+            *reinterpret_cast<int4*>(s.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+            *reinterpret_cast<int4*>(s.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+        } else {
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k)
+                if (t0 + k < s.tokens) s.slots[t0 + k] = slot[k], s.positions[t0 + k] = pos[k];
+        }
     }
 }
 
@@ -165,7 +198,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_release_kernel(PagedView c
             }
             const bool held = e >= 0 && (uint32_t)e < c.blocks;
             uint32_t here;
-            const uint32_t rank = have + block_scan(held ? 1u : 0u, 0x7fffffffu, warp_sums, &here);
+            const uint32_t rank = have + block_scan<kPlanThreads>(held ? 1u : 0u, 0x7fffffffu, warp_sums, &here);
             if (held && rank < c.blocks) free_list[rank] = e;
             have = min(have + here, c.blocks);
         }
@@ -202,93 +235,129 @@ __device__ __forceinline__ uint32_t recode(uint32_t word, uint32_t byte, float r
     return (uint32_t)__float2int_rn(__fmul_rn((float)(int8_t)(word >> (8 * byte)), ratio)) & 0xffu;
 }
 
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedView c, StepView s, const float* __restrict__ qkv, uint32_t heads,
+template <int DIM>
+__global__ void __launch_bounds__(kAppendThreads, 4) paged_append_kernel(PagedView c, StepView s, const float* __restrict__ qkv, uint32_t heads,
                                                                      const float* __restrict__ cosv, const float* __restrict__ sinv, uint32_t max_pos,
                                                                      float* __restrict__ q_out) {
     GQ_GRID_DEP_SYNC();
+    // A thread has four components and the four half a head further, of every kRows-th row; kHeld of its rows stay in
+    // registers between the two passes, the others are read again.
+    constexpr uint32_t kHalf = DIM / 2, kQuads = kHalf / 4, kRows = kAppendThreads / kQuads, kHeld = 4;
     __shared__ uint32_t most[kAppendThreads / 32];
-    const uint32_t tid = threadIdx.x, dim = c.dim, half = dim / 2, quads = half / 4, pitch = (heads + 2 * c.kv_heads) * dim;
-    const uint32_t total = paged_start(s, c.seqs);
+    const uint32_t tid = threadIdx.x, d = tid % kQuads * 4, row0 = tid / kQuads, pitch = (heads + 2 * c.kv_heads) * DIM;
     const uint32_t r = blockIdx.x;
-    const uint32_t t0 = (uint32_t)max(s.runs[r], 0), t1 = min((uint32_t)max(s.runs[r + 1], 0), total);
+    const uint32_t t0 = (uint32_t)max(s.runs[r], 0), t1 = min((uint32_t)max(s.runs[r + 1], 0), paged_start(s, c.seqs));
     if (t0 >= t1) return;  // behind the last run
-    if (blockIdx.y >= 2 * c.kv_heads) {  // q
-        const uint32_t h0 = (blockIdx.y - 2 * c.kv_heads) * kQHeads, hn = min(kQHeads, heads - h0), per_row = hn * quads;
-        for (uint32_t i = tid; i < (t1 - t0) * per_row; i += kAppendThreads) {
-            const uint32_t row = i / per_row, e = i - row * per_row, t = t0 + row, d = (e % quads) * 4, h = h0 + e / quads;
-            const uint32_t p = min((uint32_t)max(s.positions[t], 0), max_pos - 1);
-            const float* src = qkv + (size_t)t * pitch + h * dim + d;
-            float4 lo, hi;
-            rotate4(*reinterpret_cast<const float4*>(src), *reinterpret_cast<const float4*>(src + half), cosv + (size_t)p * dim, sinv + (size_t)p * dim,
-                    d, half, lo, hi);
-            float* dst = q_out + ((size_t)t * heads + h) * dim + d;
-            *reinterpret_cast<float4*>(dst) = lo;
-            *reinterpret_cast<float4*>(dst + half) = hi;
+    const uint32_t pos0 = (uint32_t)max(s.positions[t0], 0);  // a run's positions follow one another
+    auto position = [&](uint32_t t) { return min(pos0 + (t - t0), max_pos - 1); };
+    if (blockIdx.y >= 2 * c.kv_heads) {  // q: kQHeads heads of every row
+        const uint32_t h0 = (blockIdx.y - 2 * c.kv_heads) * kQHeads, items = (t1 - t0) * kQHeads;
+        constexpr uint32_t kAtOnce = 4;
+        for (uint32_t i0 = row0; i0 < items; i0 += kAtOnce * kRows) {
+            float4 lo[kAtOnce], hi[kAtOnce];
+#pragma unroll
+            for (uint32_t j = 0; j < kAtOnce; ++j) {
+                const uint32_t i = i0 + j * kRows, t = t0 + i / kQHeads, h = h0 + i % kQHeads;
+                if (i >= items || h >= heads) continue;
+                const float* src = qkv + (size_t)t * pitch + h * DIM + d;
+                lo[j] = __ldcs(reinterpret_cast<const float4*>(src)), hi[j] = __ldcs(reinterpret_cast<const float4*>(src + kHalf));
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < kAtOnce; ++j) {
+                const uint32_t i = i0 + j * kRows, t = t0 + i / kQHeads, h = h0 + i % kQHeads;
+                if (i >= items || h >= heads) continue;
+                const size_t p = (size_t)position(t) * DIM;
+                float4 a, b;
+                rotate4(lo[j], hi[j], cosv + p, sinv + p, d, kHalf, a, b);
+                float* dst = q_out + ((size_t)t * heads + h) * DIM + d;
+                *reinterpret_cast<float4*>(dst) = a;
+                *reinterpret_cast<float4*>(dst + kHalf) = b;
+            }
         }
         return;
     }
-    const uint32_t head = blockIdx.y >> 1, is_v = blockIdx.y & 1;
+    const uint32_t head = blockIdx.y >> 1;
+    const bool is_v = blockIdx.y & 1;
     const int32_t slot = s.slots[t0];
     if (slot < 0 || ((uint32_t)slot >> c.shift) >= c.blocks) return;  // no room for this run
     const uint32_t block = (uint32_t)slot >> c.shift, off0 = (uint32_t)slot & (c.block - 1), n = min(t1 - t0, c.block - off0);
-    const float* src = qkv + (size_t)t0 * pitch + (size_t)(heads + (is_v ? c.kv_heads : 0) + head) * dim;
-    auto key_quads = [&](uint32_t row, uint32_t d, float4& lo, float4& hi) {
-        const uint32_t p = min((uint32_t)max(s.positions[t0 + row], 0), max_pos - 1);
+    const float* src = qkv + (size_t)t0 * pitch + (size_t)(heads + (is_v ? c.kv_heads : 0) + head) * DIM;
+    float* scale_at = (is_v ? c.vscale : c.kscale) + (size_t)block * c.kv_heads + head;
+    const float old = off0 ? *scale_at : 0.0f;
+    auto load = [&](uint32_t row, float4& lo, float4& hi) {
         const float* x = src + (size_t)row * pitch + d;
-        rotate4(*reinterpret_cast<const float4*>(x), *reinterpret_cast<const float4*>(x + half), cosv + (size_t)p * dim, sinv + (size_t)p * dim, d, half,
-                lo, hi);
+        lo = *reinterpret_cast<const float4*>(x), hi = *reinterpret_cast<const float4*>(x + kHalf);
+    };
+    auto turn = [&](uint32_t row, float4& lo, float4& hi) {
+        const size_t p = (size_t)position(t0 + row) * DIM;
+        float4 a, b;
+        rotate4(lo, hi, cosv + p, sinv + p, d, kHalf, a, b);
+        lo = a, hi = b;
     };
     uint32_t m = 0;
-    if (!is_v) {
-        for (uint32_t i = tid; i < n * quads; i += kAppendThreads) {
-            float4 lo, hi;
-            key_quads(i / quads, (i % quads) * 4, lo, hi);
-            m = max(m, max(mag4(lo), mag4(hi)));
+    float4 lo[kHeld], hi[kHeld];
+#pragma unroll
+    for (uint32_t j = 0; j < kHeld; ++j)
+        if (row0 + j * kRows < n) load(row0 + j * kRows, lo[j], hi[j]);
+#pragma unroll
+    for (uint32_t j = 0; j < kHeld; ++j)
+        if (row0 + j * kRows < n) {
+            if (!is_v) turn(row0 + j * kRows, lo[j], hi[j]);
+            m = max(m, max(mag4(lo[j]), mag4(hi[j])));
         }
-    } else {
-        for (uint32_t i = tid; i < n * 2 * quads; i += kAppendThreads)
-            m = max(m, mag4(*reinterpret_cast<const float4*>(src + (size_t)(i / (2 * quads)) * pitch + (i % (2 * quads)) * 4)));
+    for (uint32_t row = row0 + kHeld * kRows; row < n; row += kRows) {
+        float4 a, b;
+        load(row, a, b);
+        if (!is_v) turn(row, a, b);
+        m = max(m, max(mag4(a), mag4(b)));
     }
     m = __reduce_max_sync(0xffffffffu, m);
     if ((tid & 31) == 0) most[tid >> 5] = m;
-    float* scale_at = (is_v ? c.vscale : c.kscale) + (size_t)block * c.kv_heads + head;
-    const float old = off0 ? *scale_at : 0.0f;
-    __syncthreads();
+    __syncthreads();  // (and every thread has read the old scale)
 #pragma unroll
     for (int w = 0; w < kAppendThreads / 32; ++w) m = max(m, most[w]);
     const uint32_t fresh = mag(__fdiv_rn(__uint_as_float(m), 127.0f));
     const bool grows = fresh > mag(old);
     const float scale = grows ? __uint_as_float(fresh) : old, ratio = grows ? __fdiv_rn(old, scale) : 1.0f;
     if (tid == 0) *scale_at = scale;
-    uint32_t* pool = reinterpret_cast<uint32_t*>((is_v ? c.v : c.k) + ((size_t)block * c.kv_heads + head) * c.block * dim);
+    uint32_t* pool = reinterpret_cast<uint32_t*>((is_v ? c.v : c.k) + ((size_t)block * c.kv_heads + head) * c.block * DIM);
     if (!is_v) {
         if (grows)  // the block's other tokens, a word = four components of one token
-            for (uint32_t i = tid; i < (c.block - n) * 2 * quads; i += kAppendThreads) {
-                uint32_t t = i / (2 * quads);
+            for (uint32_t i = tid; i < (c.block - n) * 2 * kQuads; i += kAppendThreads) {
+                uint32_t t = i / (2 * kQuads);
                 t += t < off0 ? 0 : n;
-                uint32_t* w = pool + key_at(dim, t, (i % (2 * quads)) * 4) / 4;
+                uint32_t* w = pool + key_at(DIM, t, i % (2 * kQuads) * 4) / 4;
                 const uint32_t was = off0 ? *w : 0u;  // a block that starts anew starts as zeros
                 *w = recode(was, 0, ratio) | recode(was, 1, ratio) << 8 | recode(was, 2, ratio) << 16 | recode(was, 3, ratio) << 24;
             }
-        for (uint32_t i = tid; i < n * quads; i += kAppendThreads) {
-            const uint32_t row = i / quads, d = (i % quads) * 4;
-            float4 lo, hi;
-            key_quads(row, d, lo, hi);
-            pool[key_at(dim, off0 + row, d) / 4] = code_of(lo.x, scale) | code_of(lo.y, scale) << 8 | code_of(lo.z, scale) << 16 | code_of(lo.w, scale) << 24;
-            pool[key_at(dim, off0 + row, d + half) / 4] =
-                code_of(hi.x, scale) | code_of(hi.y, scale) << 8 | code_of(hi.z, scale) << 16 | code_of(hi.w, scale) << 24;
+        auto store = [&](uint32_t row, const float4& a, const float4& b) {
+            pool[key_at(DIM, off0 + row, d) / 4] = code_of(a.x, scale) | code_of(a.y, scale) << 8 | code_of(a.z, scale) << 16 | code_of(a.w, scale) << 24;
+            pool[key_at(DIM, off0 + row, d + kHalf) / 4] = code_of(b.x, scale) | code_of(b.y, scale) << 8 | code_of(b.z, scale) << 16 | code_of(b.w, scale) << 24;
+        };
+#pragma unroll
+        for (uint32_t j = 0; j < kHeld; ++j)
+            if (row0 + j * kRows < n) store(row0 + j * kRows, lo[j], hi[j]);
+        for (uint32_t row = row0 + kHeld * kRows; row < n; row += kRows) {
+            float4 a, b;
+            load(row, a, b);
+            turn(row, a, b);
+            store(row, a, b);
         }
     } else {
         // a word = four tokens of one component: the run's first and last may hold others too
         const uint32_t w0 = grows ? 0 : off0 >> 2, w1 = grows ? c.block >> 2 : (off0 + n + 3) >> 2;
-        for (uint32_t i = tid; i < (w1 - w0) * dim; i += kAppendThreads) {
-            const uint32_t d = i % dim, t = (w0 + i / dim) * 4;
-            uint32_t* at = pool + value_at(c.block, t, d) / 4;
+#pragma unroll 2
+        for (uint32_t i = tid; i < (w1 - w0) * DIM; i += kAppendThreads) {
+            const uint32_t comp = i % DIM, t = (w0 + i / DIM) * 4;
+            uint32_t* at = pool + value_at(c.block, t, comp) / 4;
             uint32_t word = (t < off0 || t + 4 > off0 + n) && (off0 || !grows) ? *at : 0u;
+            float x[4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) x[j] = t + j >= off0 && t + j < off0 + n ? src[(size_t)(t + j - off0) * pitch + comp] : 0.0f;
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) {
                 uint32_t code = word >> (8 * j) & 0xffu;
-                if (t + j >= off0 && t + j < off0 + n) code = code_of(src[(size_t)(t + j - off0) * pitch + d], scale);
+                if (t + j >= off0 && t + j < off0 + n) code = code_of(x[j], scale);
                 else if (grows) code = recode(word, j, ratio);
                 word = (word & ~(0xffu << (8 * j))) | code << (8 * j);
             }
@@ -300,19 +369,21 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedView 
 }  // namespace
 
 void launch_paged_plan(cudaStream_t s, const PagedView& c, const StepView& st, const int32_t* counts, const int32_t* free_list, int32_t* free_count) {
-    // One CTA fills 8192 rows of the maps in the time that the cluster's barrier takes.
+    // One CTA fills 8192 rows of the maps in about the time that the cluster's start and barrier take.
     const uint32_t ctas = st.tokens > 8192 ? kPlanCluster : 1;
+    const bool few = c.seqs <= kPlanFew && st.tokens <= 4 * kPlanFew;
     const size_t smem = (size_t)(3 * c.seqs + 2) * 4;
-    if (smem + 256 > 48 * 1024) GQ_CUDA(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    auto kernel = few ? paged_plan_kernel<kPlanFew> : paged_plan_kernel<kPlanThreads>;
+    if (smem + 256 > 48 * 1024) GQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(kPlanThreads), cfg.dynamicSmemBytes = smem, cfg.stream = s;
+    cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(few ? kPlanFew : kPlanThreads), cfg.dynamicSmemBytes = smem, cfg.stream = s;
     cudaLaunchAttribute attr[2]{};
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = ctas, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr, cfg.numAttrs = 2;
-    GQ_CUDA(cudaLaunchKernelEx(&cfg, paged_plan_kernel, c, st, counts, free_list, free_count));
+    GQ_CUDA(cudaLaunchKernelEx(&cfg, kernel, c, st, counts, free_list, free_count));
 }
 
 void launch_paged_advance(cudaStream_t s, const PagedView& c, const StepView& st) {
@@ -326,7 +397,8 @@ void launch_paged_release(cudaStream_t s, const PagedView& c, const int32_t* whi
 void launch_paged_append(cudaStream_t s, const PagedView& c, const StepView& st, const float* qkv, uint32_t heads, const float* cosv, const float* sinv,
                          uint32_t max_pos, float* q_out) {
     const uint32_t parts = 2 * c.kv_heads + (heads + kQHeads - 1) / kQHeads;
-    launch_after(paged_append_kernel, dim3(st.runs_cap, parts), dim3(kAppendThreads), 0, s, c, st, qkv, heads, cosv, sinv, max_pos, q_out);
+    auto kernel = c.dim == 128 ? paged_append_kernel<128> : c.dim == 64 ? paged_append_kernel<64> : paged_append_kernel<32>;
+    launch_after(kernel, dim3(st.runs_cap, parts), dim3(kAppendThreads), 0, s, c, st, qkv, heads, cosv, sinv, max_pos, q_out);
 }
 
 }  // namespace gq
