@@ -7,10 +7,10 @@
 // k_j = kscale_j K_j with 128 keys on the lanes of tensor memory, v_j = vscale_j V_j with the components on the lanes. What
 // meets them is held as an exact fixed-point integer in three base-256 digits, so three products in int32 and one join
 // give a float32 result:
-//   q_r = 2^(e_r - 22) Q, Q in signed digits; kscale_j is a factor of a lane;
-//   w vscale = 2^-22 P, P in unsigned digits. The value scales are folded into P because the sum over j runs across blocks;
+//   q_r = max|q_r| / 8323072 Q, Q in signed digits (8323072 = 127 * 2^16, what they hold); kscale_j is a factor of a lane;
+//   w vscale = 2^-23 P, P in unsigned digits. The value scales are folded into P because the sum over j runs across blocks;
 //     so that P fits, the reference of a row is the running maximum of s + log2 vscale (the largest contribution, not the largest
-//     score) and P's steps are 2^-22 of the largest contribution so far, whatever the blocks' scales are. The denominator
+//     score) and P's steps are 2^-23 of the largest contribution so far, whatever the blocks' scales are. The denominator
 //     sums the w themselves in float32. The reference stays until it is passed by a factor of 2: as long as no row of a warpgroup
 //     passes it D goes on adding up in int32, and is read, joined and added to the float32 sums only when one does (or
 //     after 256 tiles, before a sum could leave 32 bits).
@@ -41,8 +41,8 @@ namespace {
 constexpr uint32_t kKeys = 128;    // keys of a tile
 constexpr float kNone = -INFINITY;
 constexpr uint32_t kMostPerSm = 4;  // CTAs of an SM
-constexpr float kMagic = 8388608.0f;  // 2^23: x + 2^23 has rint(x) in its low 23 bits
-constexpr float kUnit = 4194304.0f;   // 2^22: P's steps of the reference
+constexpr float kUnit = 8388608.0f;  // 2^23: P's steps of the reference; P passes it by a factor of 2 at most, so it has 24 bits
+constexpr float kQMost = 8323072.0f;  // 127 * 2^16
 
 template <int RP, int WG, int DIM>
 struct Split {
@@ -102,7 +102,7 @@ __device__ __forceinline__ float join(uint32_t d0, uint32_t d1, uint32_t d2) {
 }
 
 // What the softmax needs to know of a block: x = its key scale; y = log2 of its value scale (of at least 2^-100) and a margin for the
-// rounding, so that P stays below 2^23; z = the value scale times 2^22; w = 0, 1 where a scale is none (negative, beyond 2^100 or
+// rounding, so that P stays below 2^24; z = the value scale times 2^23; w = 0, 1 where a scale is none (negative, beyond 2^100 or
 // no number; x is 1 then), 2 where there is no block.
 __device__ __forceinline__ float4 block_scale(float ks, float vs) {
     const bool good = vs >= 0.0f && vs <= 1.2676506e30f && ks >= 0.0f && ks <= 3.0e38f;
@@ -460,18 +460,17 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                                      max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
 #pragma unroll
                     for (uint32_t o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                    const uint32_t e = max(m >> 23, 32u);  // 2^(e - 126) > max |q|
-                    const float mult = e < 255 ? copysignf(__uint_as_float((275u - e) << 23), scale) : 0.0f;  // Q = rint(+-q 2^(22 - e)), |Q| <= 2^22
+                    const bool finite = m < 0x7f800000u;
+                    const float most = fmaxf(__uint_as_float(m), 1e-30f), mult = finite ? copysignf(__fdiv_rn(kQMost, most), scale) : 0.0f;
                     if (sub == 0) {
-                        const float inv = e < 255 ? __uint_as_float((e - 21u) << 23) : __uint_as_float(0x7fc00000u);
-                        row_scale[r] = inv * fabsf(scale);
+                        row_scale[r] = finite ? __fdiv_rn(most, kQMost) * fabsf(scale) : __uint_as_float(0x7fc00000u);
                         row_seen[r] = r < g.rows ? (int)min(g.len + token, g.keys - 1) : -1;
                     }
                     const float x[4] = {v.x, v.y, v.z, v.w};
                     uint32_t w0 = 0, w1 = 0, w2 = 0;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        int Q = __float2int_rn(x[j] * mult);
+                        int Q = __float2int_rn(x[j] * mult);  // +-q in steps of its row; |Q| <= 8323072
                         const int d0 = (int)(int8_t)Q;
                         Q = (Q - d0) >> 8;
                         const int d1 = (int)(int8_t)Q, d2 = (Q - d1) >> 8;
@@ -582,8 +581,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                         const float f = i == 0 ? fc.x : i == 1 ? fc.y : i == 2 ? fc.z : fc.w, ref = i == 0 ? rf.x : i == 1 ? rf.y : i == 2 ? rf.z : rf.w;
                         const float p = exp2_fast(__fmaf_rn(a[r + i], ONE ? f : factor_of(f, sc.x), ref));
                         l[r + i] += p;
-                        // rint(p vscale 2^22) in the low 23 bits (the last place of 2^23 is 1)
-                        x[i] = __float_as_uint(fminf(__fmaf_rn(p, sc.z, kMagic), 16777215.0f));
+                        x[i] = min(__float2uint_rn(p * sc.z), 0xffffffu);  // P
                     }
                     // digit d of the four rows, one row to a byte
                     const uint32_t y0 = __byte_perm(x[0], x[1], 0x5140), y1 = __byte_perm(x[2], x[3], 0x5140);
