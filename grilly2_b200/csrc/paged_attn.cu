@@ -16,7 +16,7 @@
 //     after 256 tiles, before a sum could leave 32 bits).
 // A warp's 32 keys share one block and so one scale (blocks of 32 and more): the maximum is taken over the joined integers
 // and scaled afterwards, and the exponent is one multiplication and addition of the integer.
-// Scales of values from 2^-100 to 2^100 (and 0) are exact; larger, negative or non-finite ones read as NaN.
+// Scales of values from 2^-100 to 2^90 (and 0) lose nothing; larger, negative or non-finite ones read as NaN.
 //
 // A CTA takes a contiguous range of all (request, row tile, KV head, 128-key tile) units, equal ranges for all CTAs: with ragged
 // lengths no CTA waits for a long request, and a single request fills the GPU. A row tile is RP rows of (token, head of the
@@ -41,7 +41,8 @@ namespace {
 constexpr uint32_t kKeys = 128;    // keys of a tile
 constexpr float kNone = -INFINITY;
 constexpr uint32_t kMostPerSm = 4;  // CTAs of an SM
-constexpr float kUnit = 8388608.0f;  // 2^23: P's steps of the reference; P passes it by a factor of 2 at most, so it has 24 bits
+constexpr float kUnit = 8388608.0f;  // 2^23: P's steps of the reference; P passes it by a factor of 2 at most, so it has 24 bits,
+                                     // the upper ones of a word whose conversion stops at 2^32 of itself
 constexpr float kQMost = 8323072.0f;  // 127 * 2^16
 
 template <int RP, int WG, int DIM>
@@ -102,11 +103,11 @@ __device__ __forceinline__ float join(uint32_t d0, uint32_t d1, uint32_t d2) {
 }
 
 // What the softmax needs to know of a block: x = its key scale; y = log2 of its value scale (of at least 2^-100) and a margin for the
-// rounding, so that P stays below 2^24; z = the value scale times 2^23; w = 0, 1 where a scale is none (negative, beyond 2^100 or
+// rounding, so that P stays below 2^24; z = the value scale times 2^31; w = 0, 1 where a scale is none (negative, beyond 2^90 or
 // no number; x is 1 then), 2 where there is no block.
 __device__ __forceinline__ float4 block_scale(float ks, float vs) {
-    const bool good = vs >= 0.0f && vs <= 1.2676506e30f && ks >= 0.0f && ks <= 3.0e38f;
-    return make_float4(good ? ks : 1.0f, fmaxf(__log2f(vs), -100.0f) + 0.001f, vs * kUnit, good ? 0.0f : 1.0f);
+    const bool good = vs >= 0.0f && vs <= 1.2379401e27f && ks >= 0.0f && ks <= 3.0e38f;
+    return make_float4(good ? ks : 1.0f, fmaxf(__log2f(vs), -100.0f) + 0.001f, vs * kUnit * 256.0f, good ? 0.0f : 1.0f);
 }
 
 // sum of floor((a i + b) / m) for i < n, by Euclid's steps on (a, m); the divisions in 32 bits where the numbers allow (a
@@ -159,6 +160,7 @@ struct Segment {
     uint32_t clear;              // keys that every row of the item sees
     uint32_t start, len, keys;   // of the request
     uint32_t whole, more;        // the item is this segment; 0: no segment, the end
+    uint32_t c0, parts, second;  // the item's first CTA, how many have a part of it, whether the first one's is its second part
     uint64_t first, last;        // the item's units [first, last)
 };
 constexpr uint32_t kSegments = 4;  // of the ring
@@ -213,11 +215,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
     uint64_t* q_full = d_full + 2;                       // Q is written
     uint64_t* seg_full = q_full + 1;                     // [kSegments] a segment is written
     uint64_t* seg_free = seg_full + kSegments;           // [kSegments] ... and done with
-    uint64_t* scan = seg_free + kSegments;               // [24]
-    uint64_t* found = scan + 24;                         // the units before the row tile that the range starts in
-    uint32_t* found_b = reinterpret_cast<uint32_t*>(found + 1);
-    uint32_t* found_qt = found_b + 1;
-    uint32_t* tmem_slot = found_qt + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(seg_free + kSegments);
     uint32_t* arrived = tmem_slot + 1;
     volatile uint32_t* failed = arrived + 1;
     volatile uint32_t* go_on = arrived + 2;              // [2] whether a warpgroup's D goes on adding up
@@ -247,50 +245,47 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
     const uint32_t tmem = *tmem_slot;
     GQ_GRID_DEP_SYNC();
 
-    // the units of all requests, and the request and row tile that this CTA's range starts in
-    const uint32_t per = (c.seqs + T::kThreads - 1) / T::kThreads, b0 = min(tid * per, c.seqs), b1 = min(b0 + per, c.seqs);
-    uint64_t mine = 0;
-    for (uint32_t b = b0; b < b1; ++b) mine += request_of(c, s, b, group, RP).units();
-    uint64_t upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t y = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= (uint32_t)o) upto += y;
-    }
-    if (lane == 31) scan[warp] = upto;
-    __syncthreads();
-    uint64_t total = 0, before = upto - mine;
-    for (uint32_t w = 0; w < T::kThreads / 32; ++w) {
-        if (w < warp) before += scan[w];
-        total += scan[w];
-    }
-    // ranges of `share` units, the first `extra` ones of one more
-    const uint32_t ctas = (uint32_t)min((uint64_t)gridDim.x, total);
-    const uint64_t share = ctas ? (total >> 32 ? total / ctas : (uint32_t)total / ctas) : 0, extra = total - share * ctas;
-    auto range_at = [&](uint32_t i) { return i * share + min((uint64_t)i, extra); };
-    auto cta_of = [&](uint64_t u) {  // whose range holds unit u
-        const uint64_t longer = extra * (share + 1);
-        const uint64_t v = u < longer ? u : u - longer, by = u < longer ? share + 1 : share;
-        return (uint32_t)((u < longer ? 0 : extra) + (v >> 32 || by >> 32 ? v / by : (uint32_t)v / (uint32_t)by));
-    };
-    if (blockIdx.x < ctas) {
-        const uint64_t u = range_at(blockIdx.x);
-        if (u >= before && u < before + mine) {
-            uint32_t b = b0;
-            uint64_t base = before, units;
-            while (u >= base + (units = request_of(c, s, b, group, RP).units())) base += units, ++b;
-            *found = base, *found_b = b;
-        }
-    }
-    __syncthreads();
     bool ok = true;
 
     if (warp == 4 * WG + 1) {
+        // the units of all requests: lane = a stretch of requests
+        const uint32_t per = (c.seqs + 31) / 32, b0 = min(lane * per, c.seqs), b1 = min(b0 + per, c.seqs);
+        uint64_t mine = 0;
+#pragma unroll 4
+        for (uint32_t b = b0; b < b1; ++b) mine += request_of(c, s, b, group, RP).units();
+        auto scanned = [&](uint64_t v) {
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint64_t y = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= (uint32_t)o) v += y;
+            }
+            return v;
+        };
+        const uint64_t upto = scanned(mine), total = __shfl_sync(0xffffffffu, upto, 31);
+        // ranges of `share` units, the first `extra` ones of one more
+        const uint32_t ctas = (uint32_t)min((uint64_t)gridDim.x, total);
+        const uint64_t share = ctas ? (total >> 32 ? total / ctas : (uint32_t)total / ctas) : 0, extra = total - share * ctas;
+        auto range_at = [&](uint32_t i) { return i * share + min((uint64_t)i, extra); };
+        auto cta_of = [&](uint64_t u) {  // whose range holds unit u
+            const uint64_t longer = extra * (share + 1);
+            const uint64_t v = u < longer ? u : u - longer, by = u < longer ? share + 1 : share;
+            return (uint32_t)((u < longer ? 0 : extra) + (v >> 32 || by >> 32 ? v / by : (uint32_t)v / (uint32_t)by));
+        };
         Walk walk;
         walk.u = walk.hi = 0;
         if (blockIdx.x < ctas) {
             walk.u = range_at(blockIdx.x), walk.hi = range_at(blockIdx.x + 1);
-            walk.b = *found_b, walk.base = *found, walk.qt = 0;
+            // the request that the range starts in: its stretch, then the stretch request by request
+            const int in = __ffs(__ballot_sync(0xffffffffu, walk.u >= upto - mine && walk.u < upto)) - 1;
+            const uint32_t end = __shfl_sync(0xffffffffu, b1, in);
+            walk.b = __shfl_sync(0xffffffffu, b0, in), walk.base = __shfl_sync(0xffffffffu, upto - mine, in), walk.qt = 0;
+            for (;;) {
+                const uint64_t units = walk.b + lane < end ? request_of(c, s, walk.b + lane, group, RP).units() : 0, through = scanned(units);
+                const uint32_t hit = __ballot_sync(0xffffffffu, walk.u < walk.base + through);
+                const int at = hit ? __ffs(hit) - 1 : 31;
+                walk.base += __shfl_sync(0xffffffffu, hit ? through - units : through, at), walk.b += hit ? at : 32;
+                if (hit || walk.b >= end) break;
+            }
             walk.r = request_of(c, s, walk.b, group, RP);
             if (walk.r.row_tiles > 1) {  // the last row tile that begins at or before u, 32 candidates a round
                 const uint64_t v = walk.u - walk.base;
@@ -311,6 +306,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
             if (seg >= kSegments) ok = mbar_wait(seg_free + seg % kSegments, (seg / kSegments - 1) & 1, failed, status, kStatusEmptyWaitTimedOut);
             if (__ballot_sync(0xffffffffu, !ok)) ok = false;
             if (!ok) break;
+            if (more && !g.whole) g.c0 = cta_of(g.first), g.parts = cta_of(g.last - 1) - g.c0 + 1, g.second = range_at(g.c0) != g.first;
             if (lane == 0) {
                 segments[seg % kSegments] = g;
                 mbar_arrive(seg_full + seg % kSegments);
@@ -581,12 +577,12 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                         const float f = i == 0 ? fc.x : i == 1 ? fc.y : i == 2 ? fc.z : fc.w, ref = i == 0 ? rf.x : i == 1 ? rf.y : i == 2 ? rf.z : rf.w;
                         const float p = exp2_fast(__fmaf_rn(a[r + i], ONE ? f : factor_of(f, sc.x), ref));
                         l[r + i] += p;
-                        x[i] = min(__float2uint_rn(p * sc.z), 0xffffffu);  // P
+                        x[i] = __float2uint_rn(__fmaf_rn(p, sc.z, 128.0f));  // 256 P, P rounded
                     }
                     // digit d of the four rows, one row to a byte
-                    const uint32_t y0 = __byte_perm(x[0], x[1], 0x5140), y1 = __byte_perm(x[2], x[3], 0x5140);
+                    const uint32_t y0 = __byte_perm(x[0], x[1], 0x6251), y1 = __byte_perm(x[2], x[3], 0x6251);
                     uint32_t w[3] = {__byte_perm(y0, y1, 0x5410), __byte_perm(y0, y1, 0x7632),
-                                     __byte_perm(__byte_perm(x[0], x[1], 0x0062), __byte_perm(x[2], x[3], 0x0062), 0x5410)};
+                                     __byte_perm(__byte_perm(x[0], x[1], 0x0073), __byte_perm(x[2], x[3], 0x0073), 0x5410)};
 #pragma unroll
                     for (uint32_t d = 0; d < 3; ++d) {  // ... becomes row r + lane % 4 of four lanes' keys, one key to a byte
                         w[d] = __byte_perm(w[d], __shfl_xor_sync(0xffffffffu, w[d], 1), sel1);
@@ -632,8 +628,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
             }
             // a part of an item: what this CTA has, and the last CTA to arrive adds the parts up
             constexpr uint32_t kPart = RP * (DIM + 2);
-            const uint32_t c0 = cta_of(g.first), parts = cta_of(g.last - 1) - c0 + 1;
-            const uint32_t second = range_at(c0) != g.first;  // the first CTA's range began with another item
+            const uint32_t c0 = g.c0, parts = g.parts, second = g.second;
             auto part_of = [&](uint32_t cta) { return partials + (size_t)(cta * 2 + (cta == c0 ? second : 0)) * kPart; };
             float* part = part_of(blockIdx.x);
             if (owner)

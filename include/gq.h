@@ -445,7 +445,8 @@ int32_t gq_paged_append(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer
                         uint64_t max_pos, const gq_paged_step* step, gq_buf q_out);
 /* Causal grouped-query attention of the step's rows over the cache: row t of request b, at position p = lens[b] + t -
  * starts[b], attends to positions 0 .. p. out[t] = softmax(scale q k^T) v. Positions whose block is missing are
- * skipped; a row that is left with none gives zeros. q and out float32 [max_tokens][heads dim], not overlapping; rows behind
+ * skipped; a row that is left with none gives zeros. A row that sees a block whose scales are negative, no number or
+ * beyond 2^90 (for values) is NaN. q and out float32 [max_tokens][heads dim], not overlapping; rows behind
  * starts[seqs] are left as they were. max_count is the largest counts[b] the caller expects (1 for a decode step): it chooses
  * how the work is cut, never what is computed. */
 int32_t gq_paged_attn(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer, gq_buf q, uint64_t heads, float scale, const gq_paged_step* step,

@@ -337,6 +337,28 @@ def test_peaked_and_flat_scores():
         attend(t, [1, 30], scale=scale)
 
 
+@pytest.mark.parametrize("value", [1e-25, 1e-6, 1e6, 1e20])
+def test_value_scales_of_any_size(value):
+    rng = np.random.default_rng(16)
+    t = filled(rng, 4, 2, 64, 32, [200, 40], [1, 33], spread=0.3)
+    t.scales["v"] *= np.float32(value)
+    t.cache.vscale.copy_(dev(t.scales["v"]).reshape(t.cache.vscale.shape))
+    attend(t, [1, 33])
+
+
+def test_scales_that_are_none_make_their_rows_nan():
+    rng = np.random.default_rng(17)
+    for name, bad in [("k", -1.0), ("k", np.inf), ("v", -1.0), ("v", np.inf), ("v", 2.0 ** 91), ("k", np.nan)]:
+        t = filled(rng, 2, 1, 32, 32, [70, 70], [1, 1])
+        scales, on_device = t.scales[name], t.cache.kscale if name == "k" else t.cache.vscale
+        scales[t.table[1, 0]] = bad
+        on_device.copy_(dev(scales).reshape(on_device.shape))
+        st = t.Step(t.cache, 2)
+        t.cache.plan(dev(np.ones(2, np.int32)), st)
+        out = t.cache.attend(0, dev(rng.standard_normal((2, 64)).astype(np.float32)), 2, st, max_count=1).numpy()
+        assert np.isfinite(out[0]).all() and np.isnan(out[1]).all(), (name, bad)
+
+
 def test_two_requests_may_read_the_same_blocks():
     rng = np.random.default_rng(13)
     t = filled(rng, 8, 2, 64, 32, [64, 70, 64], [1, 1, 1])
