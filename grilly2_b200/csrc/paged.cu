@@ -226,9 +226,13 @@ __device__ __forceinline__ void rotate4(const float4& lo, const float4& hi, cons
 __device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 __device__ __forceinline__ uint32_t mag4(const float4& v) { return max(max(mag(v.x), mag(v.y)), max(mag(v.z), mag(v.w))); }
 
-// rint(v / s) in the codes' range; an empty scale (all zeros) and a value that is not a number give 0
-__device__ __forceinline__ uint32_t code_of(float v, float s) {
-    const float r = s == 0.0f ? 0.0f : __fdiv_rn(v, s);
+// rint(v / s) in the codes' range, the quotient rounded as IEEE division does; an empty scale (all zeros) and a value that is not a
+// number give 0. The product with the reciprocal differs from the quotient by two roundings, 127 * 2^-23 = 1.5e-5 at most, so only
+// next to a half does it take the division to tell.
+__device__ __forceinline__ uint32_t code_of(float v, float s, float inverse) {
+    float r = v * inverse;
+    const float whole = rintf(r);
+    if (!(fabsf(r - whole) <= 0.4998f)) r = __fdiv_rn(v, s);
     return (uint32_t)max(-127, min(127, __float2int_rn(r))) & 0xffu;
 }
 __device__ __forceinline__ uint32_t recode(uint32_t word, uint32_t byte, float ratio) {
@@ -319,6 +323,8 @@ __global__ void __launch_bounds__(kAppendThreads, 4) paged_append_kernel(PagedVi
     const uint32_t fresh = mag(__fdiv_rn(__uint_as_float(m), 127.0f));
     const bool grows = fresh > mag(old);
     const float scale = grows ? __uint_as_float(fresh) : old, ratio = grows ? __fdiv_rn(old, scale) : 1.0f;
+    // a scale whose reciprocal may not be a normal number has none: every code of it is divided for
+    const float inverse = scale == 0.0f ? 0.0f : scale > 0x1p-100f && scale < 0x1p100f ? __fdiv_rn(1.0f, scale) : __int_as_float(0x7fc00000);
     if (tid == 0) *scale_at = scale;
     uint32_t* pool = reinterpret_cast<uint32_t*>((is_v ? c.v : c.k) + ((size_t)block * c.kv_heads + head) * c.block * DIM);
     if (!is_v) {
@@ -331,8 +337,8 @@ __global__ void __launch_bounds__(kAppendThreads, 4) paged_append_kernel(PagedVi
                 *w = recode(was, 0, ratio) | recode(was, 1, ratio) << 8 | recode(was, 2, ratio) << 16 | recode(was, 3, ratio) << 24;
             }
         auto store = [&](uint32_t row, const float4& a, const float4& b) {
-            pool[key_at(DIM, off0 + row, d) / 4] = code_of(a.x, scale) | code_of(a.y, scale) << 8 | code_of(a.z, scale) << 16 | code_of(a.w, scale) << 24;
-            pool[key_at(DIM, off0 + row, d + kHalf) / 4] = code_of(b.x, scale) | code_of(b.y, scale) << 8 | code_of(b.z, scale) << 16 | code_of(b.w, scale) << 24;
+            pool[key_at(DIM, off0 + row, d) / 4] = code_of(a.x, scale, inverse) | code_of(a.y, scale, inverse) << 8 | code_of(a.z, scale, inverse) << 16 | code_of(a.w, scale, inverse) << 24;
+            pool[key_at(DIM, off0 + row, d + kHalf) / 4] = code_of(b.x, scale, inverse) | code_of(b.y, scale, inverse) << 8 | code_of(b.z, scale, inverse) << 16 | code_of(b.w, scale, inverse) << 24;
         };
 #pragma unroll
         for (uint32_t j = 0; j < kHeld; ++j)
@@ -357,7 +363,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) paged_append_kernel(PagedVi
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) {
                 uint32_t code = word >> (8 * j) & 0xffu;
-                if (t + j >= off0 && t + j < off0 + n) code = code_of(x[j], scale);
+                if (t + j >= off0 && t + j < off0 + n) code = code_of(x[j], scale, inverse);
                 else if (grows) code = recode(word, j, ratio);
                 word = (word & ~(0xffu << (8 * j))) | code << (8 * j);
             }

@@ -229,6 +229,24 @@ def test_append_zeros_and_values_that_are_no_numbers():
     np.testing.assert_array_equal(bad, [[False, False], [True, False], [False, True]])
 
 
+@pytest.mark.parametrize("size", [1e-43, 3e-39, 1e-30, 0.37, 1e31, 2.5e38])
+def test_append_next_to_halves_and_at_the_ends_of_the_range(size):
+    """Values on and beside every border between two codes, for scales from the subnormal ones to the largest: the codes are the
+    rounded quotients, bit for bit."""
+    t = Twin(np.random.default_rng(8), seqs=1, heads=1, kvh=1, dim=128, bs=16, mb=1, blocks=1)
+    t.cos[:], t.sin[:] = 1.0, 0.0
+    with np.errstate(all="ignore"):
+        step = np.float32(size) / np.float32(127)
+        border = ((np.arange(-127, 128) + 0.5)[:, None] * step).astype(np.float32)
+        x = np.concatenate([np.nextafter(border, np.float32(-np.inf)), border, np.nextafter(border, np.float32(np.inf))], 1).reshape(-1)
+    x = np.clip(x, -np.float32(size), np.float32(size))[:6 * 128].reshape(-1)
+    rows = -(-x.size // 128)
+    x = np.concatenate([x, np.full(rows * 128 - x.size, size, np.float32)]).reshape(rows, 1, 128)
+    assert rows <= 16 and np.abs(x).max() == np.float32(size)
+    t.step([rows], qkv=np.concatenate([x, x, x], 1))
+    t.check_pool()
+
+
 def test_append_skips_rows_without_room():
     t = Twin(np.random.default_rng(6), seqs=3, heads=2, kvh=1, dim=32, bs=16, mb=2, blocks=3)
     st, want, turned = t.step([40, 3, 20])  # 32 tokens fit the table, three blocks the pool
