@@ -10,11 +10,15 @@
 //     bin where it reaches k. Those are listed in the first CTA's shared memory, and it finishes the row alone: it
 //     counts for every listed token how many and how much lie above, and for the kept ones how much lies before.
 //   3 otherwise, for top-k and then top-p: a histogram of all tokens (counts or masses), its crossing bin, and that bin's
-//     tokens as a list that is ranked the same way
+//     tokens as a list that is ranked the same way, or bisected where it is long
 //   4 every thread's kept mass, a thread owning consecutive tokens; the thread that holds the target walks its own
 // A bin of more tokens than the list holds (ties, a flat row) falls back to bisecting the float's bits with a pass over the
-// row per step. Bound: latency (4 to 12 cluster barriers); of large batches without top-k the arithmetic of a float64
-// exponential a token.
+// row per step.
+//
+// Bound: latency and instruction issue, not memory: one row of 151936 (0.6 MB) takes 13.2 us, 64 rows (39 MB, 5.9 us at the rate
+// of a copy) 73, 200 rows of 32003 (26 MB, 3.9 us) 40. 15 us of the 73 go into reading the rows into shared memory, 30 into
+// the masses' histogram (a float64 exponential a token, 33 instructions, and an atomic addition), 18 into listing and ranking
+// its crossing bin, 10 into the draw; 64 rows of eight CTAs run as two waves, since 39 MB do not fit the SMs at once.
 #include <cooperative_groups.h>
 
 #include "gq_internal.h"
@@ -27,7 +31,9 @@ namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr uint32_t kBins = 2048, kList = 2048, kMostCtas = 8;
+constexpr int kFixedBits = 40;
 constexpr double kFixed = 1099511627776.0;  // 2^40
+constexpr uint32_t kRanked = 96;            // tokens that are ranked by comparing all with all; more are bisected (see select)
 constexpr uint32_t kStaged = 19 * 1024;     // logits of a row that a CTA keeps at most: two CTAs an SM
 
 __device__ __forceinline__ uint32_t key_of(float f) {  // a < b as floats <=> key_of(a) < key_of(b)
@@ -54,7 +60,7 @@ struct Control {
     unsigned long long scan[kWarps];
 };
 struct alignas(16) Shared {  // the logits behind it are stored four at a time
-    double pow2[8];  // 2^(i / 8)
+    double pow2[16];  // 2^(i / 16)
     Control ctl;
     union {
         struct {
@@ -67,21 +73,21 @@ struct alignas(16) Shared {  // the logits behind it are stored four at a time
     };
 };
 
-// exp(d ln 2 / 8 step) for d <= 0, step = 8 / (T ln 2): 2^(n / 8) from a table of eight (small enough that the lanes' loads meet
-// no bank conflicts) times the Taylor polynomial of 2^(f / 8), |f| <= 1/2, whose next term is below 6e-14. The result keeps an
-// exponent above 2^-1022 for all that weighs more than e^-64.
-__device__ __forceinline__ double exp_of(double d, double step, const double* pow2) {
+// exp(d ln 2 / 16 step) 2^PLUS + add for d <= 0, step = 16 / (T ln 2): 2^(n / 16) from a table of sixteen (as many as give the
+// lanes' loads no bank conflicts) with n's whole part in its exponent, times the Taylor polynomial of 2^(f / 16), |f| <= 1/2,
+// whose next term is below 2e-13. The exponent stays above 2^-1022 for all that weighs more than e^-64.
+template <int PLUS>
+__device__ __forceinline__ double exp_of(double d, double step, const double* pow2, double add) {
     const double t = __fma_rn(d, step, 6755399441055744.0);  // 1.5 * 2^52 rounds to a whole number
     const int n = __double2loint(t);
     const double f = __fma_rn(d, step, -(t - 6755399441055744.0));
-    double p = __fma_rn(f, 5.87598052726044e-10, 4.069079024178602e-08);  // (ln 2 / 8)^k / k!
-    p = __fma_rn(p, f, 2.3481760516671086e-06);
-    p = __fma_rn(p, f, 0.00010840646223597965);
-    p = __fma_rn(p, f, 0.0037535391712359488);
-    p = __fma_rn(p, f, 0.08664339756999316);
+    double p = __fma_rn(f, 1.271587195055813e-09, 1.467610032291943e-07);  // (ln 2 / 16)^k / k!
+    p = __fma_rn(p, f, 1.3550807779497455e-05);
+    p = __fma_rn(p, f, 0.0009383847928089871);
+    p = __fma_rn(p, f, 0.04332169878499658);
     p = __fma_rn(p, f, 1.0);
-    const double v = p * pow2[n & 7];
-    return __hiloint2double(__double2hiint(v) + ((n >> 3) << 20), __double2loint(v));
+    const double v = pow2[n & 15];
+    return __fma_rn(p, __hiloint2double(__double2hiint(v) + (n & ~15) * 65536 + PLUS * 1048576, __double2loint(v)), add);
 }
 
 // STAGED: a CTA's logits fit its shared memory.
@@ -102,7 +108,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* _
     const float* x = logits + (size_t)row * vocab + first;
     Shared* lead = cluster.map_shared_rank(&sh, 0);
 
-    if (tid < 8) sh.pow2[tid] = exp2((double)tid / 8.0);
+    if (tid < 16) sh.pow2[tid] = exp2((double)tid / 16.0);
     for (uint32_t i = tid; i < kBins; i += kThreads) sh.hist.lo[i] = sh.hist.hi[i] = 0;
     const float u = uniforms[(size_t)(draws ? *draws % uniform_rows : 0u) * rows + row];
     if (tid == 0) sh.ctl.top[0] = 0, sh.ctl.top[1] = 0xffffffffu, sh.ctl.listed = 0, sh.ctl.range_lo = 0xffffffffu, sh.ctl.range_hi = 0;
@@ -161,14 +167,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* _
         return;
     }
     const bool greedy = !(tf > 0.0f);
-    const double Md = (double)M, step = greedy ? 0.0 : 11.541560327111707 / (double)tf;  // 8 / ln 2
-    const float per_x = fmaxf(32.0f / tf, (float)(kBins - 1) / (M - value_of(lk)));
-    auto weight = [&](float v) { return v == M ? 1.0 : exp_of(widen(v) - Md, step, sh.pow2); };  // of what is not below `low`
+    const double Md = widen(M), step = greedy ? 0.0 : 23.083120654223414 / (double)tf;  // 16 / ln 2
+    const float per_x = fminf(fmaxf(32.0f / tf, (float)(kBins - 1) / (M - value_of(lk))), 3e38f), top = fminf(M, 3.402823466e+38f);
+    auto weight = [&](float v) { return exp_of<0>(widen(v) - Md, step, sh.pow2, 0.0); };  // of what is not below `low`; the largest's is 1
     auto fixed = [&](float v) {  // w 2^40 as a whole number, by the last place of 2^52
-        return (unsigned long long)__double_as_longlong(__fma_rn(weight(v), kFixed, 4503599627370496.0)) & 0xfffffffffffffull;
+        return (unsigned long long)__double_as_longlong(exp_of<kFixedBits>(widen(v) - Md, step, sh.pow2, 4503599627370496.0)) & 0xfffffffffffffull;
     };
-    // falls as v rises; rounded by the last place of 2^23
-    auto bin_of = [&](float v) { return v == M ? 0 : (int)(__float_as_uint(fminf((M - v) * per_x, (float)(kBins - 1)) + 8388608.0f) & (kBins - 1)); };
+    // falls as v rises; rounded by the last place of 2^23 (+inf, where that is the largest: -inf, whose last bits are 0)
+    auto bin_of = [&](float v) { return (int)(__float_as_uint(fminf((top - v) * per_x, (float)(kBins - 1)) + 8388608.0f) & (kBins - 1)); };
     // tokens below are dropped: at first what weighs less than e^-64 (in a bin behind the last, too)
     float low = greedy ? M : fmaxf(M - 64.0f * tf, -3.402823466e+38f);
 
@@ -244,14 +250,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* _
             if (i < listed && part == 0) done(i, sum);
         }
     };
+    auto warp_sum = [](unsigned long long v) {  // in pieces of 22 bits
+        const uint32_t lo = __reduce_add_sync(0xffffffffu, (uint32_t)v & 0x3fffffu), mid = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 22) & 0x3fffffu);
+        return lo + ((unsigned long long)mid << 22) + ((unsigned long long)__reduce_add_sync(0xffffffffu, (uint32_t)(v >> 44)) << 44);
+    };
     auto block_sum = [&](unsigned long long v) {  // of the CTA's threads, the same for all
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        v = warp_sum(v);
         if (lane == 0) sh.ctl.scan[warp] = v;
         __syncthreads();
-        v = lane < kWarps ? sh.ctl.scan[lane] : 0ull;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        v = warp_sum(lane < kWarps ? sh.ctl.scan[lane] : 0ull);
         __syncthreads();
         return v;
     };
@@ -316,14 +323,37 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* _
         lo = lead->ctl.range_lo, hi = lead->ctl.range_hi;
         if (listed <= kList) {
             if (rank == 0) {
-                if (tid == 0) sh.ctl.low = hi;
-                __syncthreads();
-                each_listed(
-                    listed,
-                    [&](uint32_t i, uint32_t j) { return sh.list.key[j] > sh.list.key[i] ? sh.list.mass[j] : 0ull; },
-                    [&](uint32_t i, unsigned long long mass) {
-                        if (above + mass < target) atomicMin(&sh.ctl.low, sh.list.key[i]);
-                    });
+                if (listed <= kRanked) {
+                    if (tid == 0) sh.ctl.low = hi;
+                    __syncthreads();
+                    each_listed(
+                        listed,
+                        [&](uint32_t i, uint32_t j) { return sh.list.key[j] > sh.list.key[i] ? sh.list.mass[j] : 0ull; },
+                        [&](uint32_t i, unsigned long long mass) {
+                            if (above + mass < target) atomicMin(&sh.ctl.low, sh.list.key[i]);
+                        });
+                } else {
+                    // The floats' bits bisected, every thread with its tokens in registers: 3.3k cycles however many they are, where
+                    // comparing all with all takes 2k for 60 tokens and 12k for 250. (64 rows of 151936: 74.6 us with the bisection
+                    // alone, 78.3 without it, 72.9 from 96 tokens on; 200 rows of 32003: 43.9, 40.0, 40.0.)
+                    constexpr uint32_t kPer = kList / kThreads;
+                    uint32_t key[kPer];
+                    unsigned long long mass[kPer];
+#pragma unroll
+                    for (uint32_t j = 0; j < kPer; ++j) {
+                        const uint32_t i = tid + j * kThreads;
+                        key[j] = i < listed ? sh.list.key[i] : 0u, mass[j] = i < listed ? sh.list.mass[i] : 0ull;
+                    }
+                    while (lo < hi) {
+                        const uint32_t mid = lo + (hi - lo) / 2;
+                        unsigned long long over = 0;
+#pragma unroll
+                        for (uint32_t j = 0; j < kPer; ++j) over += key[j] > mid ? mass[j] : 0ull;
+                        if (above + block_sum(over) < target) hi = mid;
+                        else lo = mid + 1;
+                    }
+                    if (tid == 0) sh.ctl.low = lo;
+                }
             }
             cluster.sync();
             low = value_of(lead->ctl.low);
@@ -509,8 +539,8 @@ void launch_sample_rows(cudaStream_t s, int sm_count, const float* logits, uint3
                         const float* top_p, const float* min_p, const float* uniforms, uint32_t uniform_rows, uint32_t* draws, int32_t* tokens, float* probs,
                         uint32_t* ticket) {
     // CTAs of a row: as many as leave each some thousands of tokens while the CTAs an SM holds (two) hold all rows, and as
-    // many as keep the row in shared memory. (1024 threads and one CTA an SM: 14.6 us for one row of 151936 against 13.6, 49 for
-    // 200 rows of 32003 against 43, 77 for 64 rows of 151936 against 84.)
+    // many as keep the row in shared memory. (1024 threads and one CTA an SM, before the exponential and the ranking were made
+    // shorter: 14.6 us for one row of 151936 against 13.6, 49 for 200 rows of 32003 against 43, 77 for 64 rows of 151936 against 84.)
     uint32_t ctas = 1;
     while (ctas < kMostCtas && ((vocab / ctas >= 8192 && rows * ctas <= (uint32_t)sm_count) || (vocab + ctas - 1) / ctas > kStaged)) ctas *= 2;
     const uint32_t slice = ((vocab + ctas - 1) / ctas + 3) / 4 * 4, staged = slice <= kStaged;
