@@ -138,7 +138,7 @@ static void host_wait(gq_ctx* ctx) {
     if (ctx->status_host && *ctx->status_host) {
         const uint32_t code = *ctx->status_host;
         *ctx->status_host = 0;
-        cudaMemset(ctx->paged_state, 0, paged_attn_state_bytes());  // a call that gave up may have left some of its arrivals
+        cudaMemsetAsync(ctx->paged_state, 0, paged_attn_state_bytes(), ctx->stream);  // a call that gave up may have left some of its arrivals
         if (code >= kStatusPeerWaitTimedOut)
             fail("a gather gave up waiting for rank %u's block of the output (code %u = 16 + the rank; the limit is set by "
                  "gq_set_wait_limit_us); its results are not valid", code - kStatusPeerWaitTimedOut, code);

@@ -165,6 +165,12 @@ int32_t gq_sample_rows(gq_ctx* ctx, gq_buf logits, uint64_t l_off, uint64_t rows
         auto dp = draws ? (uint32_t*)view(ctx, draws, 0, 1, 4, "gq_sample_rows draw counter") : nullptr;
         auto op = (int32_t*)view(ctx, tokens, 0, rows, 4, "gq_sample_rows tokens");
         auto rp = probs ? (float*)view(ctx, probs, 0, rows, 4, "gq_sample_rows probabilities") : nullptr;
+        // a row's CTAs read its settings, logits and numbers while other rows' results are written
+        const std::pair<const void*, uint64_t> read[] = {{lp, rows * vocab}, {tp, rows}, {kp, rows}, {pp, rows}, {mp, rows}, {up, uniform_rows * rows}, {dp, dp ? 1 : 0}};
+        for (const auto& in : read)
+            if (ranges_overlap(op, rows * 4, in.first, in.second * 4) || (rp && ranges_overlap(rp, rows * 4, in.first, in.second * 4)))
+                fail("gq_sample_rows: the outputs must not overlap the inputs");
+        if (rp && ranges_overlap(op, rows * 4, rp, rows * 4)) fail("gq_sample_rows: tokens and probabilities must not overlap");
         if (rows == 0) return;
         launch_sample_rows(ctx->stream, ctx->prop.multiProcessorCount, lp, (uint32_t)rows, (uint32_t)vocab, tp, kp, pp, mp, up, (uint32_t)uniform_rows, dp, op, rp,
                            (uint32_t*)ctx->sample_state);

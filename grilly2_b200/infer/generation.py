@@ -132,17 +132,19 @@ def generate_batch(model, prompts, generation_config: GenerationConfig | None = 
         setattr(config, k, v)
     if config.num_beams != 1:
         raise NotImplementedError("grilly: generate_batch() with num_beams > 1 (beam search) is not implemented yet")
+    if not config.use_cache:
+        raise NotImplementedError("grilly: generate_batch(use_cache=False) is not implemented yet")
     if config.repetition_penalty not in (None, 1.0):
         raise NotImplementedError("grilly: generate_batch() with a repetition penalty is not implemented yet")
     cfg = model.cfg
     new = [(config.max_new_tokens if config.max_new_tokens is not None else config.max_length - r.size) for r in rows]
     new = [max(v, 0) for v in new]
     steps = max(new)
-    if any(r.size + v > cfg.max_cache_len + 1 for r, v in zip(rows, new)):
-        raise RuntimeError(f"a request may hold {cfg.max_cache_len} cached positions; prompt + new tokens = "
-                           f"{max(r.size + v for r, v in zip(rows, new))}")
     if steps == 0:
         return [r.astype(np.int64) for r in rows]
+    held = [r.size + v - 1 if v else 0 for r, v in zip(rows, new)]  # cached positions: the last token never is, nor what asks for no token
+    if max(held) > cfg.max_cache_len:
+        raise RuntimeError(f"a request may hold {cfg.max_cache_len} cached positions; prompt + new tokens = {max(held) + 1}")
     sampled = _per_request("do_sample", config.do_sample, n, False, bool)
     heat = _per_request("temperature", config.temperature, n, 1.0, np.float32)
     if (sampled & ~(heat > 0)).any():
@@ -154,19 +156,20 @@ def generate_batch(model, prompts, generation_config: GenerationConfig | None = 
                 "min_p": T(_per_request("min_p", min_p, n, 0.0, np.float32))}
     eos = config.eos_token_id
     eos = set() if eos is None else {int(eos)} if isinstance(eos, (int, np.integer)) else {int(e) for e in eos}
-    if blocks is None:  # the last token is never cached
-        blocks = sum(-(-max(r.size + v - 1, 1) // block_size) for r, v in zip(rows, new))
+    if blocks is None:
+        blocks = sum(-(-h // block_size) for h in held)
     cache = PagedKvCache.for_model(cfg, seqs=n, blocks=blocks, block_size=block_size)
     uniforms = T((generator or _default_generator).uniform((steps, n)))
     draws, chosen = T(np.zeros(1, dtype=np.int32)), _C.Tensor.empty((n,), "int32")
-    counts, tokens = T(np.array([r.size for r in rows], dtype=np.int32)), T(np.concatenate(rows).astype(np.int32))
+    first = [r if v else r[:0] for r, v in zip(rows, new)]  # what runs as the prompts' step
+    counts, tokens = T(np.array([r.size for r in first], dtype=np.int32)), T(np.concatenate(first).astype(np.int32))
 
     def run(tokens, counts, step, max_count):
         cache.plan(counts, step)
         sample_rows(model.step_paged(tokens, cache, step, max_count=max_count), uniforms, draws=draws, tokens=chosen, **settings)
 
     prompt_step = PagedStep(cache, tokens.numel())
-    run(tokens, counts, prompt_step, max(r.size for r in rows))
+    run(tokens, counts, prompt_step, max(r.size for r in first))
     if prompt_step.shortfall():
         raise RuntimeError(f"the pool of {blocks} blocks cannot hold the prompts: {prompt_step.shortfall()} more are needed")
     step = PagedStep(cache, n)
@@ -182,8 +185,10 @@ def generate_batch(model, prompts, generation_config: GenerationConfig | None = 
     while True:
         for b, t in enumerate(chosen.numpy()):
             if running[b]:
+                if t < 0:
+                    raise RuntimeError(f"no token can be drawn for request {b}: its logits are no numbers")
                 out[b].append(int(t))
-                running[b] = len(out[b]) < rows[b].size + new[b] and int(t) not in eos and t >= 0
+                running[b] = len(out[b]) < rows[b].size + new[b] and int(t) not in eos
         over = [not r and not x for r, x in zip(running, gone)]
         if any(over):
             cache.release(T(np.array(over, dtype=np.int32)))

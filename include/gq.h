@@ -448,7 +448,8 @@ int32_t gq_paged_append(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer
  * skipped; a row that is left with none gives zeros. A row that sees a block whose scales are negative, no number or
  * beyond 2^90 (for values) is NaN. q and out float32 [max_tokens][heads dim], not overlapping; rows behind
  * starts[seqs] are left as they were. max_count is the largest counts[b] the caller expects (1 for a decode step): it chooses
- * how the work is cut, never what is computed. */
+ * how the work is cut, never what is computed (beyond the order of float32 sums). Uses the context's scratch, which grows on
+ * first use: one eager call with this dim before a capture. */
 int32_t gq_paged_attn(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer, gq_buf q, uint64_t heads, float scale, const gq_paged_step* step,
                       uint64_t max_count, gq_buf out);
 /* The next token of every row, each row with settings of its own (float32 or int32 [rows], on the device, so that a captured
@@ -459,7 +460,7 @@ int32_t gq_paged_attn(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer, 
  * the largest always stays. The draw is the inverse CDF in token order with u in [0, 1): the first kept token whose cumulative
  * weight exceeds u * total. u is uniforms[*draws % uniform_rows][row] (uniform_rows x rows floats), and the uint32 word
  * `draws` is advanced by one, so that a captured step takes the next numbers at each replay; draws == 0: the first row. temperature <= 0 takes the first largest. tokens: int32 per row, -1
- * where every logit is -inf; probs (0 = none) receives the token's share of what was kept. Sums and weights in 64 bits; tokens below
+ * where every logit is -inf; probs (0 = none) receives the token's share of what was kept; neither may overlap the inputs. Sums and weights in 64 bits; tokens below
  * exp(-64) of the largest weight are never drawn. vocab at most 2^23.
  * Replaces nothing of the reference: its sampler has one setting for all rows and no min_p (gq_sample). */
 int32_t gq_sample_rows(gq_ctx* ctx, gq_buf logits, uint64_t l_off, uint64_t rows, uint64_t vocab, gq_buf temperature, gq_buf top_k, gq_buf top_p,

@@ -104,6 +104,24 @@ def test_sampled_batch_is_seeded_and_settings_are_per_request():
     assert a[1].tolist() == greedy[1].tolist()
 
 
+def test_a_prompt_at_its_end_takes_no_room():
+    """A request that asks for no token is returned as it is, whatever its length, beside others that go on."""
+    from grilly2_b200.infer.generation import generate_batch
+    cfg, model, _ = build(26)
+    long, short = list(range(33)), [7, 8, 9]
+    got = generate_batch(model, [long, short, [1] * 120], max_length=33, block_size=16)
+    assert [len(x) for x in got] == [33, 33, 120] and got[0].tolist() == long
+    assert got[1].tolist() == generate_batch(model, [short], max_length=33, block_size=16)[0].tolist()
+    assert [x.tolist() for x in generate_batch(model, [long, short], max_new_tokens=0)] == [long, short]
+
+
+def test_logits_that_are_no_numbers_end_the_batch():
+    from grilly2_b200.infer.generation import generate_batch
+    cfg, model, _ = build(27)
+    with pytest.raises(RuntimeError, match="request 1"):
+        generate_batch(model, [[3, 4], [500]], max_new_tokens=3)  # no such token
+
+
 def test_refusals_of_the_batch():
     from grilly2_b200.infer.generation import generate_batch
     from grilly2_b200.infer.paged import PagedKvCache, PagedStep
@@ -114,6 +132,8 @@ def test_refusals_of_the_batch():
         generate_batch(model, PROMPTS, max_new_tokens=2, top_k=[1, 2])
     with pytest.raises(ValueError, match="not used by the model"):
         generate_batch(model, PROMPTS, max_new_tokens=2, banana=1)
+    with pytest.raises(NotImplementedError, match="use_cache"):
+        generate_batch(model, PROMPTS, max_new_tokens=2, use_cache=False)
     with pytest.raises(NotImplementedError, match="repetition"):
         generate_batch(model, PROMPTS, max_new_tokens=2, repetition_penalty=1.2)
     with pytest.raises(ValueError, match="temperature"):

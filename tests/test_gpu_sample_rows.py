@@ -134,5 +134,9 @@ def test_logits_at_an_offset_and_refusals():
         sample_rows(full(1.0), full(0.4), **args)
     with pytest.raises(RuntimeError, match="vocab > 0"):
         sample_rows(_C.Tensor.empty((2, 0), "float32"), full(0.4), **args)
+    with pytest.raises(RuntimeError, match="must not overlap the inputs"):
+        sample_rows(T(x).narrow_rows(0, 2), full(0.4), probs=args["temperature"], **args)
+    with pytest.raises(RuntimeError, match="must not overlap the inputs"):
+        sample_rows(T(x).narrow_rows(0, 2), full(0.4), tokens=args["top_k"], **args)
     empty = sample_rows(_C.Tensor.empty((0, 9), "float32"), _C.Tensor.empty((0,), "float32"), **{n: _C.Tensor.empty((0,), t.dtype) for n, t in args.items()})
     assert empty.numel() == 0
