@@ -596,34 +596,39 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                 mbar_arrive(p_full + wg);
             }
             if (t0 < t1) products(tile - 1), drain();
-            // the rows' sums over the keys, in a fixed order
+            // the rows' sums over the keys, in a fixed order: a lane gives away half of its rows with each step, until it has row
+            // lane / kShare
+            constexpr uint32_t kShare = 32 / R;
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                float v = l[r];
+            for (uint32_t w = R / 2, o = 16; o > 0; w >>= 1, o >>= 1) {
+                if (w == 0) l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-                if (lane == (uint32_t)r) lsum[quarter * RP + wrow + r] = v;
+                for (uint32_t i = 0; i < w; ++i) {
+                    const float keep = lane & o ? l[i + w] : l[i], give = lane & o ? l[i] : l[i + w];
+                    l[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                }
             }
-            named_barrier_sync(8, T::kSoft);
+            if (lane % kShare == 0) lsum[quarter * RP + wrow + lane / kShare] = l[0];
+            named_barrier_sync(8, T::kSoft);  // (the next segment's first barrier keeps lsum until all have read it)
             auto sum_of = [&](uint32_t r) { return (lsum[r] + lsum[RP + r]) + (lsum[2 * RP + r] + lsum[3 * RP + r]); };
             // a row that saw no key has neither sum and gives zeros
             auto share_of = [](float sum) { return sum == 0.0f ? 0.0f : __fdiv_rn(1.0f / kUnit, sum); };
             if (g.whole) {
-                // the rows' factors and places, once each (the arrays of the tile loop are free)
-                if (tid < RP) {
-                    row_scale[tid] = share_of(sum_of(tid));
-                    row_seen[tid] = tid < g.rows ? (int)((g.row0 + tid) / group * heads + (g.row0 + tid) % group) : -1;
+                float share = 0.0f;  // of row `lane`, and its place
+                int place = -1;
+                if (lane < (uint32_t)R) {
+                    const uint32_t row = g.row0 + wrow + lane;
+                    share = share_of(sum_of(wrow + lane));
+                    if (wrow + lane < g.rows) place = (int)(row / group * heads + row % group);
                 }
-                named_barrier_sync(8, T::kSoft);
                 float* at = out + ((size_t)g.start * heads + g.head * group) * DIM + comp;
-                if (owner)
-#pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        const int row = row_seen[wrow + r];
-                        if (row >= 0) at[(size_t)row * DIM] = O[r] * row_scale[wrow + r];
-                    }
-                named_barrier_sync(8, T::kSoft);  // lsum and the rows' arrays are free
                 mbar_arrive(seg_free + seg % kSegments);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const int row = __shfl_sync(0xffffffffu, place, r);
+                    const float v = O[r] * __shfl_sync(0xffffffffu, share, r);
+                    if (owner && row >= 0) at[(size_t)row * DIM] = v;
+                }
                 continue;
             }
             // a part of an item: what this CTA has, and the last CTA to arrive adds the parts up
