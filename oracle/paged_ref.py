@@ -97,9 +97,9 @@ def attend(q, kcodes, vcodes, kscale, vscale, table, lens, steps, scale):
 
     The allowance, per row and head, of the largest |value| it sees: a score is off by half a step of q's 23-bit fixed point
     on every component (2^-22 of max|q| times the sum of |k|) and by six float32 roundings of its own size, its weight by as much
-    and by 2^-21 for the exponential; numerator and denominator both. The weights are fixed-point numbers of 23 bits of the
-    largest of a tile: a uniform rounding error of +-2^-24 a key, at six standard deviations of the sum over n keys, over
-    the row's denominator (at least 1)."""
+    and by 2^-21 for the exponential; numerator and denominator both. The weights are whole numbers of 2^-23 of a reference
+    that never exceeds the row's largest contribution: a uniform rounding error of +-2^-24 a key, at six standard
+    deviations of the sum over n keys, over the row's denominator (at least 1)."""
     rows, heads, dim = q.shape
     blocks, kvh, bs, _ = kcodes.shape
     out, tol = np.zeros(q.shape), np.zeros((rows, heads))
