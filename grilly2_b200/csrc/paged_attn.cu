@@ -102,11 +102,9 @@ __device__ __forceinline__ float factor_of(float row, float key) {
     const float f = row * key;
     return f < 1e-37f ? 1e-37f : f;
 }
-// Three digit sums of up to 22 bits, joined with two roundings. The upper one becomes a float by an integer addition (it is
-// below 2^22), which spares the conversion pipe the exponentials go through.
+// three digit sums of up to 22 bits, joined with two roundings
 __device__ __forceinline__ float join(uint32_t d0, uint32_t d1, uint32_t d2) {
-    const float high = __int_as_float((int)d2 + 0x4b400000) - 12582912.0f;
-    return __fmaf_rn(high, 65536.0f, (float)((int)d0 + ((int)d1 << 8)));
+    return __fmaf_rn((float)(int)d2, 65536.0f, (float)((int)d0 + ((int)d1 << 8)));
 }
 
 // What the softmax needs to know of a block: x = its key scale; y = log2 of its value scale (of at least 2^-100) and a margin for the

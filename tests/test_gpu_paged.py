@@ -421,6 +421,37 @@ def test_a_captured_step_follows_the_device_state():
     np.testing.assert_array_equal(a.k.numpy(), b.k.numpy())
 
 
+def test_two_graphs_and_eager_calls_share_the_scratch():
+    """Captured steps of both kinds, replayed in turn with an eager step between, give what each gives alone."""
+    from grilly2_b200 import _C
+    rng = np.random.default_rng(31)
+    kinds = []
+    for lens, counts in (([900, 40, 2000], [1, 1, 1]), ([300, 0, 777], [60, 200, 31])):
+        t = filled(rng, 14, 2, 64, 64, lens, counts)
+        tokens = sum(counts)
+        st = t.Step(t.cache, tokens)
+        t.cache.plan(dev(np.array(counts, np.int32)), st)
+        q, out = dev((rng.standard_normal((tokens, 14 * 64))).astype(np.float32)), _C_filled((tokens, 14 * 64), 0.0)
+        kinds.append((lambda t=t, q=q, st=st, out=out, m=max(counts): t.cache.attend(0, q, 14, st, max_count=m, out=out), out))
+    alone = []
+    for call, out in kinds:
+        call()
+        alone.append(out.numpy())
+    graphs = []
+    for call, _ in kinds:
+        _C.begin_capture()
+        call()
+        graphs.append(_C.end_capture())
+    for turn in ((0, 1), (1, 0), (1, 1), (0, 0)):
+        for _, out in kinds:
+            out.copy_(_C_filled(out.shape, 9.0))
+        graphs[turn[0]].replay()
+        kinds[turn[1]][0]()
+        graphs[1 - turn[0]].replay()
+        for (_, out), want in zip(kinds, alone):
+            np.testing.assert_array_equal(out.numpy(), want)
+
+
 def test_the_same_call_twice_gives_the_same_bits():
     rng = np.random.default_rng(15)
     t = filled(rng, 14, 2, 64, 64, [3000, 10, 777], [1, 1, 1])
