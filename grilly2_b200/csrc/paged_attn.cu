@@ -18,9 +18,9 @@
 // and scaled afterwards, and the exponent is one multiplication and addition of the integer.
 // Scales of values from 2^-100 to 2^90 (and 0) lose nothing; larger, negative or non-finite ones read as NaN.
 //
-// A CTA takes a contiguous range of all (request, row tile, KV head, 128-key tile) units, equal ranges for all CTAs: with ragged
-// lengths no CTA waits for a long request, and a single request fills the GPU. A row tile is RP rows of (token, head of the
-// group), N = 3 RP digit rows. An (item = request, row tile, KV head) that ends inside one range is written out; the
+// A CTA takes a contiguous range of all (request, row tile, KV head, 128-key tile) units, with two more units for what an (item
+// = request, row tile, KV head) costs beside its tiles, equal ranges for all CTAs: with ragged lengths no CTA waits for a long request, and a single request fills the GPU. A row tile is RP rows of (token, head of the
+// group), N = 3 RP digit rows. An item that ends inside one range is written out; the
 // others leave (max, sum, weighted V) per CTA and the last CTA of an item to arrive adds them in order (deterministic).
 //   last warp      copies the tile's K and V blocks into a ring of stages (bulk copies; the table gives the addresses)
 //   the one before issues the products: S = K Q (128 x N) of the next tile as soon as S is read, D = V P (dim x N) when P is written
@@ -30,13 +30,13 @@
 //                  its float32 sums
 //
 // Bound, and what was measured (B200):
-//   long contexts (32 requests of 2000 to 15000 tokens, 32 heads over 8 of 128): the codes' bytes, 442 MB in 81 us = 5.4 TB/s
-//   one request, a small batch (700 tokens, 11.5 us; 64 requests of up to 4095 tokens, 24 MB, 20.1 us): latency. The units' scan,
+//   long contexts (32 requests of 2000 to 15000 tokens, 32 heads over 8 of 128): the codes' bytes, 442 MB in 80 us = 5.5 TB/s
+//   one request, a small batch (700 tokens, 11.5 us; 64 requests of up to 4095 tokens, 24 MB, 18.1 us): latency. The units' scan,
 //     the first blocks, three dependent steps a tile and the joining of the parts through L2 are some 10 us
-//   chunks of prompts (2 requests, 2795 rows over 3000 cached tokens each, 32 heads of 128): 174 GFLOP in 647 us. Three int8 products would take 157;
+//   chunks of prompts (2 requests, 2795 rows over 3000 cached tokens each, 32 heads of 128): 174 GFLOP in 640 us. Three int8 products would take 157;
 //     the float32 work beside them is 42 warp instructions per 32 scores, issued at 0.63 of the schedulers' rate
-//   short prompts (300 to 1100 tokens, 14 heads over 2 of 64): 116 us, a third of it an item's beginning and end (2500 cycles for q's
-//     digits, 2000 for the last sums and the output, beside 3300 a tile)
+//   short prompts (300 to 1100 tokens, 14 heads over 2 of 64): 79 us, a good third of it items' beginnings and ends (2500 cycles for
+//     q's digits, 3000 for the last sums and the output, beside 3300 a tile)
 #include "gq_internal.h"
 #include "paged.cuh"
 #include "tc_common.cuh"
@@ -136,16 +136,21 @@ __device__ uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
                                                         : floor_sum_in<uint64_t>(n, m, a, b);
 }
 
-// One request's share of the units. A row tile's units are the 128-key tiles that its last row sees: all of the request's
-// for the last row tile, floor((len + last token) / 128) + 1 for the others.
+// What an item's beginning and end cost, in tiles: q's digits, the last sums, the output. Where items have few tiles
+// ranges of equal tiles would leave some CTAs with many items (with 0 / 1 / 2 / 3 / 4: prompts of 300 to 1100 tokens
+// 115 / 84 / 79 / 82 / 84 us, 64 single tokens 20.2 / 18.8 / 18.1 / 18.6 / 18.8, chunks 646 / 643 / 640 / 640 / 638).
+constexpr uint32_t kItem = 2;
+
+// One request's share of the units. A row tile's units are kItem and the 128-key tiles that its last row sees: all of the
+// request's for the last row tile, floor((len + last token) / 128) + 1 for the others.
 struct Request {
     uint32_t start, rows, len, keys, tiles, row_tiles, group, kv_heads;  // keys = cached and new ones, inside the table
     uint32_t rp;
     __device__ uint32_t tiles_of(uint32_t qt) const { return qt + 1 == row_tiles ? tiles : (len + ((qt + 1) * rp - 1) / group) / kKeys + 1; }
     __device__ uint64_t units_before(uint32_t qt) const {  // qt < row_tiles
-        return qt ? kv_heads * (qt + floor_sum(qt, (uint64_t)kKeys * group, rp, (uint64_t)len * group + rp - 1)) : 0;
+        return qt ? kv_heads * ((uint64_t)qt * (1 + kItem) + floor_sum(qt, (uint64_t)kKeys * group, rp, (uint64_t)len * group + rp - 1)) : 0;
     }
-    __device__ uint64_t units() const { return row_tiles ? units_before(row_tiles - 1) + (uint64_t)kv_heads * tiles : 0; }
+    __device__ uint64_t units() const { return row_tiles ? units_before(row_tiles - 1) + (uint64_t)kv_heads * (tiles + kItem) : 0; }
 };
 __device__ __forceinline__ Request request_of(const PagedView& c, const StepView& s, uint32_t b, uint32_t group, uint32_t rp) {
     Request r;
@@ -166,7 +171,7 @@ struct Segment {
     uint32_t start, len, keys;   // of the request
     uint32_t whole, more;        // the item is this segment; 0: no segment, the end
     uint32_t c0, parts, second;  // the item's first CTA, how many have a part of it, whether the first one's is its second part
-    uint64_t first, last;        // the item's units [first, last)
+    uint64_t first, last;        // the item's units [first, last), of which the first kItem are no tiles
 };
 constexpr uint32_t kSegments = 4;  // of the ring
 
@@ -176,29 +181,34 @@ struct Walk {
     uint32_t b, qt;
     Request r;
     __device__ bool next(const PagedView& c, const StepView& s, Segment& g) {
-        g.more = u < hi;
-        if (!g.more) return false;
-        uint32_t tiles;
         for (;;) {
-            if (qt < r.row_tiles) {
-                tiles = r.tiles_of(qt);
-                if (u < base + (uint64_t)r.kv_heads * tiles) break;
-                base += (uint64_t)r.kv_heads * tiles, ++qt;
-            } else {
+            g.more = u < hi;
+            if (!g.more) return false;
+            const uint32_t cost = qt < r.row_tiles ? r.tiles_of(qt) + kItem : 0;  // of an item
+            if (cost == 0) {
                 r = request_of(c, s, ++b, r.group, r.rp), qt = 0;
+                continue;
             }
+            if (u >= base + (uint64_t)r.kv_heads * cost) {
+                base += (uint64_t)r.kv_heads * cost, ++qt;
+                continue;
+            }
+            const uint32_t v = (uint32_t)(u - base);
+            g.head = v / cost;
+            const uint32_t at = v - g.head * cost;  // of the item's units; the first kItem are no tiles
+            g.first = base + (uint64_t)g.head * cost, g.last = g.first + cost;
+            const uint64_t end = min(hi, g.last);
+            u = end;
+            if (end <= g.first + kItem) continue;  // none of the item's tiles
+            g.b = b, g.start = r.start, g.len = r.len, g.keys = r.keys;
+            g.whole = at <= kItem && end == g.last;
+            g.row0 = qt * r.rp, g.rows = min(r.rp, r.rows - g.row0);
+            const uint32_t seen = min(r.len + (g.row0 + g.rows - 1) / r.group + 1, r.keys);  // keys of the tile's last token
+            g.clear = min(r.len + g.row0 / r.group + 1, r.keys);
+            g.t0 = max(at, kItem) - kItem;
+            g.t1 = max(g.t0, min((uint32_t)(end - g.first) - kItem, (seen + kKeys - 1) / kKeys));
+            return true;
         }
-        const uint32_t v = (uint32_t)(u - base);
-        g.b = b, g.start = r.start, g.len = r.len, g.keys = r.keys, g.head = v / tiles, g.t0 = v - g.head * tiles;
-        g.first = base + (uint64_t)g.head * tiles, g.last = g.first + tiles;
-        const uint64_t end = min(hi, g.last);
-        g.whole = u == g.first && end == g.last;
-        g.row0 = qt * r.rp, g.rows = min(r.rp, r.rows - g.row0);
-        const uint32_t seen = min(r.len + (g.row0 + g.rows - 1) / r.group + 1, r.keys);  // keys of the tile's last token
-        g.clear = min(r.len + g.row0 / r.group + 1, r.keys);
-        g.t1 = max(g.t0, min(g.t0 + (uint32_t)(end - u), (seen + kKeys - 1) / kKeys));
-        u = end;
-        return true;
     }
 };
 
@@ -311,7 +321,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
             if (seg >= kSegments) ok = mbar_wait(seg_free + seg % kSegments, (seg / kSegments - 1) & 1, failed, status, kStatusEmptyWaitTimedOut);
             if (__ballot_sync(0xffffffffu, !ok)) ok = false;
             if (!ok) break;
-            if (more && !g.whole) g.c0 = cta_of(g.first), g.parts = cta_of(g.last - 1) - g.c0 + 1, g.second = range_at(g.c0) != g.first;
+            if (more && !g.whole) g.c0 = cta_of(g.first + kItem), g.parts = cta_of(g.last - 1) - g.c0 + 1, g.second = range_at(g.c0) < g.first;
             if (lane == 0) {
                 segments[seg % kSegments] = g;
                 mbar_arrive(seg_full + seg % kSegments);
@@ -716,7 +726,7 @@ template <bool ONE>
 void launch_blocks(cudaStream_t s, int sm_count, uint32_t* status, const PagedView& c, const StepView& st, const float* q, uint32_t heads, float scale,
                    uint64_t rows, float* out, void* state, void* scratch) {
     // Rows of a tile: as few as hold a request's rows while these are few, since a score costs the same whether its row is real
-    // or not. Tiles of 8 / 16 / 32 rows: 64 requests with one token of 7 heads a group 20.1 / 24.3 / 30.3 us, 32 long
+    // or not. Tiles of 8 / 16 / 32 rows (before items had units of their own): 64 requests with one token of 7 heads a group 20.1 / 24.3 / 30.3 us, 32 long
     // contexts of 4 heads a group 81 / 101 / 125; prompts of 300 to 1100 tokens 165 / 140 / 116, chunks of 1400 tokens
     // 1118 / 923 / 647. Many rows: 32 over two warpgroups, two CTAs an SM, took 638 us for the chunks and 112 for the
     // prompts, tiles of 40 rows 696 and 122, of 64 rows
