@@ -19,9 +19,9 @@
 // Scales of values from 2^-100 to 2^90 (and 0) lose nothing; larger, negative or non-finite ones read as NaN.
 //
 // A CTA takes a contiguous range of all (request, row tile, KV head, 128-key tile) units, with two more units for what an (item
-// = request, row tile, KV head) costs beside its tiles, equal ranges for all CTAs: with ragged lengths no CTA waits for a long request, and a single request fills the GPU. A row tile is RP rows of (token, head of the
-// group), N = 3 RP digit rows. An item that ends inside one range is written out; the
-// others leave (max, sum, weighted V) per CTA and the last CTA of an item to arrive adds them in order (deterministic).
+// = request, row tile, KV head) costs beside its tiles, equal ranges for all CTAs: with ragged lengths no CTA waits for a
+// long request, and a single request fills the GPU. A row tile is RP rows of (token, head of the group), N = 3 RP digit
+// rows. An item that ends inside one range is written out; the others leave (max, sum, weighted V) per CTA and the last CTA of an item to arrive adds them in order (deterministic).
 //   last warp      copies the tile's K and V blocks into a ring of stages (bulk copies; the table gives the addresses)
 //   the one before issues the products: S = K Q (128 x N) of the next tile as soon as S is read, D = V P (dim x N) when P is written
 //   4 WG warps     a thread owns a key of S and RP / WG rows: joins the digits, one maximum over the 128 keys per row (warp
@@ -31,11 +31,11 @@
 //
 // Bound, and what was measured (B200):
 //   long contexts (32 requests of 2000 to 15000 tokens, 32 heads over 8 of 128): the codes' bytes, 442 MB in 80 us = 5.5 TB/s
-//   one request, a small batch (700 tokens, 11.5 us; 64 requests of up to 4095 tokens, 24 MB, 18.1 us): latency. The units' scan,
+//   one request, a small batch (700 tokens, 11.3 us; 64 requests of up to 4095 tokens, 24 MB, 18.0 us): latency. The units' scan,
 //     the first blocks, three dependent steps a tile and the joining of the parts through L2 are some 10 us
-//   chunks of prompts (2 requests, 2795 rows over 3000 cached tokens each, 32 heads of 128): 174 GFLOP in 640 us. Three int8 products would take 157;
-//     the float32 work beside them is 42 warp instructions per 32 scores, issued at 0.63 of the schedulers' rate
-//   short prompts (300 to 1100 tokens, 14 heads over 2 of 64): 79 us, a good third of it items' beginnings and ends (2500 cycles for
+//   chunks of prompts (2 requests, 2795 rows over 3000 cached tokens each, 32 heads of 128): 174 GFLOP in 637 us. Three int8
+//     products would take 157; the float32 work beside them is 42 warp instructions per 32 scores, issued at 0.63 of the schedulers' rate
+//   short prompts (300 to 1100 tokens, 14 heads over 2 of 64): 78 us, a good third of it items' beginnings and ends (2500 cycles for
 //     q's digits, 3000 for the last sums and the output, beside 3300 a tile)
 #include "gq_internal.h"
 #include "paged.cuh"
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
             const int in = __ffs(__ballot_sync(0xffffffffu, walk.u >= upto - mine && walk.u < upto)) - 1;
             const uint32_t end = __shfl_sync(0xffffffffu, b1, in);
             walk.b = __shfl_sync(0xffffffffu, b0, in), walk.base = __shfl_sync(0xffffffffu, upto - mine, in), walk.qt = 0;
-            for (;;) {
+            while (per > 1) {
                 const uint64_t units = walk.b + lane < end ? request_of(c, s, walk.b + lane, group, RP).units() : 0, through = scanned(units);
                 const uint32_t hit = __ballot_sync(0xffffffffu, walk.u < walk.base + through);
                 const int at = hit ? __ffs(hit) - 1 : 31;
@@ -304,13 +304,16 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
             walk.r = request_of(c, s, walk.b, group, RP);
             if (walk.r.row_tiles > 1) {  // the last row tile that begins at or before u, 32 candidates a round
                 const uint64_t v = walk.u - walk.base;
+                uint64_t before = 0;
                 uint32_t lo = 0, hi = walk.r.row_tiles;
                 while (hi - lo > 1) {
                     const uint32_t step = (hi - lo + 31) / 32, k = lo + lane * step;
-                    const uint32_t at = 31 - __clz(__ballot_sync(0xffffffffu, k < hi && walk.r.units_before(k) <= v));
+                    const uint64_t units = k < hi ? walk.r.units_before(k) : ~0ull;
+                    const uint32_t at = 31 - __clz(__ballot_sync(0xffffffffu, units <= v));
+                    before = __shfl_sync(0xffffffffu, units, at);
                     lo += at * step, hi = min(hi, lo + step);
                 }
-                walk.base += walk.r.units_before(lo), walk.qt = lo;
+                walk.base += before, walk.qt = lo;
             }
         }
         uint32_t st = 0, round = 0;
@@ -321,21 +324,21 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
             if (seg >= kSegments) ok = mbar_wait(seg_free + seg % kSegments, (seg / kSegments - 1) & 1, failed, status, kStatusEmptyWaitTimedOut);
             if (__ballot_sync(0xffffffffu, !ok)) ok = false;
             if (!ok) break;
+            const int32_t* table = c.table + (more ? (size_t)g.b * c.max_blocks : 0);
+            auto entry = [&](uint32_t t) {  // one lane per block
+                const uint32_t j = t * per_tile + lane;
+                return t < g.t1 && lane < per_tile && (j << c.shift) < g.keys ? table[j] : -1;
+            };
+            int32_t e = more ? entry(g.t0) : -1;  // (requested before the divisions below)
             if (more && !g.whole) g.c0 = cta_of(g.first + kItem), g.parts = cta_of(g.last - 1) - g.c0 + 1, g.second = range_at(g.c0) < g.first;
             if (lane == 0) {
                 segments[seg % kSegments] = g;
                 mbar_arrive(seg_full + seg % kSegments);
             }
             if (!more) break;
-            const int32_t* table = c.table + (size_t)g.b * c.max_blocks;
-            auto entry = [&](uint32_t t) {  // one lane per block
-                const uint32_t j = t * per_tile + lane;
-                const int32_t e = t < g.t1 && lane < per_tile && (j << c.shift) < g.keys ? table[j] : -1;
-                return e >= 0 && (uint32_t)e < c.blocks ? e : -1;
-            };
-            int32_t e = entry(g.t0);
             for (uint32_t t = g.t0; t < g.t1; ++t) {
                 const int32_t e_next = entry(t + 1);
+                e = e >= 0 && (uint32_t)e < c.blocks ? e : -1;
                 const size_t at = ((size_t)max(e, 0) * c.kv_heads + g.head);
                 const float ks = e >= 0 ? c.kscale[at] : 0.0f, vs = e >= 0 ? c.vscale[at] : 0.0f;
                 if (round) ok = ok && mbar_wait(empty + st, (round - 1) & 1, failed, status, kStatusEmptyWaitTimedOut);
