@@ -7,7 +7,7 @@
 // k_j = kscale_j K_j with 128 keys on the lanes of tensor memory, v_j = vscale_j V_j with the components on the lanes. What
 // meets them is held as an exact fixed-point integer in three base-256 digits, so three products in int32 and one join
 // give a float32 result:
-//   q_r = max|q_r| / 8323072 Q, Q in signed digits (8323072 = 127 * 2^16, what they hold); kscale_j is a factor of a lane;
+//   q_r = max|q_r| / (127 * 2^16) Q, Q in signed digits (which hold 127 * 2^16); kscale_j is a factor of a lane;
 //   w vscale = 2^-23 P, P in unsigned digits. The value scales are folded into P because the sum over j runs across blocks;
 //     so that P fits, the reference of a row is the running maximum of s + log2 vscale (the largest contribution, not the largest
 //     score) and P's steps are 2^-23 of the largest contribution so far, whatever the blocks' scales are. The denominator
@@ -50,7 +50,7 @@ constexpr float kNone = -INFINITY;
 constexpr uint32_t kMostPerSm = 4;  // CTAs of an SM
 constexpr float kUnit = 8388608.0f;  // 2^23: P's steps of the reference; P passes it by a factor of 2 at most, so it has 24 bits,
                                      // the upper ones of a word whose conversion stops at 2^32 of itself
-constexpr float kQMost = 8323072.0f;  // 127 * 2^16
+constexpr float kQMost = 127.0f * 65536.0f;
 
 template <int RP, int WG, int DIM>
 struct Split {
@@ -484,7 +484,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                     uint32_t w0 = 0, w1 = 0, w2 = 0;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        int Q = __float2int_rn(x[j] * mult);  // +-q in steps of its row; |Q| <= 8323072
+                        int Q = __float2int_rn(x[j] * mult);  // +-q in steps of its row; |Q| <= 127 * 2^16
                         const int d0 = (int)(int8_t)Q;
                         Q = (Q - d0) >> 8;
                         const int d1 = (int)(int8_t)Q, d2 = (Q - d1) >> 8;
