@@ -128,6 +128,9 @@ void check_dims(const char* op, uint64_t a, uint64_t b, uint64_t c = 1);
 // is read or written before the wait); what is saved is the launch gap. A kernel lets the one behind it start only AFTER its
 // own wait has returned, so whatever runs early in that next kernel knows that everything up to the kernel before this one is
 // complete: the only writes in doubt are this kernel's own. Inside a capture the edge is recorded as such.
+// Tensor memory is allocated behind the wait: an allocation blocks, without a limit, until the columns are free, and a kernel
+// ahead may still be about to make its own while it holds this one at its wait. A kernel that a call launches right behind its
+// own conversion of x (which has no tensor memory and has waited) may allocate earlier, and let the next one start earlier.
 #ifdef __CUDACC__
 #define GQ_GRID_DEP_SYNC()                                                  \
     do {                                                                    \

@@ -217,6 +217,9 @@ template <int RP, int WG, int DIM, bool ONE>
 __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG, DIM>::kPerSm))
     paged_attn_kernel(PagedView c, StepView s, const float* __restrict__ q, uint32_t heads, float scale, float* __restrict__ out,
                       float* __restrict__ partials, uint32_t* counters, uint32_t* status) {
+    // Before anything else, the tensor memory above all: a kernel ahead that lets this one start before it has its own columns
+    // would wait for those held here, and this one for its end.
+    GQ_GRID_DEP_SYNC();
     using T = Split<RP, WG, DIM>;
     constexpr int R = T::kRows;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -258,7 +261,6 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = *tmem_slot;
-    GQ_GRID_DEP_SYNC();
 
     bool ok = true;
 
