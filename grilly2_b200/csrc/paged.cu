@@ -3,7 +3,8 @@
 //
 // plan: the new tokens of every request get positions, rows, blocks and slots. With c_b = counts[b] and n_b = lens[b]:
 //   starts = exclusive sum of c; request b touches the table entries n_b / bs .. (n_b + c_b - 1) / bs, one RUN of rows each;
-//   the r-th touched entry without a block, in order of (b, entry), takes free[free_count - 1 - r];
+//   the r-th touched entry without a block, in order of (b, entry), takes free[free_count - 1 - r] — unless n_b lies inside it:
+//   then its earlier tokens found no room, and a block given now would be read as if it held them;
 //   slot = table[b][p / bs] * bs + p % bs for p = n_b + (row - starts[b]).
 // Both sums are block scans over the requests; runs and rows find their request by a binary search in shared memory. Few
 // rows run as one CTA; many as a cluster of eight, whose first CTA hands out the blocks while the cluster barrier holds
@@ -74,12 +75,13 @@ __global__ void __launch_bounds__(NT) paged_plan_kernel(PagedView c, StepView s,
                                                                  const int32_t* __restrict__ free_list, int32_t* free_count) {
     GQ_GRID_DEP_SYNC();
     extern __shared__ uint32_t smem[];
-    __shared__ uint32_t warp_sums[32];
+    __shared__ uint32_t warp_sums[32], refused;
     uint32_t* start = smem;                  // [seqs + 1]
     uint32_t* run = start + c.seqs + 1;      // [seqs + 1]
     uint32_t* len = run + c.seqs + 1;        // [seqs]
     const uint32_t tid = threadIdx.x, per = (c.seqs + NT - 1) / NT, b0 = tid * per, b1 = min(b0 + per, c.seqs);
     uint32_t total, runs, sum = 0;
+    if (tid == 0) refused = 0;
     for (uint32_t b = b0; b < b1; ++b) sum = min(sum + min((uint32_t)max(counts[b], 0), s.tokens), s.tokens);
     uint32_t at = block_scan<NT>(sum, s.tokens, warp_sums, &total);
     sum = 0;
@@ -105,7 +107,7 @@ __global__ void __launch_bounds__(NT) paged_plan_kernel(PagedView c, StepView s,
         uint32_t wanted = 0;
         for (uint32_t r0 = 0; r0 < runs; r0 += kAtOnce * NT) {
             int32_t* entry[kAtOnce];
-            uint32_t need = 0, packed_lo = 0, packed_hi = 0;  // four counts of 16 bits, one for each slab of NT runs
+            uint32_t need = 0, inside = 0, packed_lo = 0, packed_hi = 0;  // four counts of 16 bits, one for each slab of NT runs
 #pragma unroll
             for (uint32_t k = 0; k < kAtOnce; ++k) {
                 const uint32_t r = r0 + k * NT + tid;
@@ -114,11 +116,15 @@ __global__ void __launch_bounds__(NT) paged_plan_kernel(PagedView c, StepView s,
                     const uint32_t b = owner_of(run, c.seqs, r), j = (len[b] >> c.shift) + (r - run[b]);
                     s.runs[r] = (int32_t)(r == run[b] ? start[b] : start[b] + ((j << c.shift) - len[b]));
                     if (j < c.max_blocks) entry[k] = c.table + (size_t)b * c.max_blocks + j;
+                    if ((j << c.shift) < len[b]) inside |= 1u << k;
                 }
             }
 #pragma unroll
             for (uint32_t k = 0; k < kAtOnce; ++k)
-                if (entry[k] && *entry[k] < 0) need |= 1u << k;
+                if (entry[k] && *entry[k] < 0) {
+                    if (inside >> k & 1) atomicAdd(&refused, 1u);  // (rare; the scan's barriers publish it)
+                    else need |= 1u << k;
+                }
             packed_lo = (need & 1) | (need & 2) << 15, packed_hi = (need >> 2 & 1) | (need & 8) << 13;
             uint32_t all_lo, all_hi = 0, before_hi = 0;
             const uint32_t before_lo = block_scan<NT>(packed_lo, 0xffffffffu, warp_sums, &all_lo);
@@ -139,7 +145,7 @@ __global__ void __launch_bounds__(NT) paged_plan_kernel(PagedView c, StepView s,
         }
         if (tid == 0) {  // every thread read *free_count before the scans' barriers (or nothing was wanted)
             if (wanted) *free_count = (int32_t)(have - min(wanted, have));
-            s.info[0] = (int32_t)total, s.info[1] = (int32_t)(wanted - min(wanted, have));
+            s.info[0] = (int32_t)total, s.info[1] = (int32_t)(wanted - min(wanted, have) + refused);
         }
     }
     if (gridDim.x > 1) cluster_barrier();

@@ -160,5 +160,6 @@ class PagedStep:
         self._ref = ctypes.byref(self._desc)
 
     def shortfall(self) -> int:
-        """Blocks the last plan wanted when the free list was empty (a host copy; waits for the device)."""
+        """Blocks that the last plan's rows lack: the free list was empty, then or when the entry's first tokens came (a host
+        copy; waits for the device)."""
         return int(self.info.numpy()[1])

@@ -414,7 +414,7 @@ typedef struct gq_paged_cache {
  *   runs      [GQ_PAGED_RUNS(max_tokens, block_size, seqs) + 1]  the first row of each stretch of rows that share a block;
  *             behind the last one starts[seqs]
  *   last      [seqs]        the last row of request b, -1 where it has none
- *   info      [2]           rows in use; blocks that were wanted when the free list was empty */
+ *   info      [2]           rows in use; blocks that its rows lack, as gq_paged_plan says */
 typedef struct gq_paged_step {
     uint64_t max_tokens;
     gq_buf starts, slots, positions, runs, last, info;
@@ -425,11 +425,13 @@ typedef struct gq_paged_step {
          : (uint64_t)(max_tokens) / (block_size) + 2 * (uint64_t)(seqs))
 /* The step's maps from the requests' lengths: counts[b] (int32, negative = 0) new tokens for request b, at positions
  * lens[b] .. lens[b] + counts[b] - 1. Where these reach a table entry without a block one is taken off the free list (int32
- * [blocks], of which the first *free_count are free; the last is taken first), in order of (b, entry). Rows beyond max_tokens
- * are cut; tokens beyond max_blocks * block_size, or without a block because the list is empty, get slot -1. lens is not
- * advanced (gq_paged_advance), so calling it again gives the same maps and takes no more blocks. */
+ * [blocks], of which the first *free_count are free; the last is taken first), in order of (b, entry). An entry that lens[b]
+ * lies inside gets none: its earlier tokens were advanced over without room, and whatever a block holds would be read as
+ * theirs; the request has blocks again from its next entry on. Rows beyond max_tokens are cut; tokens beyond max_blocks *
+ * block_size, or without a block, get slot -1. info[1] counts the entries left without a block, by an empty list or by that rule.
+ * lens is not advanced (gq_paged_advance), so calling it again gives the same maps and takes no more blocks. */
 int32_t gq_paged_plan(gq_ctx* ctx, const gq_paged_cache* cache, gq_buf counts, gq_buf free_list, gq_buf free_count, const gq_paged_step* step);
-/* lens[b] += the step's rows of request b (at most max_blocks * block_size): once per step, behind the last layer. */
+/* lens[b] += the step's rows of request b (at most max_blocks * block_size), with or without room: once per step, behind the last layer. */
 int32_t gq_paged_advance(gq_ctx* ctx, const gq_paged_cache* cache, const gq_paged_step* step);
 /* For every b with which[b] != 0 (int32 [seqs]): its blocks go back on the free list in table order, its table entries become -1
  * and lens[b] 0. A block that several requests name must not be released through more than one of them. */

@@ -30,6 +30,7 @@ def runs_cap(tokens, bs, seqs):
 def plan(lens, counts, table, free, free_count, bs, blocks, tokens):
     """The step's maps; table (updated in place), free_count after."""
     seqs, mb = table.shape
+    refused = 0
     starts, slots, positions, runs, last = [0], np.full(tokens, -1, np.int32), np.full(tokens, -1, np.int32), [], np.full(seqs, -1, np.int32)
     have = min(max(int(free_count), 0), blocks)
     wanted = 0
@@ -41,9 +42,12 @@ def plan(lens, counts, table, free, free_count, bs, blocks, tokens):
             if p == n or p % bs == 0:
                 runs.append(row)
                 if j < mb and table[b, j] < 0:
-                    if wanted < have:
-                        table[b, j] = free[have - 1 - wanted]
-                    wanted += 1
+                    if p % bs:  # its earlier tokens found no room: a block given now would be read as theirs
+                        refused += 1
+                    else:
+                        if wanted < have:
+                            table[b, j] = free[have - 1 - wanted]
+                        wanted += 1
             if j < mb and 0 <= table[b, j] < blocks:
                 slots[row] = table[b, j] * bs + p % bs
             positions[row] = p
@@ -54,7 +58,7 @@ def plan(lens, counts, table, free, free_count, bs, blocks, tokens):
     cap = runs_cap(tokens, bs, seqs)
     return {"starts": np.array(starts, np.int32), "slots": slots, "positions": positions, "last": last,
             "runs": np.array(runs + [starts[-1]] * (cap + 1 - len(runs)), np.int32),
-            "info": np.array([starts[-1], wanted - min(wanted, have)], np.int32)}, have - min(wanted, have)
+            "info": np.array([starts[-1], wanted - min(wanted, have) + refused], np.int32)}, have - min(wanted, have)
 
 
 def rotate(x, cos, sin):

@@ -1,0 +1,46 @@
+"""The paged int8 cache where it could go wrong beside the cases of test_gpu_paged.py, whose twin of device and checker this uses:
+pools that run out and are filled again, contributions far apart, batches of many requests, sums near the ends of their range."""
+import numpy as np
+import pytest
+
+from test_gpu_paged import Twin, _C_filled, attend, dev, filled, words
+
+pytestmark = pytest.mark.gpu
+
+
+def test_a_request_never_reads_what_another_left_in_its_block():
+    """A pool that is full drops tokens of a request; the block it gets later, in the middle of that block's positions, held
+    another request's keys. Outputs and maps are those of a pool in which the other request never was."""
+    outs = []
+    for other in (9.0, 0.0):
+        t = Twin(np.random.default_rng(41), seqs=2, heads=2, kvh=1, dim=32, bs=16, mb=3, blocks=2, layers=1, layer=0)
+        st, want, _ = t.step([16, 16], qkv=_rows(1, 32, 4, 32, [1.0] * 16 + [other] * 16))
+        t.advance(st, want)
+        st, want, turned = t.step([1, 0], qkv=_rows(2, 1, 4, 32, [1.0]))  # position 16: no block is free
+        assert want["info"][1] == 1 and step_info(st) == 1 and want["slots"][0] == -1
+        t.advance(st, want)
+        t.cache.release(dev(np.array([0, 1], np.int32)))
+        t.free, t.count = t.cache.free.numpy(), t.cache.free_blocks()
+        t.lens[1], t.table[1] = 0, -1
+        got = []
+        for i in range(16):  # positions 17 .. 32; from 32 on there is a block again
+            st, want, turned = t.step([1, 0], qkv=_rows(3 + i, 1, 4, 32, [1.0]))
+            np.testing.assert_array_equal(st.slots.numpy(), want["slots"])
+            np.testing.assert_array_equal(st.info.numpy(), want["info"])
+            np.testing.assert_array_equal(t.cache.table.numpy(), t.table)
+            assert (want["slots"][0] < 0) == (i < 15) and want["info"][1] == (i < 15)
+            t.check_pool()
+            t.check_attention(st, want, turned, max_count=1)
+            got.append(t.cache.attend(0, dev(turned.reshape(1, -1)), 2, st, max_count=1).numpy())
+            t.advance(st, want)
+        outs.append(got)
+    np.testing.assert_array_equal(outs[0], outs[1])
+
+
+def _rows(seed, n, heads, dim, sizes):
+    x = np.random.default_rng(seed).standard_normal((n, heads, dim)) * np.array(sizes)[:, None, None]
+    return x.astype(np.float32)
+
+
+def step_info(st):
+    return int(st.info.numpy()[1])
