@@ -631,8 +631,9 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
             if (lane % kShare == 0) lsum[quarter * RP + wrow + lane / kShare] = l[0];
             named_barrier_sync(8, T::kSoft);  // (the next segment's first barrier keeps lsum until all have read it)
             auto sum_of = [&](uint32_t r) { return (lsum[r] + lsum[RP + r]) + (lsum[2 * RP + r] + lsum[3 * RP + r]); };
-            // a row that saw no key has neither sum and gives zeros
-            auto share_of = [](float sum) { return sum == 0.0f ? 0.0f : __fdiv_rn(1.0f / kUnit, sum); };
+            // a row that saw no key has neither sum and gives zeros. (P's unit is taken out of the other sum: where value scales are near
+            // 2^-100, so that the weights' sum is beyond 2^100, the quotient would leave the normal numbers with it.)
+            auto share_of = [](float sum) { return sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum); };
             if (g.whole) {
                 float share = 0.0f;  // of row `lane`, and its place
                 int place = -1;
@@ -646,7 +647,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     const int row = __shfl_sync(0xffffffffu, place, r);
-                    const float v = O[r] * __shfl_sync(0xffffffffu, share, r);
+                    const float v = O[r] * (1.0f / kUnit) * __shfl_sync(0xffffffffu, share, r);
                     if (owner && row >= 0) at[(size_t)row * DIM] = v;
                 }
                 continue;
@@ -701,7 +702,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                 for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                 const float factor = share_of(sum);
 #pragma unroll
-                for (uint32_t d = 0; d < kVec; ++d) out_at(r)[lane + 32 * d] = acc[d] * factor;
+                for (uint32_t d = 0; d < kVec; ++d) out_at(r)[lane + 32 * d] = acc[d] * (1.0f / kUnit) * factor;
             }
             mbar_arrive(seg_free + seg % kSegments);
         }

@@ -44,3 +44,24 @@ def _rows(seed, n, heads, dim, sizes):
 
 def step_info(st):
     return int(st.info.numpy()[1])
+
+
+# ── contributions far apart ────────────────────────────────────────────────
+
+
+def put(t):
+    """The twin's codes and scales on the device."""
+    for name, a in (("k", words(t.ref.pack_k(t.codes["k"]))), ("v", words(t.ref.pack_v(t.codes["v"]))), ("kscale", dev(t.scales["k"])), ("vscale", dev(t.scales["v"]))):
+        on = getattr(t.cache, name)
+        on.copy_(a.reshape(on.shape))
+
+
+@pytest.mark.parametrize("counts", [[1], [33]], ids=["token", "prompt"])
+def test_value_scales_at_the_lower_end(counts):
+    """Thousands of keys of about equal weight, value scales of 2^-100: the sums' quotients stay normal numbers."""
+    rng = np.random.default_rng(53)
+    t = filled(rng, 2, 1, 64, 64, [5000], counts, spread=0.0)
+    t.codes["v"] = np.abs(t.codes["v"])
+    t.scales["v"][:] = np.float32(2.0 ** -100)
+    put(t)
+    attend(t, counts, scale=1e-3)
