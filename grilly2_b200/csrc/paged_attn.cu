@@ -5,18 +5,22 @@
 //
 // The cached codes are the A operand exactly as they lie in the pool (its blocks are core matrices of 8 x 16 bytes):
 // k_j = kscale_j K_j with 128 keys on the lanes of tensor memory, v_j = vscale_j V_j with the components on the lanes. What
-// meets them is held as an exact fixed-point integer in three base-256 digits, so three products in int32 and one join
+// meets them is held as an exact fixed-point integer in base-256 digits, so that three or four products in int32 and one join
 // give a float32 result:
-//   q_r = max|q_r| / (127 * 2^16) Q, Q in signed digits (which hold 127 * 2^16); kscale_j is a factor of a lane;
-//   w vscale = 2^-23 P, P in unsigned digits. The value scales are folded into P because the sum over j runs across blocks;
-//     so that P fits, the reference of a row is the running maximum of s + log2 vscale (the largest contribution, not the largest
-//     score) and P's steps are 2^-23 of the largest contribution so far, whatever the blocks' scales are. The denominator
-//     sums the w themselves in float32. The reference stays until it is passed by a factor of 2: as long as no row of a warpgroup
-//     passes it D goes on adding up in int32, and is read, joined and added to the float32 sums only when one does (or
-//     after 256 tiles, before a sum could leave 32 bits).
+//   q_r = max|q_r| / (127 * 2^16) Q, Q in three signed digits (which hold 127 * 2^16); kscale_j is a factor of a lane;
+//   w vscale = 2^-31 P, P in four unsigned digits. The value scales are folded into P because the sum over j runs across blocks:
+//     so that P fits, the reference of a row's P is one of its contributions' s + log2 vscale (not of the scores). It follows the
+//     tiles of 128 keys: up where a tile's largest contribution passes it, down where that lies 2^10 below it, so that what
+//     an attention sink outweighs keeps its digits: a weight is off by 2^-32 of a reference that lies 2^11 above its own tile's
+//     largest at most, 2^4 in the usual case. (Three digits and one reference per row lost what lay 2^-24 below the row's largest: 1e-4 of
+//     the row where a key of no value stood 10 nats above 4095 others, 2e-2 at 17 nats; now 4e-7 and 2e-5. They took 632 us
+//     for the chunks below and 77 for the prompts.) The denominator sums the w themselves in float32, in P's reference.
+// As long as no row of a warpgroup moves its reference D goes on adding up in int32, and is read, joined and added to the float32
+// sums only when one does (or after 256 tiles, before a sum could leave 32 bits). References are whole numbers, so sums follow them exactly.
 // A warp's 32 keys share one block and so one scale (blocks of 32 and more): the maximum is taken over the joined integers
 // and scaled afterwards, and the exponent is one multiplication and addition of the integer.
-// Scales of values from 2^-100 to 2^90 (and 0) lose nothing; larger, negative or non-finite ones read as NaN.
+// Scales of values from 2^-100 to 2^90 (and 0) lose nothing; larger, negative or non-finite ones read as NaN. (Below 2^-34 P's
+// reference follows the tiles less far down, so that the weights' sum stays a number.)
 //
 // A CTA takes a contiguous range of all (request, row tile, KV head, 128-key tile) units, with two more units for what an (item
 // = request, row tile, KV head) costs beside its tiles, equal ranges for all CTAs: with ragged lengths no CTA waits for a
@@ -31,11 +35,12 @@
 //
 // Bound, and what was measured (B200):
 //   long contexts (32 requests of 2000 to 15000 tokens, 32 heads over 8 of 128): the codes' bytes, 442 MB in 80 us = 5.5 TB/s
-//   one request, a small batch (700 tokens, 11.3 us; 64 requests of up to 4095 tokens, 24 MB, 18.0 us): latency. The units' scan,
+//   one request, a small batch (700 tokens, 11.7 us; 64 requests of up to 4095 tokens, 24 MB, 18.2 us): latency. The units' scan,
 //     the first blocks, three dependent steps a tile and the joining of the parts through L2 are some 10 us
-//   chunks of prompts (2 requests, 2795 rows over 3000 cached tokens each, 32 heads of 128): 174 GFLOP in 637 us. Three int8
-//     products would take 157; the float32 work beside them is 42 warp instructions per 32 scores, issued at 0.63 of the schedulers' rate
-//   short prompts (300 to 1100 tokens, 14 heads over 2 of 64): 78 us, a good third of it items' beginnings and ends (2500 cycles for
+//   chunks of prompts (2 requests, 2795 rows over 3000 cached tokens each, 32 heads of 128): 174 GFLOP in 652 us. Three int8
+//     products for S and four for D would take 184; the float32 work beside them is some 44 warp instructions per 32 scores, issued at 0.6 of
+//     the schedulers' rate
+//   short prompts (300 to 1100 tokens, 14 heads over 2 of 64): 81 us, a good third of it items' beginnings and ends (2500 cycles for
 //     q's digits, 3000 for the last sums and the output, beside 3300 a tile)
 #include "gq_internal.h"
 #include "paged.cuh"
@@ -48,36 +53,50 @@ namespace {
 constexpr uint32_t kKeys = 128;    // keys of a tile
 constexpr float kNone = -INFINITY;
 constexpr uint32_t kMostPerSm = 4;  // CTAs of an SM
-constexpr float kUnit = 8388608.0f;  // 2^23: P's steps of the reference; P passes it by a factor of 2 at most, so it has 24 bits,
-                                     // the upper ones of a word whose conversion stops at 2^32 of itself
+constexpr float kUnit = 2147483648.0f;  // 2^31: P's steps of the reference; P passes it by a factor of 2 at most and so has 32 bits
+// (all log2) how far above a tile's largest contribution its reference is laid where the quarters' largest lie within kEven of each
+// other, and how far below the reference a later tile's may fall before that follows
+constexpr float kRoom = 4.0f, kEven = 8.0f, kDrop = 6.0f;
 constexpr float kQMost = 127.0f * 65536.0f;
 
 template <int RP, int WG, int DIM>
 struct Split {
     static constexpr int kRows = RP / WG;                                        // rows of a thread
     static constexpr int kSoft = 128 * WG, kThreads = kSoft + 64;                // softmax threads; all
-    static constexpr uint32_t kNw = (3 * kRows + 15) / 16 * 16, kN = WG * kNw;   // columns: digit d of a warpgroup's row r in its column d kRows + r
-    static constexpr uint32_t kCols = kN <= 32 ? 32 : kN <= 64 ? 64 : 128;       // S at column 0, D at kCols
+    static constexpr uint32_t kNw = (3 * kRows + 15) / 16 * 16, kN = WG * kNw;   // columns of S: digit d of a warpgroup's row r in its column d kRows + r
+    static constexpr uint32_t kDw = 4 * kRows, kD = WG * kDw;                    // of D
+    // bytes from a core matrix of P to that of the next 16 keys: 128 would have the two halves of a warp write the same banks
+    static constexpr uint32_t kPStep = RP == 32 ? 192 : 128;
+    static constexpr uint32_t kCols = kD <= 32 ? 32 : kD <= 64 ? 64 : 128;       // S at column 0, D at kCols (three digits' columns are fewer than four's)
     static constexpr uint32_t kM = DIM == 128 ? 128 : 64;                        // lanes of D: dim, at least 64
     static constexpr uint32_t kTileBytes = kKeys * DIM, kStageBytes = 2 * kTileBytes;
     static constexpr uint32_t kStages = DIM == 128 ? 2 : DIM == 64 ? 3 : 4;
     // (dim 32: the 64 lanes of D read 32 rows that are not there, up to 4 KB behind the last stage; nobody reads the sums)
     static constexpr uint32_t kQAt = kStages * kStageBytes + (DIM == 32 ? 4096 : 0);
-    static constexpr uint32_t kPAt = kQAt + kN * DIM, kMiscAt = kPAt + kN * kKeys;
+    static constexpr uint32_t kPAt = kQAt + kN * DIM, kMiscAt = kPAt + kD * (kKeys / 16) * (kPStep / 8);
     // blocks' scales of each stage; rows' arrays: scale, last position seen, [4] sums, [2][4] maxima, [4] raw maximum or factor,
-    // reference and correction of each warp
-    static constexpr uint32_t kSmem = kMiscAt + 1024 + kStages * 128 + RP * 4 * (1 + 1 + 4 + 8 + 12);
+    // reference of O and (negative) of P, corrections of O and l, lift and the lift of what D holds, of each warp
+    static constexpr uint32_t kSmem = kMiscAt + 1024 + kStages * 128 + RP * 4 * (1 + 1 + 4 + 8 + 28);
     // CTAs of an SM: what shared memory and tensor memory hold
     static constexpr uint32_t kBySmem = (227 * 1024) / (kSmem + 1024), kByTmem = 512 / (2 * kCols), kHeld = kBySmem < kByTmem ? kBySmem : kByTmem;
     static constexpr uint32_t kMost = RP == 16 ? 3 : kMostPerSm;  // (registers)
     static constexpr uint32_t kPerSm = kHeld < kMost ? kHeld : kMost;
     static_assert(kPerSm >= 1 && kPerSm * RP <= kMostPerSm * 32, "the scratch holds the parts");
+    static_assert(kN <= kCols, "S and D lie side by side");
 };
 
 __device__ __forceinline__ float warp_max(float v) {  // the largest that is a number
     float r;
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
     return r;
+}
+template <int N>
+struct Rows {
+    static constexpr int value = N;
+};
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[8]) { tmem_ld8(addr, r); }
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 // a barrier of the softmax threads that tells every one of them whether all say yes
 __device__ __forceinline__ bool all_of(bool mine, uint32_t threads) {
@@ -102,17 +121,20 @@ __device__ __forceinline__ float factor_of(float row, float key) {
     const float f = row * key;
     return f < 1e-37f ? 1e-37f : f;
 }
+// 2^n for a whole n of at most 127, 0 below the normal numbers (and for what is no number)
+__device__ __forceinline__ float power_of_two(float n) { return n > -127.0f ? __int_as_float(((int)n + 127) << 23) : 0.0f; }
 // three digit sums of up to 22 bits, joined with two roundings
 __device__ __forceinline__ float join(uint32_t d0, uint32_t d1, uint32_t d2) {
     return __fmaf_rn((float)(int)d2, 65536.0f, (float)((int)d0 + ((int)d1 << 8)));
 }
 
-// What the softmax needs to know of a block: x = its key scale; y = log2 of its value scale (of at least 2^-100) and a margin for the
-// rounding, so that P stays below 2^24; z = the value scale times 2^31; w = 0, 1 where a scale is none (negative, beyond 2^90 or
+// What the softmax needs to know of a block: x = its key scale; y = log2 of its value scale (of at least 2^-100; of a scale of 0, which
+// contributes to the weights' sum alone, as if it were 2^-60) and a margin for the
+// rounding, so that P stays below 2^32; z = the value scale times 2^31; w = 0, 1 where a scale is none (negative, beyond 2^90 or
 // no number; x is 1 then), 2 where there is no block.
 __device__ __forceinline__ float4 block_scale(float ks, float vs) {
     const bool good = vs >= 0.0f && vs <= 1.2379401e27f && ks >= 0.0f && ks <= 3.0e38f;
-    return make_float4(good ? ks : 1.0f, fmaxf(__log2f(vs), -100.0f) + 0.001f, vs * kUnit * 256.0f, good ? 0.0f : 1.0f);
+    return make_float4(good ? ks : 1.0f, fmaxf(__log2f(vs), vs == 0.0f ? -60.0f : -100.0f) + 0.001f, vs * kUnit, good ? 0.0f : 1.0f);
 }
 
 // sum of floor((a i + b) / m) for i < n, by Euclid's steps on (a, m); the divisions in 32 bits where the numbers allow (a
@@ -237,6 +259,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
     uint32_t* arrived = tmem_slot + 1;
     volatile uint32_t* failed = arrived + 1;
     volatile uint32_t* go_on = arrived + 2;              // [2] whether a warpgroup's D goes on adding up
+    float* low_scale = reinterpret_cast<float*>(misc + 256);      // [kStages] the smallest log2 of a value scale up to the tile
     Segment* segments = reinterpret_cast<Segment*>(misc + 512);   // [kSegments]
     float4* block_scales = reinterpret_cast<float4*>(misc + 1024);  // [kStages][8] what block_scale() gives
     float* row_scale = reinterpret_cast<float*>(misc + 1024 + T::kStages * 128);  // [RP] scale of a row's Q, times log2 e
@@ -245,7 +268,11 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
     float* exchange = lsum + 4 * RP;                            // [2][RP][4] warps' maxima
     float* refs = exchange + 8 * RP;                            // [4][RP] the rows' references (negative), a copy per warp
     float* corrs = refs + 4 * RP;                               // [4][RP] what older sums are multiplied by
-    float* factors = corrs + 4 * RP;                            // [4][RP] a warp's raw maxima, then the row's scale times the warp's key scale
+    float* l_corrs = corrs + 4 * RP;                            // [4][RP] ... the older weights' sum
+    float* lifts = l_corrs + 4 * RP;                            // [4][RP] 2^(reference of P - reference of O)
+    float* held_lifts = lifts + 4 * RP;                         // [4][RP] ... of what is in D
+    float* sum_refs = held_lifts + 4 * RP;                      // [4][RP] the references of O
+    float* factors = sum_refs + 4 * RP;                        // [4][RP] a warp's raw maxima, then the row's scale times the warp's key scale
 
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = heads / c.kv_heads;
     if (tid == 0) {
@@ -338,6 +365,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                 mbar_arrive(seg_full + seg % kSegments);
             }
             if (!more) break;
+            float low = 0.0f;
             for (uint32_t t = g.t0; t < g.t1; ++t) {
                 const int32_t e_next = entry(t + 1);
                 e = e >= 0 && (uint32_t)e < c.blocks ? e : -1;
@@ -354,7 +382,10 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                     bulk_load(dst, c.k + at * bytes, bytes, full + st);
                     bulk_load(dst + T::kTileBytes, c.v + at * bytes, bytes, full + st);
                 }
-                if (lane < per_tile) block_scales[st * 8 + lane] = e >= 0 ? block_scale(ks, vs) : make_float4(1.0f, -100.0f, 0.0f, 2.0f);
+                const float4 sc = e >= 0 ? block_scale(ks, vs) : make_float4(1.0f, 0.0f, 0.0f, 2.0f);
+                if (lane < per_tile) block_scales[st * 8 + lane] = sc;
+                low = fminf(low, -warp_max(-sc.y));
+                if (lane == 0) low_scale[st] = low;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full + st);
                 e = e_next;
@@ -372,7 +403,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
     } else if (warp == 4 * WG) {
         if (lane == 0) {
             constexpr uint32_t s_desc = umma_idesc(2, 1, 1, kKeys, T::kN);  // s32 sums, s8 codes x s8 digits of q
-            constexpr uint32_t d_desc = umma_idesc(2, 1, 0, T::kM, T::kNw);  // s32 sums, s8 codes x u8 digits of P
+            constexpr uint32_t d_desc = umma_idesc(2, 1, 0, T::kM, T::kDw);  // s32 sums, s8 codes x u8 digits of P
             const uint32_t q_addr = smem_u32(smem + T::kQAt), p_addr = smem_u32(smem + T::kPAt);
             uint32_t st = 0, round = 0, tile = 0;
             auto score = [&](uint32_t stage, uint32_t parity) {  // S of the tile in `stage`
@@ -411,8 +442,8 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                             // keys 32 i ..: two core matrices of one block, or (blocks of 16) of two
                             const uint32_t k0 = 32 * i, at = (k0 >> c.shift) * c.block * DIM + (k0 & (c.block - 1)) * 8;
                             const uint32_t step = c.shift == 4 ? 16 * DIM : 128;
-                            umma_i8_ss(tmem + T::kCols + w * T::kNw, umma_desc_plain(v_addr + at, step, 8 * c.block),
-                                       umma_desc_plain(p_addr + w * T::kNw * kKeys + 256 * i, 128, 8 * kKeys), d_desc, i != 0 || more);
+                            umma_i8_ss(tmem + T::kCols + w * T::kDw, umma_desc_plain(v_addr + at, step, 8 * c.block),
+                                       umma_desc_plain(p_addr + w * T::kDw * T::kPStep + 2 * T::kPStep * i, T::kPStep, 8 * T::kPStep), d_desc, i != 0 || more);
                         }
                         umma_commit(d_full + w);
                     }
@@ -425,27 +456,39 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
         const uint32_t quarter = warp & 3, wg = warp >> 2, key = tid & 127, wrow = wg * R;  // this thread's key, its first row
         const uint32_t comp = T::kM == 128 ? key : 16 * quarter + lane;                    // the component of D on its lane
         const bool owner = T::kM == 128 || (lane < 16 && comp < (uint32_t)DIM);
-        // a 4 x 4 transposition of bytes between lanes: which bytes a lane keeps in its two steps
-        const uint32_t sel1 = lane & 1 ? 0x3715u : 0x6240u, sel2 = lane & 2 ? 0x3276u : 0x5410u;
-        uint8_t* const p_at = smem + T::kPAt + wg * T::kNw * kKeys + (2 * quarter + (lane >> 4)) * 128 + (lane & 3) * 16 + ((lane >> 2) & 3) * 4;
+        // Four neighbouring lanes give each other their keys' words, a row to a lane: whose words come first, and how a row's four words
+        // (of this lane's key, its neighbour's, and the two of the other pair) become its four digits, one key to a byte
+        const bool odd = lane & 1, upper = lane & 2;
+        const uint32_t sel1 = odd ? 0x1504u : 0x5140u, sel2 = upper ? 0x1054u : 0x5410u;
+        uint8_t* const p_at = smem + T::kPAt + wg * T::kDw * T::kPStep + (2 * quarter + (lane >> 4)) * T::kPStep + (lane & 3) * 16 + ((lane >> 2) & 3) * 4;
         float* const my_refs = refs + quarter * RP + wrow;
         float* const my_corrs = corrs + quarter * RP + wrow;
         float* const my_factors = factors + quarter * RP + wrow;
+        float* const my_sum_refs = sum_refs + quarter * RP + wrow;
+        float* const my_l_corrs = l_corrs + quarter * RP + wrow;
+        float* const my_lifts = lifts + quarter * RP + wrow;
+        float* const my_held = held_lifts + quarter * RP + wrow;
         uint32_t tile = 0, st = 0, round = 0;
         float O[R], l[R];
         auto products = [&](uint32_t of_tile) {  // D of the tile is complete, P may be written
             ok = ok && mbar_wait(d_full + wg, of_tile & 1, failed, status, kStatusMmaWaitTimedOut);
         };
-        auto drain = [&]() {  // adds D to the float32 sums
+        auto drain = [&](const float* held, auto at_once) {  // adds D, times its rows' lifts, to the float32 sums, some rows at a time
             tc_fence_after_sync();
+            constexpr int kAtOnce = decltype(at_once)::value;
 #pragma unroll
-            for (int r0 = 0; r0 < R; r0 += 8) {
-                uint32_t d0[8], d1[8], d2[8];
-                const uint32_t at = tmem_addr(tmem, 32 * quarter, T::kCols + wg * T::kNw + r0);
-                tmem_ld8(at, d0), tmem_ld8(at + R, d1), tmem_ld8(at + 2 * R, d2);
+            for (int r0 = 0; r0 < R; r0 += kAtOnce) {
+                uint32_t d[4][kAtOnce];
+                const uint32_t at = tmem_addr(tmem, 32 * quarter, T::kCols + wg * T::kDw + r0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_ld(at + i * R, d[i]);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) O[r0 + i] = __fmaf_rn((float)(int)d2[i], 65536.0f, __fmaf_rn((float)(int)d1[i], 256.0f, O[r0 + i] + (float)(int)d0[i]));
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const float low = __fmaf_rn((float)(int)d[1][i], 256.0f, (float)(int)d[0][i]);
+                    const float sum = __fmaf_rn((float)(int)d[3][i], 16777216.0f, __fmaf_rn((float)(int)d[2][i], 65536.0f, low));
+                    O[r0 + i] = __fmaf_rn(sum, held[r0 + i], O[r0 + i]);
+                }
             }
             tc_fence_before_sync();
         };
@@ -506,14 +549,13 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
             }
 #pragma unroll
             for (int r = 0; r < R; ++r) O[r] = l[r] = 0.0f;
-            float M = kNone;  // the reference of row `lane`
             uint32_t since = 0;  // tiles in D
-            if (lane < (uint32_t)R) my_refs[lane] = 0.0f;  // (of a row that sees no key)
+            if (lane < (uint32_t)R) my_sum_refs[lane] = kNone, my_refs[lane] = 0.0f, my_lifts[lane] = 0.0f;  // (a row that sees no key keeps these)
             __syncwarp();
-            const float my_scale = lane < (uint32_t)R ? row_scale[wrow + lane] : 0.0f;  // of row `lane`
             for (uint32_t t = t0; t < t1; ++t, ++tile) {
                 ok = ok && mbar_wait(full + st, round & 1, failed, status, kStatusFullWaitTimedOut);
                 const float4 sc = block_scales[st * 8 + (key >> c.shift)];
+                const float* const low = low_scale + st;
                 if (++st == T::kStages) st = 0, ++round;
                 ok = ok && mbar_wait(s_full, tile & 1, failed, status, kStatusMmaWaitTimedOut);
                 tc_fence_after_sync();
@@ -553,38 +595,43 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                 }
                 __syncwarp();
                 if (lane < (uint32_t)R) {
-                    const float raw = my_factors[lane], f = factor_of(my_scale, sc.x);
+                    const float raw = my_factors[lane], f = factor_of(row_scale[wrow + lane], sc.x);
                     ex[lane * 4 + quarter] = ONE ? __fmaf_rn(raw, f, sc.y) : raw;
                     if (ONE) my_factors[lane] = f;
                 }
                 named_barrier_sync(1 + wg, 128);
-                bool moved = false;
+                // References are whole numbers: what older sums are multiplied by, and D on its way into O, are exact powers of two.
+                // P's lies up to 2^60 below O's, and by less where a weight is many times its contribution: l stays below 2^127.
+                bool moved = false, raised = false;
                 if (lane < (uint32_t)R) {
                     const float4 m = *reinterpret_cast<const float4*>(ex + lane * 4);
-                    const float top = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));
-                    moved = top > M + 1.0f;  // (-inf passes nothing, anything passes -inf)
-                    if (moved) {
-                        my_refs[lane] = -top, my_corrs[lane] = exp2_fast(M - top);
-                        M = top;
-                    } else {
-                        my_corrs[lane] = 1.0f;
-                    }
+                    const float top = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w)), M = my_sum_refs[lane], mu = -my_refs[lane];
+                    raised = top > M + 1.0f;  // (-inf passes nothing, anything passes -inf)
+                    // room above for the tiles to come, except for a tile in which some keys tower over the others
+                    const float room = ceilf(top) + (top - fminf(fminf(m.x, m.y), fminf(m.z, m.w)) < kEven ? kRoom : 0.0f);
+                    const float next = raised ? room : fmaxf(room, M - fmaxf(fminf(94.0f + *low, 60.0f), 0.0f));
+                    moved = raised || top > mu + 1.0f || (next < mu - kDrop && top > kNone);
+                    my_held[lane] = my_lifts[lane];
+                    my_corrs[lane] = raised ? power_of_two(M - next) : 1.0f;
+                    my_l_corrs[lane] = !moved ? 1.0f : M == kNone ? 0.0f : power_of_two(mu - next);
+                    if (raised) my_sum_refs[lane] = next;
+                    if (moved) my_refs[lane] = -next, my_lifts[lane] = raised ? 1.0f : power_of_two(next - M);
                 }
                 __syncwarp();
                 // the same in all four warps of the warpgroup
                 const uint32_t rows_moved = __ballot_sync(0xffffffffu, moved);
                 const bool more = t > t0 && !rows_moved && since < 255;
                 if (t > t0) products(tile - 1);
-                if (t > t0 && !more) drain();
+                if (t > t0 && !more) drain(my_held, Rows<R == 16 ? 4 : 8>());  // (fewer registers beside the scores)
                 since = more ? since + 1 : 0;
                 if (key == 0) go_on[wg] = more;
                 if (rows_moved) {
 #pragma unroll
                     for (int r = 0; r < R; r += 4)
                         if (rows_moved >> r & 15u) {
-                            const float4 cr = *reinterpret_cast<const float4*>(my_corrs + r);
+                            const float4 cr = *reinterpret_cast<const float4*>(my_corrs + r), lr = *reinterpret_cast<const float4*>(my_l_corrs + r);
                             O[r] *= cr.x, O[r + 1] *= cr.y, O[r + 2] *= cr.z, O[r + 3] *= cr.w;
-                            l[r] *= cr.x, l[r + 1] *= cr.y, l[r + 2] *= cr.z, l[r + 3] *= cr.w;
+                            l[r] *= lr.x, l[r + 1] *= lr.y, l[r + 2] *= lr.z, l[r + 3] *= lr.w;
                         }
                 }
 #pragma unroll
@@ -597,25 +644,27 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
                         const float f = i == 0 ? fc.x : i == 1 ? fc.y : i == 2 ? fc.z : fc.w, ref = i == 0 ? rf.x : i == 1 ? rf.y : i == 2 ? rf.z : rf.w;
                         const float p = exp2_fast(__fmaf_rn(a[r + i], ONE ? f : factor_of(f, sc.x), ref));
                         l[r + i] += p;
-                        x[i] = __float2uint_rn(__fmaf_rn(p, sc.z, 128.0f));  // 256 P, P rounded
+                        x[i] = __float2uint_rn(p * sc.z);  // P
                     }
-                    // digit d of the four rows, one row to a byte
-                    const uint32_t y0 = __byte_perm(x[0], x[1], 0x6251), y1 = __byte_perm(x[2], x[3], 0x6251);
-                    uint32_t w[3] = {__byte_perm(y0, y1, 0x5410), __byte_perm(y0, y1, 0x7632),
-                                     __byte_perm(__byte_perm(x[0], x[1], 0x0073), __byte_perm(x[2], x[3], 0x0073), 0x5410)};
+                    const uint32_t k0 = odd ? x[1] : x[0], k1 = odd ? x[3] : x[2];
+                    const uint32_t g0 = __shfl_xor_sync(0xffffffffu, odd ? x[0] : x[1], 1), g1 = __shfl_xor_sync(0xffffffffu, odd ? x[2] : x[3], 1);
+                    const uint32_t own = upper ? k1 : k0, next = upper ? g1 : g0;  // row r + lane % 4 of this lane's key and its neighbour's
+                    const uint32_t far = __shfl_xor_sync(0xffffffffu, upper ? k0 : k1, 2), last = __shfl_xor_sync(0xffffffffu, upper ? g0 : g1, 2);
+                    const uint32_t a01 = __byte_perm(own, next, sel1), a23 = __byte_perm(own, next, sel1 + 0x2222u);
+                    const uint32_t b01 = __byte_perm(far, last, sel1), b23 = __byte_perm(far, last, sel1 + 0x2222u);
+                    const uint32_t w[4] = {__byte_perm(a01, b01, sel2), __byte_perm(a01, b01, sel2 + 0x2222u), __byte_perm(a23, b23, sel2),
+                                           __byte_perm(a23, b23, sel2 + 0x2222u)};
 #pragma unroll
-                    for (uint32_t d = 0; d < 3; ++d) {  // ... becomes row r + lane % 4 of four lanes' keys, one key to a byte
-                        w[d] = __byte_perm(w[d], __shfl_xor_sync(0xffffffffu, w[d], 1), sel1);
-                        w[d] = __byte_perm(w[d], __shfl_xor_sync(0xffffffffu, w[d], 2), sel2);
+                    for (uint32_t d = 0; d < 4; ++d) {
                         const uint32_t n = d * R + r;
-                        *reinterpret_cast<uint32_t*>(p_at + (n >> 3) * 8 * kKeys + (n & 7) * 16) = w[d];
+                        *reinterpret_cast<uint32_t*>(p_at + (n >> 3) * 8 * T::kPStep + (n & 7) * 16) = w[d];
                     }
                 }
                 fence_proxy_async_smem();
                 tc_fence_before_sync();
                 mbar_arrive(p_full + wg);
             }
-            if (t0 < t1) products(tile - 1), drain();
+            if (t0 < t1) products(tile - 1), drain(my_lifts, Rows<8>());
             // the rows' sums over the keys, in a fixed order: a lane gives away half of its rows with each step, until it has row
             // lane / kShare
             constexpr uint32_t kShare = 32 / R;
@@ -630,7 +679,8 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
             }
             if (lane % kShare == 0) lsum[quarter * RP + wrow + lane / kShare] = l[0];
             named_barrier_sync(8, T::kSoft);  // (the next segment's first barrier keeps lsum until all have read it)
-            auto sum_of = [&](uint32_t r) { return (lsum[r] + lsum[RP + r]) + (lsum[2 * RP + r] + lsum[3 * RP + r]); };
+            // of row r, in O's reference
+            auto sum_of = [&](uint32_t r) { return ((lsum[r] + lsum[RP + r]) + (lsum[2 * RP + r] + lsum[3 * RP + r])) * lifts[r]; };
             // a row that saw no key has neither sum and gives zeros. (P's unit is taken out of the other sum: where value scales are near
             // 2^-100, so that the weights' sum is beyond 2^100, the quotient would leave the normal numbers with it.)
             auto share_of = [](float sum) { return sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum); };
@@ -660,7 +710,7 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
             if (owner)
 #pragma unroll
                 for (int r = 0; r < R; ++r) part[(wrow + r) * DIM + comp] = O[r];
-            if (quarter == 0 && lane < (uint32_t)R) part[RP * DIM + wrow + lane] = M, part[RP * DIM + RP + wrow + lane] = sum_of(wrow + lane);
+            if (quarter == 0 && lane < (uint32_t)R) part[RP * DIM + wrow + lane] = my_sum_refs[lane], part[RP * DIM + RP + wrow + lane] = sum_of(wrow + lane);
             __threadfence();
             named_barrier_sync(8, T::kSoft);
             if (tid == 0) *arrived = atomicAdd(counters + c0, 1u);

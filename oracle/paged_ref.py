@@ -99,11 +99,15 @@ def attend(q, kcodes, vcodes, kscale, vscale, table, lens, steps, scale):
     """float64 attention of every row, and how far a float32 kernel may be from it: [rows][heads][dim] and [rows][heads]. q float32
     [rows][heads][dim]; codes [blocks][kv][bs][dim].
 
-    The allowance, per row and head, of the largest |value| it sees: a score is off by half a step of q's 23-bit fixed point
-    on every component (2^-22 of max|q| times the sum of |k|) and by six float32 roundings of its own size, its weight by as much
-    and by 2^-21 for the exponential; numerator and denominator both. The weights are whole numbers of 2^-23 of a reference
-    that never exceeds the row's largest contribution: a uniform rounding error of +-2^-24 a key, at six standard
-    deviations of the sum over n keys, over the row's denominator (at least 1)."""
+    The allowance, per row and head. A score is off by half a step of q's 23-bit fixed point on every component (2^-22 of
+    max|q| times the sum of |k|), by six float32 roundings of its own size and by one of the exponent it becomes, which holds
+    log2 of a value scale too; its weight by as much, by 2^-21 for the exponential and by a rounding for each tile of 128 keys that a sum
+    runs over. That bears on the weighted values and, through the denominator, on the row itself.
+    Beside it the weights are whole numbers of a step: a contribution c = w vscale is off by half of one at most, and by no more
+    than itself. The step is 2^-31 of a power of two that lies at most 2^11 above the largest c of the tile; where that c towers over
+    all other tiles' (by more than 2^8) the power has just been set: at most 2^5 above it, or 2 where it towers over
+    a quarter of its own tile too. It never lies more than 2^60 below the row's largest (less where value scales are so small that
+    the weights' sum needs the room): what the step is then is the bound for all tiles."""
     rows, heads, dim = q.shape
     blocks, kvh, bs, _ = kcodes.shape
     out, tol = np.zeros(q.shape), np.zeros((rows, heads))
@@ -124,8 +128,21 @@ def attend(q, kcodes, vcodes, kscale, vscale, table, lens, steps, scale):
                 s = (k @ qd) * scale
                 w = np.exp(s - s.max())
                 out[t, h] = (w @ v) / w.sum()
-                ds = scale * 2.0 ** -22 * np.abs(qd).max() * np.abs(k).sum(1).max() + 6 * 2.0 ** -24 * np.abs(s).max() * 1.45
-                tol[t, h] = np.abs(v).max() * (2 * (ds + 2.0 ** -21) + 6 * np.sqrt(len(s) / 3) * 2.0 ** -24 / w.sum())
+                logs = np.abs(np.log2(np.maximum(vscale[e, g].astype(np.float64), 2.0 ** -100))).max()
+                ds = scale * 2.0 ** -22 * np.abs(qd).max() * np.abs(k).sum(1).max() + 2.0 ** -24 * (6 * 1.45 * np.abs(s).max() + logs)
+                c, tile = w * vscale[e, g], pos[ok] // 128
+                top, quarters = np.zeros(n // 128 + 1), np.zeros((n // 128 + 1, 4))
+                np.maximum.at(top, tile, c)
+                np.maximum.at(quarters, (tile, pos[ok] % 128 // 32), c)
+                most = np.argmax(top)
+                step = 2.0 ** 11 * top
+                if top[most] > 2.0 ** 8 * np.delete(top, most).max(initial=0.0):
+                    step[most] = top[most] * (2.0 if quarters[most].min() < 2.0 ** -8.1 * top[most] else 2.0 ** 5)
+                step = np.maximum(step, top[most] * 2.0 ** (5 - min(max(94 - logs, 0), 60)))
+                codes = np.abs(vcodes[e, g, o].astype(np.float64)).max(1)
+                lost = (np.minimum(c, 2.0 ** -32 * step[tile]) * codes).sum()
+                off = ds + 2.0 ** -21 + (n // 128 + 1) * 2.0 ** -24
+                tol[t, h] = ((w * np.abs(v).max(1)).sum() / w.sum() + np.abs(out[t, h]).max()) * off + lost / w.sum()
     return out, tol
 
 

@@ -56,6 +56,57 @@ def put(t):
         on.copy_(a.reshape(on.shape))
 
 
+def with_sink(keys, gap, at, value, dim=64, bs=64):
+    """One request of `keys` cached tokens, one of which scores `gap` nats above the others' mean (0.3 nats apart), with
+    values of one sign so that nothing cancels, the lone key's of size `value` of theirs."""
+    rng = np.random.default_rng(keys + int(gap))
+    t = filled(rng, 2, 1, dim, bs, [keys - 1], [1], spread=0.0)
+    t.codes["k"] = rng.integers(-30, 31, t.codes["k"].shape).astype(np.int8)
+    t.codes["v"] = rng.integers(40, 127, t.codes["v"].shape).astype(np.int8)
+    block, off = t.table[0, at // bs], at % bs
+    t.codes["k"][block, :, off] = 127
+    t.codes["v"][block, :, off] = (t.codes["v"][block, :, off] * value).astype(np.int8)
+    put(t)
+    st = t.Step(t.cache, 1)
+    t.cache.plan(dev(np.ones(1, np.int32)), st)
+    want, _ = t.ref.plan(t.lens, [1], t.table, t.free, t.count, bs, t.blocks, 1)
+    q = np.ones((1, 2, dim), np.float32)
+    scale = gap / (dim * 127 * float(t.scales["k"][block, 0]))
+    return t, st, want, q, scale
+
+
+@pytest.mark.parametrize("value", [0.0, 1.0], ids=["null", "full"])
+@pytest.mark.parametrize("gap", [10.0, 14.0, 17.0, 40.0])
+@pytest.mark.parametrize("keys,at", [(200, 5), (4096, 0), (4096, 3000), (15000, 0), (15000, 14990)])
+def test_one_key_far_above_the_others(keys, at, gap, value):
+    """The allowance is the checker's: what a weight's whole steps lose is bounded tile by tile, so the row's other keys
+    keep their digits outside the lone key's own tile, and inside it down to 2^-31 of it."""
+    t, st, want, q, scale = with_sink(keys, gap, at, value)
+    exact, tol = t.ref.attend(q, t.codes["k"], t.codes["v"], t.scales["k"], t.scales["v"], t.table, t.lens, want, scale)
+    got = t.cache.attend(0, dev(q.reshape(1, -1)), 2, st, scale=scale, max_count=1).numpy().reshape(1, 2, -1)
+    off = np.abs(got - exact).max(-1)
+    size = np.abs(exact).max(-1)
+    print(f"[sink] {keys} keys, {gap} nats, value {value}: {float((off / size).max()):.2e} of the row, {float((off / tol).max()):.2f} of the allowance "
+          f"({float((tol / size).max()):.1e})")
+    assert (off <= tol).all()
+
+
+@pytest.mark.parametrize("every", [1, 3])
+def test_references_that_move_up_and_down(every):
+    """Tiles whose largest scores lie some 15 nats apart in turn, rows of a prompt with different scores: the reference follows the
+    tiles down and up again, nothing is lost on the way."""
+    rng = np.random.default_rng(52)
+    for heads, counts in ((2, [1, 1]), (14, [70, 5])):
+        t = filled(rng, heads, 1, 64, 32, [3000, 900], counts, spread=0.2)
+        t.codes["v"] = rng.integers(1, 127, t.codes["v"].shape).astype(np.int8)
+        for b in range(2):
+            for j, block in enumerate(t.table[b]):
+                if block >= 0 and (j // 4) % (2 * every) >= every:
+                    t.codes["k"][block] = t.codes["k"][block] // 8
+        put(t)
+        attend(t, counts, scale=0.55, max_count=max(counts))
+
+
 @pytest.mark.parametrize("counts", [[1], [33]], ids=["token", "prompt"])
 def test_value_scales_at_the_lower_end(counts):
     """Thousands of keys of about equal weight, value scales of 2^-100: the sums' quotients stay normal numbers."""
