@@ -116,3 +116,55 @@ def test_value_scales_at_the_lower_end(counts):
     t.scales["v"][:] = np.float32(2.0 ** -100)
     put(t)
     attend(t, counts, scale=1e-3)
+
+
+# ── many requests, long ranges ─────────────────────────────────────────────
+
+
+@pytest.mark.parametrize("kind", ["tokens", "prompts", "holes"])
+@pytest.mark.parametrize("seqs", [33, 65, 1025, 4096])
+def test_batches_of_many_requests(seqs, kind):
+    """More requests than the lanes that look for a range's start: stretches of several requests a lane, whole stretches
+    without a token, more requests in a stretch than lanes."""
+    rng = np.random.default_rng(seqs)
+    lens = rng.integers(0, 40, seqs)
+    if kind == "tokens":
+        counts = np.ones(seqs, np.int64)
+    elif kind == "prompts":
+        counts = rng.integers(0, 6, seqs)
+    else:
+        counts = (rng.random(seqs) < 0.05).astype(np.int64) * rng.integers(1, 4, seqs)
+        counts[: seqs // 3] = 0
+        counts[seqs - 1] = 2
+        lens[seqs // 2] = 900
+        counts[seqs // 2] = 1
+    t = filled(rng, 2, 1, 32, 16, [int(n) for n in lens], [int(c) for c in counts])
+    attend(t, [int(c) for c in counts], pad=1, max_count=int(counts.max()))
+
+
+@pytest.mark.parametrize("dim,block", [(32, 128), (64, 128)])
+def test_a_range_of_more_tiles_than_the_integer_sums_may_hold(dim, block):
+    """Tables that name a few blocks over and over: every CTA has some 700 tiles of one request, all of equal scores, codes of
+    127. Value scales of 0.99 and of just under 32 times that: a reference that a tile of small ones laid is not moved by the large ones,
+    whose weights then fill their 32 bits, and the sums are read out only because they would leave 32 bits. The mean of the
+    values is known exactly."""
+    from grilly2_b200.infer.paged import PagedKvCache, PagedStep
+    rng = np.random.default_rng(54)
+    seqs, entries, blocks = 4, 100000, 16
+    table = rng.integers(0, blocks, (seqs, entries)).astype(np.int32)
+    last = entries * block - 1  # the last position of the table
+    codes = np.full((blocks, 1, block, dim), 127, np.int8)
+    vscale = np.where(np.arange(blocks) % 8, 31.4, 0.99).astype(np.float32)[:, None]
+    cache = PagedKvCache(layers=1, kv_heads=1, head_dim=dim, blocks=blocks, seqs=seqs, max_blocks=entries, block_size=block,
+                         buffers={"k": words(codes), "v": words(codes), "kscale": dev(np.ones((blocks, 1), np.float32)), "vscale": dev(vscale),
+                                  "table": dev(table), "lens": dev(np.full(seqs, last, np.int32)), "free_count": dev(np.zeros(1, np.int32))})
+    st = PagedStep(cache, seqs)
+    cache.plan(dev(np.ones(seqs, np.int32)), st)
+    got = cache.attend(0, _C_filled((seqs, dim), 0.0), 1, st, max_count=1).numpy()
+    want = 127 * vscale[table, 0].astype(np.float64).mean(1)
+    tiles = seqs * entries * block // 128
+    # the sums of a CTA's range, one rounding a tile each for numerator and denominator at most, and their joining
+    allowed = (2 * (tiles / 148 + 1) + 16) * 2.0 ** -24
+    off = np.abs(got - want[:, None]).max(1) / want
+    print(f"[long range] {tiles} tiles: {off.max():.2e} ({allowed:.1e})")
+    assert (off <= allowed).all()
