@@ -1,14 +1,14 @@
 // The next token of every row with settings of its own: temperature, top-k, top-p, min-p, and the draw by the inverse CDF in
 // token order (include/gq.h, gq_sample_rows). Beside gq_sample (sample.cu), which has one setting for all rows.
 //
-// w_i = exp((x_i - M) / T), M the row's maximum, in float64; where masses are added by atomics they are whole numbers w 2^40, so
-// that no result depends on their order. A row is a cluster of up to eight CTAs that keep its logits in shared memory: they
+// w_i = exp((x_i - M) / T), M the row's maximum, in float64, and so the draw's sums; what top-p compares is added by atomics, as whole
+// numbers w 2^40, so that no result depends on their order. A row is a cluster of up to eight CTAs that keep its logits in shared memory: they
 // are read from memory once, and a row's work is spread where there are few rows. "Bins" are 2048 steps linear in x over
 // the top 64 T nats, or over the row's range where that is less; what lies below weighs under e^-64 and is dropped.
 //   1 every thread's maximum, the row's maximum
 //   2 top-k, as long as there are k threads: the threads' maxima alone go into a histogram; at least k tokens lie in or above the
 //     bin where it reaches k. Those are listed in the first CTA's shared memory, and it finishes the row alone: it
-//     counts for every listed token how many and how much lie above, and for the kept ones how much lies before.
+//     counts for every listed token how many and how much lie above, and lays the kept ones' weights out in token order.
 //   3 otherwise, for top-k and then top-p: a histogram of all tokens (counts or masses), its crossing bin, and that bin's
 //     tokens as a list that is ranked the same way, or bisected where it is long
 //   4 every thread's kept mass, a thread owning consecutive tokens; the thread that holds the target walks its own
@@ -53,7 +53,7 @@ __device__ __forceinline__ double widen(float v) {
 
 struct Control {
     uint32_t top[2];             // this CTA's largest key, smallest above -inf
-    uint32_t border, listed, low, range_lo, range_hi, owner_warp, pick, last;
+    uint32_t border, listed, low, range_lo, range_hi, owner_warp, pick;
     unsigned long long above, target, part[2];
     double before, goal, total;
     double warp_sum[kWarps];
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* _
             if (listed <= kList) {
                 if (rank == 0) {
                     // what lies above a token, of all (counted) and of those top-k keeps
-                    if (tid == 0) sh.ctl.low = mk, sh.ctl.pick = 0xffffffffu, sh.ctl.last = 0;
+                    if (tid == 0) sh.ctl.low = mk, sh.ctl.pick = 0xffffffffu;
                     __syncthreads();
                     unsigned long long kept_mass = 0;  // of this thread's tokens
                     each_listed(
@@ -408,36 +408,60 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const float* _
                     const unsigned long long of_k = block_sum(kept_mass);
                     const uint32_t kth = sh.ctl.low;
                     const unsigned long long target = by_p ? (unsigned long long)fmax(ceil((double)p * (double)of_k), 1.0) : ~0ull;
-                    kept_mass = 0;
-                    // out of the list goes what top-k, top-p or min-p drop: its mass becomes 0 (no other's mass above it counts it)
+                    unsigned long long kept = 0;
+                    // out of the list goes what top-k, top-p or min-p drop: its index becomes one beyond all
                     each_listed(
                         listed,
                         [&](uint32_t i, uint32_t j) { return sh.list.key[j] > sh.list.key[i] ? sh.list.mass[j] : 0ull; },
                         [&](uint32_t i, unsigned long long mass) {
                             const uint32_t key = sh.list.key[i];
                             const bool keep = key == mk || (key >= kth && mass < target && weight(value_of(key)) >= least);
-                            if (keep) kept_mass += sh.list.mass[i];
+                            if (keep) ++kept;
                             else sh.list.at[i] |= 0x80000000u;
                         });
-                    const unsigned long long total = block_sum(kept_mass);
-                    const double goal = (double)u * (double)total;
+                    kept = block_sum(kept);
+                    // the draw, in float64 as below: the kept weights in token order (in the masses' place; a token's place in its key's)
+                    double* const w = reinterpret_cast<double*>(sh.list.mass);
                     each_listed(
-                        listed,
-                        [&](uint32_t i, uint32_t j) {  // (a dropped token's index is beyond all)
-                            return sh.list.at[j] <= sh.list.at[i] ? sh.list.mass[j] : 0ull;
-                        },
-                        [&](uint32_t i, unsigned long long mass) {
-                            const uint32_t at = sh.list.at[i];
-                            if (at >> 31 || sh.list.mass[i] == 0) return;
-                            if ((double)mass > goal) atomicMin(&sh.ctl.pick, at);
-                            atomicMax(&sh.ctl.last, at);
+                        listed, [&](uint32_t i, uint32_t j) { return sh.list.at[j] < sh.list.at[i] ? 1ull : 0ull; },
+                        [&](uint32_t i, unsigned long long place) {
+                            const uint32_t key = sh.list.key[i];
+                            const bool in = sh.list.at[i] >> 31 == 0;
+                            if (in) w[place] = weight(value_of(key));
+                            sh.list.key[i] = in ? (uint32_t)place : 0xffffffffu;
                         });
                     __syncthreads();
-                    const uint32_t chosen = sh.ctl.pick != 0xffffffffu ? sh.ctl.pick : sh.ctl.last;
+                    const uint32_t each = ((uint32_t)kept + kThreads - 1) / kThreads, t0 = min(tid * each, (uint32_t)kept), t1 = min(t0 + each, (uint32_t)kept);
+                    double sum = 0.0;
+                    for (uint32_t t = t0; t < t1; ++t) sum += w[t];
+                    double upto = sum;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const double y = __shfl_up_sync(0xffffffffu, upto, o);
+                        if (lane >= (uint32_t)o) upto += y;
+                    }
+                    if (lane == 31) sh.ctl.warp_sum[warp] = upto;
+                    __syncthreads();
+                    double total = 0.0, run = 0.0;
+                    for (uint32_t i = 0; i < kWarps; ++i) {
+                        if (i == warp) run = total;
+                        total += sh.ctl.warp_sum[i];
+                    }
+                    run += upto - sum;
+                    const double goal = (double)u * total;
+                    for (uint32_t t = t0; t < t1; ++t) {
+                        run += w[t];
+                        if (run > goal) {
+                            atomicMin(&sh.ctl.pick, t);
+                            break;
+                        }
+                    }
+                    __syncthreads();
+                    const uint32_t chosen = min(sh.ctl.pick, (uint32_t)kept - 1);  // the target at the very end: the last kept token
                     for (uint32_t i = tid; i < listed; i += kThreads)
-                        if (sh.list.at[i] == chosen) {
-                            tokens[row] = (int32_t)chosen;
-                            if (probs) probs[row] = (float)(weight(value_of(sh.list.key[i])) * kFixed / (double)total);
+                        if (sh.list.key[i] == chosen) {
+                            tokens[row] = (int32_t)sh.list.at[i];
+                            if (probs) probs[row] = (float)(w[chosen] / total);
                         }
                 }
                 cluster.sync();  // nobody leaves while its shared memory may be read

@@ -464,8 +464,8 @@ int32_t gq_paged_attn(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer, 
  * the largest always stays. The draw is the inverse CDF in token order with u in [0, 1): the first kept token whose cumulative
  * weight exceeds u * total. u is uniforms[*draws % uniform_rows][row] (uniform_rows x rows floats), and the uint32 word
  * `draws` is advanced by one, so that a captured step takes the next numbers at each replay; draws == 0: the first row. temperature <= 0 takes the first largest. tokens: int32 per row, -1
- * where every logit is -inf; probs (0 = none) receives the token's share of what was kept; neither may overlap the inputs. Sums and weights in 64 bits; tokens below
- * exp(-64) of the largest weight are never drawn. vocab at most 2^23.
+ * where every logit is -inf; probs (0 = none) receives the token's share of what was kept; neither may overlap the inputs. Weights and the draw's sums are
+ * float64; the masses that top_p compares are sums of whole multiples of 2^-40 of the largest weight; tokens below exp(-64) of it are never drawn. vocab at most 2^23.
  * Replaces nothing of the reference: its sampler has one setting for all rows and no min_p (gq_sample). */
 int32_t gq_sample_rows(gq_ctx* ctx, gq_buf logits, uint64_t l_off, uint64_t rows, uint64_t vocab, gq_buf temperature, gq_buf top_k, gq_buf top_p,
                        gq_buf min_p, gq_buf uniforms, uint64_t uniform_rows, gq_buf draws, gq_buf tokens, gq_buf probs);
