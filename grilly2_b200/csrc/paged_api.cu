@@ -58,6 +58,24 @@ void check_aligned(const char* op, std::initializer_list<const void*> ptrs) {
         if ((uintptr_t)p & 15) fail("%s: buffers must lie on 16-byte boundaries", op);
 }
 
+// A kernel's CTAs write some buffers while others read theirs: what is written must lie apart from all else the call names.
+struct Range {
+    const char* what;
+    const void* p;
+    uint64_t bytes;
+};
+void check_apart(const char* op, std::initializer_list<Range> written, std::initializer_list<Range> read) {
+    for (const Range* w = written.begin(); w != written.end(); ++w) {
+        for (const Range* o = w + 1; o != written.end(); ++o)
+            if (ranges_overlap(w->p, w->bytes, o->p, o->bytes)) fail("%s: %s must not overlap %s", op, w->what, o->what);
+        for (const Range& r : read)
+            if (ranges_overlap(w->p, w->bytes, r.p, r.bytes)) fail("%s: %s must not overlap %s", op, w->what, r.what);
+    }
+}
+uint64_t table_bytes(const PagedView& c) { return (uint64_t)c.seqs * c.max_blocks * 4; }
+uint64_t code_bytes(const PagedView& c) { return (uint64_t)c.blocks * c.kv_heads * c.dim << c.shift; }
+uint64_t scale_bytes(const PagedView& c) { return (uint64_t)c.blocks * c.kv_heads * 4; }
+
 uint64_t check_heads(const char* op, const PagedView& c, uint64_t heads) {
     if (heads == 0 || heads > 65536 || heads % c.kv_heads)
         fail("%s: %llu heads do not group over %u kv heads", op, (ull)heads, c.kv_heads);
@@ -76,6 +94,12 @@ int32_t gq_paged_plan(gq_ctx* ctx, const gq_paged_cache* cache, gq_buf counts, g
         auto np = (const int32_t*)view(ctx, counts, 0, c.seqs, 4, "gq_paged_plan counts");
         auto fp = (const int32_t*)view(ctx, free_list, 0, c.blocks, 4, "gq_paged_plan free list");
         auto fc = (int32_t*)view(ctx, free_count, 0, 1, 4, "gq_paged_plan free count");
+        const uint64_t per_seq = (uint64_t)c.seqs * 4, per_row = (uint64_t)st.tokens * 4;
+        check_apart("gq_paged_plan",
+                    {{"the step's starts", st.starts, per_seq + 4}, {"the step's slots", st.slots, per_row}, {"the step's positions", st.positions, per_row},
+                     {"the step's runs", st.runs, (uint64_t)st.runs_cap * 4 + 4}, {"the step's last rows", st.last, per_seq}, {"the step's info", st.info, 8},
+                     {"the block table", c.table, table_bytes(c)}, {"the free count", fc, 4}},
+                    {{"the counts", np, per_seq}, {"the cached lengths", c.lens, per_seq}, {"the free list", fp, (uint64_t)c.blocks * 4}});
         launch_paged_plan(ctx->stream, c, st, np, fp, fc);
         after_launch(ctx, "paged_plan", {cache->table, cache->lens, counts, free_list, free_count, step->starts, step->slots, step->positions, step->runs,
                                          step->last, step->info});
@@ -87,6 +111,7 @@ int32_t gq_paged_advance(gq_ctx* ctx, const gq_paged_cache* cache, const gq_page
         Locked l(ctx);
         const PagedView c = cache_view(ctx, "gq_paged_advance", cache, 0, false);
         const StepView st = step_view(ctx, "gq_paged_advance", cache, step);
+        check_apart("gq_paged_advance", {{"the cached lengths", c.lens, (uint64_t)c.seqs * 4}}, {{"the step's starts", st.starts, (uint64_t)c.seqs * 4 + 4}});
         launch_paged_advance(ctx->stream, c, st);
         after_launch(ctx, "paged_advance", {cache->table, cache->lens, step->starts});
     });
@@ -99,6 +124,10 @@ int32_t gq_paged_release(gq_ctx* ctx, const gq_paged_cache* cache, gq_buf which,
         auto wp = (const int32_t*)view(ctx, which, 0, c.seqs, 4, "gq_paged_release requests");
         auto fp = (int32_t*)view(ctx, free_list, 0, c.blocks, 4, "gq_paged_release free list");
         auto fc = (int32_t*)view(ctx, free_count, 0, 1, 4, "gq_paged_release free count");
+        check_apart("gq_paged_release",
+                    {{"the block table", c.table, table_bytes(c)}, {"the cached lengths", c.lens, (uint64_t)c.seqs * 4},
+                     {"the free list", fp, (uint64_t)c.blocks * 4}, {"the free count", fc, 4}},
+                    {{"the requests", wp, (uint64_t)c.seqs * 4}});
         launch_paged_release(ctx->stream, c, wp, fp, fc);
         after_launch(ctx, "paged_release", {cache->table, cache->lens, which, free_list, free_count});
     });
@@ -119,7 +148,12 @@ int32_t gq_paged_append(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer
         auto sp = (const float*)view(ctx, sin, 0, max_pos * c.dim, 4, "gq_paged_append sin");
         auto op_ = (float*)view(ctx, q_out, 0, st.tokens * width, 4, "gq_paged_append q output");
         check_aligned(op, {qp, cp, sp, op_});
-        if (ranges_overlap(op_, st.tokens * width * 4, qp, st.tokens * row * 4)) fail("%s: the output must not overlap qkv", op);
+        check_apart(op,
+                    {{"the output", op_, st.tokens * width * 4}, {"the key pool", c.k, code_bytes(c)}, {"the value pool", c.v, code_bytes(c)},
+                     {"the key scales", c.kscale, scale_bytes(c)}, {"the value scales", c.vscale, scale_bytes(c)}},
+                    {{"qkv", qp, st.tokens * row * 4}, {"cos", cp, max_pos * c.dim * 4}, {"sin", sp, max_pos * c.dim * 4},
+                     {"the step's starts", st.starts, (uint64_t)c.seqs * 4 + 4}, {"the step's slots", st.slots, (uint64_t)st.tokens * 4},
+                     {"the step's positions", st.positions, (uint64_t)st.tokens * 4}, {"the step's runs", st.runs, (uint64_t)st.runs_cap * 4 + 4}});
         launch_paged_append(ctx->stream, c, st, qp, (uint32_t)heads, cp, sp, (uint32_t)max_pos, op_);
         after_launch(ctx, "paged_append", {cache->k, cache->v, cache->kscale, cache->vscale, cache->table, cache->lens, qkv, cos, sin, step->starts,
                                            step->slots, step->positions, step->runs, q_out});
@@ -140,7 +174,10 @@ int32_t gq_paged_attn(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer, 
         auto qp = (const float*)view(ctx, q, 0, st.tokens * width, 4, "gq_paged_attn q");
         auto yp = (float*)view(ctx, out, 0, st.tokens * width, 4, "gq_paged_attn output");
         check_aligned(op, {qp, yp});
-        if (ranges_overlap(yp, st.tokens * width * 4, qp, st.tokens * width * 4)) fail("%s: the output must not overlap q", op);
+        check_apart(op, {{"the output", yp, st.tokens * width * 4}},
+                    {{"q", qp, st.tokens * width * 4}, {"the key pool", c.k, code_bytes(c)}, {"the value pool", c.v, code_bytes(c)},
+                     {"the key scales", c.kscale, scale_bytes(c)}, {"the value scales", c.vscale, scale_bytes(c)}, {"the block table", c.table, table_bytes(c)},
+                     {"the cached lengths", c.lens, (uint64_t)c.seqs * 4}, {"the step's starts", st.starts, (uint64_t)c.seqs * 4 + 4}});
         const int sms = ctx->prop.multiProcessorCount;
         void* scratch = context_scratch(ctx, paged_attn_scratch_bytes(c.dim, sms));
         launch_paged_attn(ctx->stream, sms, ctx->status_dev, c, st, qp, (uint32_t)heads, scale, max_count, yp, ctx->paged_state, scratch);

@@ -400,7 +400,8 @@ int32_t gq_argmax_rows(gq_ctx* ctx, gq_buf v, uint64_t rows, uint64_t n, gq_buf 
  *   kscale, vscale  float32 [layers][blocks][kv_heads]
  *   table   int32 [seqs][max_blocks];  lens  int32 [seqs]
  * block_size 16, 32, 64 or 128; dim 32, 64 or 128; seqs at most 4096; blocks * block_size and seqs * max_blocks below
- * 2^31; k and v on 16-byte boundaries. An entry of the table or the slot map outside the pool is treated as -1. */
+ * 2^31; k and v on 16-byte boundaries. An entry of the table or the slot map outside the pool is treated as -1. What a call
+ * writes must not overlap anything else that it names. */
 typedef struct gq_paged_cache {
     uint64_t layers, blocks, block_size, kv_heads, dim, seqs, max_blocks;
     gq_buf k, v, kscale, vscale, table, lens;

@@ -168,3 +168,50 @@ def test_a_range_of_more_tiles_than_the_integer_sums_may_hold(dim, block):
     off = np.abs(got - want[:, None]).max(1) / want
     print(f"[long range] {tiles} tiles: {off.max():.2e} ({allowed:.1e})")
     assert (off <= allowed).all()
+
+
+# ── refusals ───────────────────────────────────────────────────────────────
+
+
+def test_buffers_that_a_call_writes_lie_apart():
+    from grilly2_b200 import _C
+    from grilly2_b200.infer.paged import PagedKvCache, PagedStep
+    ints = lambda n: dev(np.zeros(n, np.int32))  # noqa: E731
+    geometry = dict(layers=1, kv_heads=2, head_dim=32, blocks=4, seqs=2, max_blocks=2, block_size=16)
+    cache, counts = PagedKvCache(**geometry), ints(2)
+    step = PagedStep(cache, 4)
+    over = lambda t, *shape: _C.Tensor(t.storage, shape, t.dtype)  # noqa: E731
+    shared = ints(16)
+    for names in (("slots", "positions"), ("starts", "last"), ("runs", "info")):
+        with pytest.raises(RuntimeError, match="must not overlap"):
+            cache.plan(counts, PagedStep(cache, 4, buffers={n: shared for n in names}))
+    with pytest.raises(RuntimeError, match="the step's last rows must not overlap the counts"):
+        cache.plan(step.last, step)
+    with pytest.raises(RuntimeError, match="the block table must not overlap the cached lengths"):
+        PagedKvCache(**geometry, buffers={"table": shared, "lens": shared}).plan(counts, step)
+    with pytest.raises(RuntimeError, match="the free count must not overlap the free list"):
+        PagedKvCache(**geometry, buffers={"free": shared, "free_count": shared}).plan(counts, step)
+    with pytest.raises(RuntimeError, match="the cached lengths must not overlap the step's starts"):
+        PagedKvCache(**geometry, buffers={"lens": step.starts}).advance(step)
+    with pytest.raises(RuntimeError, match="the cached lengths must not overlap the requests"):
+        cache.release(cache.lens)
+    with pytest.raises(RuntimeError, match="the block table must not overlap the free list"):
+        PagedKvCache(**geometry, buffers={"table": shared, "free": shared}).release(counts)
+    f = lambda *s: dev(np.zeros(s, np.float32))  # noqa: E731
+    qkv, cos, sin, room = f(4, 8 * 32), f(64, 32), f(64, 32), f(4096)
+    with pytest.raises(RuntimeError, match="the output must not overlap cos"):
+        cache.append(0, qkv, 4, cos, sin, step, q_out=over(cos, 4, 128))
+    with pytest.raises(RuntimeError, match="the output must not overlap the key pool"):
+        cache.append(0, qkv, 4, cos, sin, step, q_out=_C.Tensor(cache.k.storage, (4, 128), "float32"))
+    one = PagedKvCache(**geometry, buffers={"k": cache.k, "v": cache.k})
+    with pytest.raises(RuntimeError, match="the key pool must not overlap the value pool"):
+        one.append(0, qkv, 4, cos, sin, step)
+    with pytest.raises(RuntimeError, match="the key scales must not overlap the value scales"):
+        PagedKvCache(**geometry, buffers={"kscale": room, "vscale": room}).append(0, qkv, 4, cos, sin, step)
+    q = f(4, 128)
+    with pytest.raises(RuntimeError, match="the output must not overlap the value scales"):
+        PagedKvCache(**geometry, buffers={"vscale": room}).attend(0, q, 4, step, out=over(room, 4, 128))
+    with pytest.raises(RuntimeError, match="the output must not overlap the key pool"):
+        cache.attend(0, q, 4, step, out=_C.Tensor(cache.k.storage, (4, 128), "float32"))
+    one.attend(0, q, 4, step)  # what is only read may be named twice
+    cache.plan(counts, step)
