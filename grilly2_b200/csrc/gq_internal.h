@@ -122,7 +122,7 @@ void check_dims(const char* op, uint64_t a, uint64_t b, uint64_t c = 1);
 
 
 // ── launches that hide the launch latency behind the previous kernel ─────
-// A kernel whose FIRST statement is GQ_GRID_DEP_SYNC() may be launched with launch_after(): its CTAs are scheduled
+// A kernel that does nothing before GQ_GRID_DEP_SYNC() but set up its own shared memory may be launched with launch_after(): its CTAs are scheduled
 // as soon as the kernel before it in the stream lets them (programmatic stream serialization) and then wait, in
 // hardware, until that kernel has finished and its writes are visible. Stream-order semantics are unchanged (nothing
 // is read or written before the wait); what is saved is the launch gap. A kernel lets the one behind it start only AFTER its

@@ -58,4 +58,6 @@ def test_tensor_memory_is_allocated_behind_the_wait(path):
 def test_the_sources_are_read_as_meant():
     found = {n: b for f in FILES for n, b in _kernels(_code(f)).items()}
     assert {"paged_attn_kernel", "gemv_q4_umma_kernel", "gemv_q4_lanes_kernel", "gemm_i8_q8_kernel", "x_digits_kernel", "x_planes_kernel"} <= set(found)
-    assert found["paged_attn_kernel"].lstrip("{ \n").startswith("GQ_GRID_DEP_SYNC();")
+    body = found["paged_attn_kernel"]
+    assert 0 < body.index("GQ_GRID_DEP_SYNC();") < body.index("tmem_alloc(")
+    assert not re.search(r"\b(?:c|s)\.\w+\[|request_of|table", body[:body.index("GQ_GRID_DEP_SYNC();")])  # and reads no device memory
