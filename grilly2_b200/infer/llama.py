@@ -219,7 +219,8 @@ class LlamaDecoder:
         ``cache.plan(counts, step)`` has laid them out (prompts, single tokens, or both; rows behind the last request's are ignored).
         Returns the logits of every request's last row, [seqs, vocab], NaN where a request has no row, and advances the
         cache. Nothing reads a host integer, so a captured step replays. ``max_count``: the largest count expected (1 for a decode
-        step). No counterpart in the reference, which runs one request."""
+        step). A row without room (``step.shortfall()``, ``step.dropped()``) is computed without its own key and counted as cached:
+        a program that replays steps looks at these before it trusts the rows behind. No counterpart in the reference, which runs one request."""
         c, lib, ctx = self.cfg, _lib.load(), _C.context()
         T = step.max_tokens
         if tokens.dtype != "int32" or tokens.numel() != T or tokens.offset:

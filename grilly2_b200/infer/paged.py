@@ -163,3 +163,8 @@ class PagedStep:
         """Blocks that the last plan's rows lack: the free list was empty, then or when the entry's first tokens came (a host
         copy; waits for the device)."""
         return int(self.info.numpy()[1])
+
+    def dropped(self) -> int:
+        """Rows of the last plan whose token has no place in the pool and so is neither cached nor seen: the blocks that
+        ``shortfall`` counts were missing, or the request has outgrown its table, which it does not count (a host copy; waits for the device)."""
+        return int((self.slots.numpy()[:int(self.info.numpy()[0])] < 0).sum())

@@ -429,7 +429,8 @@ typedef struct gq_paged_step {
  * [blocks], of which the first *free_count are free; the last is taken first), in order of (b, entry). An entry that lens[b]
  * lies inside gets none: its earlier tokens were advanced over without room, and whatever a block holds would be read as
  * theirs; the request has blocks again from its next entry on. Rows beyond max_tokens are cut; tokens beyond max_blocks *
- * block_size, or without a block, get slot -1. info[1] counts the entries left without a block, by an empty list or by that rule.
+ * block_size, or without a block, get slot -1 and are neither cached nor seen; info[1] counts the entries left without a block, by
+ * an empty list or by that rule, but no tokens beyond the table, which the slots alone tell (rows in use whose slot is -1).
  * lens is not advanced (gq_paged_advance), so calling it again gives the same maps and takes no more blocks. */
 int32_t gq_paged_plan(gq_ctx* ctx, const gq_paged_cache* cache, gq_buf counts, gq_buf free_list, gq_buf free_count, const gq_paged_step* step);
 /* lens[b] += the step's rows of request b (at most max_blocks * block_size), with or without room: once per step, behind the last layer. */

@@ -46,6 +46,17 @@ def step_info(st):
     return int(st.info.numpy()[1])
 
 
+def test_every_row_without_room_is_counted():
+    """A step says how many of its rows found no place: beyond the table, where no block is wanted, as well as without a block."""
+    from grilly2_b200.infer.paged import PagedKvCache, PagedStep
+    cache = PagedKvCache(layers=1, kv_heads=1, head_dim=32, blocks=3, seqs=2, max_blocks=2, block_size=16)
+    step = PagedStep(cache, 50)
+    for counts, dropped, shortfall in (([16, 16], 0, 0), ([16, 16], 16, 1), ([1, 1], 2, 0), ([0, 0], 0, 0)):
+        cache.plan(dev(np.array(counts, np.int32)), step)
+        assert (step.dropped(), step.shortfall()) == (dropped, shortfall)
+        cache.advance(step)
+
+
 # ── contributions far apart ────────────────────────────────────────────────
 
 
