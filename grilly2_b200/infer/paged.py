@@ -39,8 +39,11 @@ def _held(buffers, name, dtype, size, make):
     return t
 
 
-def _zeros(n, dtype="int32"):
-    return _C.Tensor.from_numpy(np.zeros(n, dtype=np.int32 if dtype == "int32" else np.float32), persistent=True)
+def _filled(shape, dtype="int32", word=0):
+    """A tensor of one 32-bit word, written on the device: a pool may be larger than the host's memory."""
+    t = _C.Tensor.empty(shape, dtype, persistent=True)
+    check(_lib.load().gq_fill(_C.context(), t.storage.handle, 0, 4 * t.numel(), word))
+    return t
 
 
 def _operand(t, dtype, what, size=None):
@@ -75,11 +78,11 @@ class PagedKvCache:
         words = scales * self.block_size * self.head_dim // 4
         sizes = {"k": words, "v": words, "kscale": scales, "vscale": scales, "table": self.seqs * self.max_blocks, "lens": self.seqs,
                  "free": self.blocks, "free_count": 1}
-        make = {"table": lambda: _C.Tensor.from_numpy(np.full((self.seqs, self.max_blocks), -1, dtype=np.int32), persistent=True),
+        make = {"table": lambda: _filled((self.seqs, self.max_blocks), word=0xFFFFFFFF),
                 "free": lambda: _C.Tensor.from_numpy(np.arange(self.blocks, dtype=np.int32)[::-1].copy(), persistent=True),
                 "free_count": lambda: _C.Tensor.from_numpy(np.array([self.blocks], dtype=np.int32), persistent=True)}
         for name, dtype in _BUFFERS.items():
-            setattr(self, name, _held(given, name, dtype, sizes[name], make.get(name, lambda n=sizes[name], d=dtype: _zeros(n, d))))
+            setattr(self, name, _held(given, name, dtype, sizes[name], make.get(name, lambda n=sizes[name], d=dtype: _filled((n,), d))))
         if given:
             raise RuntimeError(f"a paged cache has no buffers {sorted(given)}")
         self._desc = _lib.PagedCache(layers=self.layers, blocks=self.blocks, block_size=self.block_size, kv_heads=self.kv_heads, dim=self.head_dim,
@@ -153,7 +156,7 @@ class PagedStep:
         runs = min(self.max_tokens, self.max_tokens // cache.block_size + 2 * cache.seqs)
         sizes = {"starts": cache.seqs + 1, "slots": self.max_tokens, "positions": self.max_tokens, "runs": runs + 1, "last": cache.seqs, "info": 2}
         for name, n in sizes.items():
-            setattr(self, name, _held(given, name, "int32", n, lambda n=n: _zeros(n)))
+            setattr(self, name, _held(given, name, "int32", n, lambda n=n: _filled((n,))))
         if given:
             raise RuntimeError(f"a step has no buffers {sorted(given)}")
         self._desc = _lib.PagedStep(max_tokens=self.max_tokens, **{n: getattr(self, n).storage.handle for n in sizes})

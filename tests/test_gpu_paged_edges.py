@@ -57,6 +57,23 @@ def test_every_row_without_room_is_counted():
         cache.advance(step)
 
 
+def test_a_new_cache_is_made_on_the_device(monkeypatch):
+    """Nothing of the size of the pool or the tables passes through the host's memory; the pool is zeros, the table empty."""
+    from grilly2_b200 import _C
+    from grilly2_b200.infer.paged import PagedKvCache, PagedStep
+    sent, upload = [], _C.Tensor.from_numpy
+    monkeypatch.setattr(_C.Tensor, "from_numpy", staticmethod(lambda a, persistent=False: (sent.append(np.asarray(a).size), upload(a, persistent))[1]))
+    rubbish = [_C.Tensor.from_numpy(np.full(n, 77, np.int32)) for n in (1 << 18, 1 << 12, 1 << 12)]
+    del rubbish, sent[:]
+    cache = PagedKvCache(layers=4, kv_heads=2, head_dim=64, blocks=128, seqs=8, max_blocks=200, block_size=16)
+    step = PagedStep(cache, 500)
+    assert max(sent) <= 128
+    for t in (cache.k, cache.v, cache.kscale, cache.vscale, cache.lens, step.slots, step.runs):
+        assert not t.numpy().any()
+    assert (cache.table.numpy() == -1).all() and cache.table.shape == (8, 200) and cache.free_blocks() == 128
+    np.testing.assert_array_equal(np.sort(cache.free.numpy()), np.arange(128))
+
+
 # ── contributions far apart ────────────────────────────────────────────────
 
 
