@@ -171,6 +171,9 @@ int32_t gq_paged_attn(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer, 
         check_dims(op, max_count, 1);
         if (max_count == 0) fail("%s: max_count must be at least 1", op);
         check_dims(op, st.tokens * heads, 1);
+        // a row tile's units (key tiles and two more, over all KV heads) are numbered in 32 bits
+        if (c.kv_heads * (((uint64_t)c.max_blocks << c.shift) / 128 + 3) > 0xffffffffull)
+            fail("%s: %u KV heads over requests of up to %llu tokens: more than 2^32 tiles of 128 keys", op, c.kv_heads, (ull)c.max_blocks << c.shift);
         auto qp = (const float*)view(ctx, q, 0, st.tokens * width, 4, "gq_paged_attn q");
         auto yp = (float*)view(ctx, out, 0, st.tokens * width, 4, "gq_paged_attn output");
         check_aligned(op, {qp, yp});

@@ -454,7 +454,8 @@ int32_t gq_paged_append(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer
  * the usual case 2^-28, of the largest such product among the 128 positions (from a multiple of 128 on) that its key lies in, and of
  * 2^-60 of the row's: a key that a neighbour outweighs by more reads as none. q and out float32 [max_tokens][heads dim], not overlapping; rows behind
  * starts[seqs] are left as they were. max_count is the largest counts[b] the caller expects (1 for a decode step): it chooses
- * how the work is cut, never what is computed (beyond the order of float32 sums). Uses the context's scratch, which grows on
+ * how the work is cut, never what is computed (beyond the order of float32 sums). kv_heads (max_blocks block_size / 128 + 3) must stay
+ * below 2^32. Uses the context's scratch, which grows on
  * first use: one eager call with this dim before a capture. */
 int32_t gq_paged_attn(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer, gq_buf q, uint64_t heads, float scale, const gq_paged_step* step,
                       uint64_t max_count, gq_buf out);

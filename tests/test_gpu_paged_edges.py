@@ -243,3 +243,17 @@ def test_buffers_that_a_call_writes_lie_apart():
         cache.attend(0, q, 4, step, out=_C.Tensor(cache.k.storage, (4, 128), "float32"))
     one.attend(0, q, 4, step)  # what is only read may be named twice
     cache.plan(counts, step)
+
+
+def test_more_tiles_than_their_numbers_hold_are_refused():
+    from grilly2_b200.infer.paged import PagedKvCache, PagedStep
+    for entries, refused in ((1 << 20, True), ((1 << 20) - 4, False)):
+        cache = PagedKvCache(layers=1, kv_heads=4096, head_dim=32, blocks=1, seqs=1, max_blocks=entries, block_size=128)
+        step = PagedStep(cache, 1)
+        cache.plan(dev(np.ones(1, np.int32)), step)
+        q = dev(np.zeros((1, 4096 * 32), np.float32))
+        if refused:
+            with pytest.raises(RuntimeError, match="2\\^32 tiles"):
+                cache.attend(0, q, 4096, step)
+        else:
+            cache.attend(0, q, 4096, step)
