@@ -124,6 +124,8 @@ def generate_batch(model, prompts, generation_config: GenerationConfig | None = 
     n = len(rows)
     if n == 0 or any(r.size == 0 or not np.issubdtype(r.dtype, np.integer) for r in rows):
         raise ValueError("`prompts` must be non-empty sequences of integer token ids")
+    if any(int(r.max()) > 0x7FFFFFFF or int(r.min()) < -0x80000000 for r in rows):
+        raise ValueError("`prompts` holds a token id that 32 bits do not hold")
     config = replace(generation_config or GenerationConfig())
     unused = [k for k in kwargs if k not in _FIELDS]
     if unused:
