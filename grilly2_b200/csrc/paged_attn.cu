@@ -10,9 +10,9 @@
 //   q_r = max|q_r| / (127 * 2^16) Q, Q in three signed digits (which hold 127 * 2^16); kscale_j is a factor of a lane;
 //   w vscale = 2^-31 P, P in four unsigned digits. The value scales are folded into P because the sum over j runs across blocks:
 //     so that P fits, the reference of a row's P is one of its contributions' s + log2 vscale (not of the scores). It follows the
-//     tiles of 128 keys: up where a tile's largest contribution passes it, down where that lies 2^10 below it, so that what
-//     an attention sink outweighs keeps its digits: a weight is off by 2^-32 of a reference that lies 2^11 above its own tile's
-//     largest at most, 2^4 in the usual case. (Three digits and one reference per row lost what lay 2^-24 below the row's largest: 1e-4 of
+//     tiles of 128 keys: up where a tile's largest contribution passes it, down where that lies 2^15 below it, so that what
+//     an attention sink outweighs keeps its digits: a weight is off by 2^-32 of a reference that lies 2^15 above its own tile's
+//     largest at most. (Three digits and one reference per row lost what lay 2^-24 below the row's largest: 1e-4 of
 //     the row where a key of no value stood 10 nats above 4095 others, 2e-2 at 17 nats; now 4e-7 and 2e-5. They took 632 us
 //     for the chunks below and 77 for the prompts.) The denominator sums the w themselves in float32, in P's reference.
 // As long as no row of a warpgroup moves its reference D goes on adding up in int32, and is read, joined and added to the float32
@@ -55,8 +55,10 @@ constexpr float kNone = -INFINITY;
 constexpr uint32_t kMostPerSm = 4;  // CTAs of an SM
 constexpr float kUnit = 2147483648.0f;  // 2^31: P's steps of the reference; P passes it by a factor of 2 at most and so has 32 bits
 // (all log2) how far above a tile's largest contribution its reference is laid where the quarters' largest lie within kEven of each
-// other, and how far below the reference a later tile's may fall before that follows
-constexpr float kRoom = 4.0f, kEven = 8.0f, kDrop = 6.0f;
+// other, and how far that of a later tile may fall below the reference before this follows. Each move reads D out, a quarter of a
+// tile's time (4, 8, 6: chunks 652 us, prompts 82.3; 5, 10, 6: 649, 81.6; these: 645, 80.6; if nothing ever moved: 627, 77); 16
+// of P's 32 bits and a sum over a tile's keys remain where the two lie farthest apart.
+constexpr float kRoom = 5.0f, kEven = 10.0f, kDrop = 9.0f;
 constexpr float kQMost = 127.0f * 65536.0f;
 
 template <int RP, int WG, int DIM>
@@ -280,14 +282,20 @@ __global__ void __launch_bounds__((Split<RP, WG, DIM>::kThreads), (Split<RP, WG,
         *failed = 0;
         mbar_fence_init();
     }
+    __syncthreads();
     // Before any tensor memory is taken: a kernel ahead that lets this one start before it has its own columns would wait for those
     // held here, and this one for its end. (Behind the barriers' set-up it costs 0.4 us less than as the first statement.)
     GQ_GRID_DEP_SYNC();
-    if (warp == 4 * WG) tmem_alloc(tmem_slot, 2 * T::kCols);
-    tc_fence_before_sync();
-    __syncthreads();
-    tc_fence_after_sync();
-    const uint32_t tmem = *tmem_slot;
+    if (warp == 4 * WG) {
+        tmem_alloc(tmem_slot, 2 * T::kCols);
+        tc_fence_before_sync();
+    }
+    uint32_t tmem = 0;
+    if (warp != 4 * WG + 1) {  // (the copying warp needs none and goes ahead)
+        named_barrier_sync(10, T::kSoft + 32);
+        tc_fence_after_sync();
+        tmem = *tmem_slot;
+    }
 
     bool ok = true;
 

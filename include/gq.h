@@ -450,9 +450,10 @@ int32_t gq_paged_append(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer
 /* Causal grouped-query attention of the step's rows over the cache: row t of request b, at position p = lens[b] + t -
  * starts[b], attends to positions 0 .. p. out[t] = softmax(scale q k^T) v. Positions whose block is missing are
  * skipped; a row that is left with none gives zeros. A row that sees a block whose scales are negative, no number or
- * beyond 2^90 (for values) is NaN. Beside float32 roundings, a weight times its block's value scale is off by at most 2^-21, in
- * the usual case 2^-28, of the largest such product among the 128 positions (from a multiple of 128 on) that its key lies in, and of
- * 2^-60 of the row's: a key that a neighbour outweighs by more reads as none. q and out float32 [max_tokens][heads dim], not overlapping; rows behind
+ * beyond 2^90 (for values) is NaN. Beside float32 roundings, a weight times its block's value scale is off by at most 2^-26 of the
+ * row's largest such product, and by at most 2^-17 of the largest among the 128 positions (from a multiple of 128 on) that its key
+ * lies in (2^-31 where that one towers over the row's others) and of 2^-60 of the row's: a key that a neighbour outweighs by
+ * 2^32 reads as none. q and out float32 [max_tokens][heads dim], not overlapping; rows behind
  * starts[seqs] are left as they were. max_count is the largest counts[b] the caller expects (1 for a decode step): it chooses
  * how the work is cut, never what is computed (beyond the order of float32 sums). kv_heads (max_blocks block_size / 128 + 3) must stay
  * below 2^32. Uses the context's scratch, which grows on

@@ -104,10 +104,10 @@ def attend(q, kcodes, vcodes, kscale, vscale, table, lens, steps, scale):
     log2 of a value scale too; its weight by as much, by 2^-21 for the exponential and by a rounding for each tile of 128 keys that a sum
     runs over. That bears on the weighted values and, through the denominator, on the row itself.
     Beside it the weights are whole numbers of a step: a contribution c = w vscale is off by half of one at most, and by no more
-    than itself. The step is 2^-31 of a power of two that lies at most 2^11 above the largest c of the tile; where that c towers over
-    all other tiles' (by more than 2^8) the power has just been set: at most 2^5 above it, or 2 where it towers over
-    a quarter of its own tile too. It never lies more than 2^60 below the row's largest (less where value scales are so small that
-    the weights' sum needs the room): what the step is then is the bound for all tiles."""
+    than itself. The step is 2^-31 of a power of two that lies at most 2^15 above the largest c of the tile and 2^6 above that of the row;
+    where a tile's towers over all others' (by more than 2^8) the power has just been set: at most 2^6 above it, or 2 where it
+    towers over a quarter of its own tile too. It never lies more than 2^60 below the row's largest (less where value scales are
+    so small that the weights' sum needs the room): what the step is then is the bound for all tiles."""
     rows, heads, dim = q.shape
     blocks, kvh, bs, _ = kcodes.shape
     out, tol = np.zeros(q.shape), np.zeros((rows, heads))
@@ -135,10 +135,10 @@ def attend(q, kcodes, vcodes, kscale, vscale, table, lens, steps, scale):
                 np.maximum.at(top, tile, c)
                 np.maximum.at(quarters, (tile, pos[ok] % 128 // 32), c)
                 most = np.argmax(top)
-                step = 2.0 ** 11 * top
+                step = np.minimum(2.0 ** 15 * top, 2.0 ** 6 * top[most])
                 if top[most] > 2.0 ** 8 * np.delete(top, most).max(initial=0.0):
-                    step[most] = top[most] * (2.0 if quarters[most].min() < 2.0 ** -8.1 * top[most] else 2.0 ** 5)
-                step = np.maximum(step, top[most] * 2.0 ** (5 - min(max(94 - logs, 0), 60)))
+                    step[most] = top[most] * (2.0 if quarters[most].min() < 2.0 ** -10.1 * top[most] else 2.0 ** 6)
+                step = np.maximum(step, top[most] * 2.0 ** (6 - min(max(94 - logs, 0), 60)))
                 codes = np.abs(vcodes[e, g, o].astype(np.float64)).max(1)
                 lost = (np.minimum(c, 2.0 ** -32 * step[tile]) * codes).sum()
                 off = ds + 2.0 ** -21 + (n // 128 + 1) * 2.0 ** -24
