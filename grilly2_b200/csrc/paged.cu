@@ -9,13 +9,13 @@
 // Both sums are block scans over the requests; runs and rows find their request by a binary search in shared memory. Few
 // rows run as one CTA; many as a cluster of eight, whose first CTA hands out the blocks while the cluster barrier holds
 // the others back from the table. Bound: latency (three scans); the maps are a few bytes per row. 8 requests with a token each
-// take 4.8 us, 1000 requests with 33 thousand rows 11.7 (a search for each of a thread's four rows, side by side: 13.4).
+// take 4.8 us, 1000 requests with 33 thousand rows 11.9 (a search for each of a thread's four rows, side by side: 13.4).
 //
 // append: one CTA per run of rows that share a block, KV head and K or V (further CTAs rotate q): the largest |value| of the
 // run gives the scale, the block's older codes are rounded again if it grew, the run's values are rounded and stored in
 // the core-matrix order of the pool. A 32-bit word of codes has one owner, so a word that holds old and new codes is
 // read and written by one thread. Bound: bytes where there are many rows (8 prompts of 5568 rows in all, 32 heads over 8 of 128:
-// 245 MB in 53.6 us = 4.6 TB/s; a chain of loads, a maximum over the CTA and stores for each run keeps it from the copy's 37),
+// 245 MB in 53.5 us = 4.6 TB/s; a chain of loads, a maximum over the CTA and stores for each run keeps it from the copy's 37),
 // launch latency for single tokens (64 requests: 5.9 us).
 #include "gq_internal.h"
 #include "paged.cuh"

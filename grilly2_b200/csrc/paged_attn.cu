@@ -13,8 +13,8 @@
 //     tiles of 128 keys: up where a tile's largest contribution passes it, down where that lies 2^15 below it, so that what
 //     an attention sink outweighs keeps its digits: a weight is off by 2^-32 of a reference that lies 2^15 above its own tile's
 //     largest at most. (Three digits and one reference per row lost what lay 2^-24 below the row's largest: 1e-4 of
-//     the row where a key of no value stood 10 nats above 4095 others, 2e-2 at 17 nats; now 4e-7 and 2e-5. They took 632 us
-//     for the chunks below and 77 for the prompts.) The denominator sums the w themselves in float32, in P's reference.
+//     the row where a key of no value stood 10 nats above 4095 others, 2e-2 at 17 nats; now 4e-7 and 2e-5. They took 633 us
+//     for the chunks below and 79.5 for the prompts.) The denominator sums the w themselves in float32, in P's reference.
 // As long as no row of a warpgroup moves its reference D goes on adding up in int32, and is read, joined and added to the float32
 // sums only when one does (or after 256 tiles, before a sum could leave 32 bits). References are whole numbers, so sums follow them exactly.
 // A warp's 32 keys share one block and so one scale (blocks of 32 and more): the maximum is taken over the joined integers
@@ -35,12 +35,12 @@
 //
 // Bound, and what was measured (B200):
 //   long contexts (32 requests of 2000 to 15000 tokens, 32 heads over 8 of 128): the codes' bytes, 442 MB in 80 us = 5.5 TB/s
-//   one request, a small batch (700 tokens, 11.5 us; 64 requests of up to 4095 tokens, 24 MB, 18.0 us): latency. The units' scan,
+//   one request, a small batch (700 tokens, 11.7 us; 64 requests of up to 4095 tokens, 24 MB, 17.8 us): latency. The units' scan,
 //     the first blocks, three dependent steps a tile and the joining of the parts through L2 are some 10 us
-//   chunks of prompts (2 requests, 2795 rows over 3000 cached tokens each, 32 heads of 128): 174 GFLOP in 652 us. Three int8
-//     products for S and four for D would take 184; the float32 work beside them is some 44 warp instructions per 32 scores, issued at 0.6 of
+//   chunks of prompts (2 requests, 2795 rows over 3000 cached tokens each, 32 heads of 128): 174 GFLOP in 644 us. Three int8
+//     products for S and four for D would take 184; the float32 work beside them is 42 warp instructions per 32 scores, issued at 0.61 of
 //     the schedulers' rate
-//   short prompts (300 to 1100 tokens, 14 heads over 2 of 64): 81 us, a good third of it items' beginnings and ends (2500 cycles for
+//   short prompts (300 to 1100 tokens, 14 heads over 2 of 64): 82 us, a good third of it items' beginnings and ends (2500 cycles for
 //     q's digits, 3000 for the last sums and the output, beside 3300 a tile)
 #include "gq_internal.h"
 #include "paged.cuh"
@@ -56,7 +56,7 @@ constexpr uint32_t kMostPerSm = 4;  // CTAs of an SM
 constexpr float kUnit = 2147483648.0f;  // 2^31: P's steps of the reference; P passes it by a factor of 2 at most and so has 32 bits
 // (all log2) how far above a tile's largest contribution its reference is laid where the quarters' largest lie within kEven of each
 // other, and how far that of a later tile may fall below the reference before this follows. Each move reads D out, a quarter of a
-// tile's time (4, 8, 6: chunks 652 us, prompts 82.3; 5, 10, 6: 649, 81.6; these: 645, 80.6; if nothing ever moved: 627, 77); 16
+// tile's time (4, 8, 6: chunks 652 us, prompts 82.3; 5, 10, 6: 649, 81.6; 5, 10, 10: 643.6, 80.3; if nothing ever moved: 627, 77); 16
 // of P's 32 bits and a sum over a tile's keys remain where the two lie farthest apart.
 constexpr float kRoom = 5.0f, kEven = 10.0f, kDrop = 9.0f;
 constexpr float kQMost = 127.0f * 65536.0f;
@@ -139,7 +139,9 @@ __device__ __forceinline__ float4 block_scale(float ks, float vs) {
     return make_float4(good ? ks : 1.0f, fmaxf(__log2f(vs), vs == 0.0f ? -60.0f : -100.0f) + 0.001f, vs * kUnit, good ? 0.0f : 1.0f);
 }
 
-// sum of floor((a i + b) / m) for i < n, by Euclid's steps on (a, m); the divisions in 32 bits where the numbers allow (a
+// sum of floor((a i + b) / m) for i < n, by Euclid's steps on (a, m): whole multiples of m are taken out of a and b, and what is left
+// counts the lattice points under a line, which the transposed line counts with a and m exchanged (Graham, Knuth and Patashnik,
+// Concrete Mathematics, section 3.5). The divisions in 32 bits where the numbers allow (a
 // 64-bit one is a hundred instructions, and a range's start takes some twenty)
 template <class U>
 __device__ uint64_t floor_sum_in(U n, U m, U a, U b) {

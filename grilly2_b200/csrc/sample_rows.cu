@@ -15,8 +15,8 @@
 // A bin of more tokens than the list holds (ties, a flat row) falls back to bisecting the float's bits with a pass over the
 // row per step.
 //
-// Bound: latency and instruction issue, not memory: one row of 151936 (0.6 MB) takes 13.2 us, 64 rows (39 MB, 5.9 us at the rate
-// of a copy) 73, 200 rows of 32003 (26 MB, 3.9 us) 40. 15 us of the 73 go into reading the rows into shared memory, 30 into
+// Bound: latency and instruction issue, not memory: one row of 151936 (0.6 MB) takes 13.4 us, 64 rows (39 MB, 5.9 us at the rate
+// of a copy) 73, 200 rows of 32003 (26 MB, 3.9 us) 40.5. 15 us of the 73 go into reading the rows into shared memory, 30 into
 // the masses' histogram (a float64 exponential a token, 33 instructions, and an atomic addition), 18 into listing and ranking
 // its crossing bin, 10 into the draw; 64 rows of eight CTAs run as two waves, since 39 MB do not fit the SMs at once.
 #include <cooperative_groups.h>
