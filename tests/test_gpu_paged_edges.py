@@ -170,6 +170,40 @@ def test_batches_of_many_requests(seqs, kind):
     attend(t, [int(c) for c in counts], pad=1, max_count=int(counts.max()))
 
 
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_attention_right_behind_an_int4_linear(dim):
+    """Both hold tensor memory, and the linear lets the next launch start before it has its own: eager and captured runs of
+    the two one behind the other end and give what each gives alone."""
+    from grilly2_b200 import _C, _lib
+    rng = np.random.default_rng(61)
+    w = _C.Int4Weight.quantize(_C.Tensor.from_numpy((rng.standard_normal((148 * 128, 512)) * 0.02).astype(np.float32)), 128)
+    x = _C.Tensor.from_numpy(rng.standard_normal((8, 512)).astype(np.float32))
+    t = filled(rng, 8, 2, dim, 32, [500, 40, 1000], [1, 1, 1])
+    st = t.Step(t.cache, 3)
+    t.cache.plan(dev(np.ones(3, np.int32)), st)
+    q, out = dev(rng.standard_normal((3, 8 * dim)).astype(np.float32)), _C_filled((3, 8 * dim), 0.0)
+    for kernel in (_lib.KERNEL_UMMA_LANES, _lib.KERNEL_UMMA):
+        y_alone = w.linear(x, None, kernel).numpy()
+        alone = t.cache.attend(0, q, 8, st, max_count=1, out=out).numpy()
+        for _ in range(20):
+            y = w.linear(x, None, kernel)
+            t.cache.attend(0, q, 8, st, max_count=1, out=out)
+            again = w.linear(x, None, kernel)
+        for got in (y, again):
+            np.testing.assert_array_equal(got.numpy(), y_alone)
+        np.testing.assert_array_equal(out.numpy(), alone)
+        _C.begin_capture()
+        for _ in range(4):
+            y = w.linear(x, None, kernel)
+            t.cache.attend(0, q, 8, st, max_count=1, out=out)
+        graph = _C.end_capture()
+        for _ in range(10):
+            graph.replay()
+        np.testing.assert_array_equal(out.numpy(), alone)
+        np.testing.assert_array_equal(y.numpy(), y_alone)
+        del graph
+
+
 @pytest.mark.parametrize("dim,block", [(32, 128), (64, 128)])
 def test_a_range_of_more_tiles_than_the_integer_sums_may_hold(dim, block):
     """Tables that name a few blocks over and over: every CTA has some 700 tiles of one request, all of equal scores, codes of
