@@ -451,13 +451,12 @@ int32_t gq_paged_append(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer
  * starts[b], attends to positions 0 .. p. out[t] = softmax(scale q k^T) v. Positions whose block is missing are
  * skipped; a row that is left with none gives zeros. A row that sees a block whose scales are negative, no number or
  * beyond 2^90 (for values) is NaN. Beside float32 roundings, a weight times its block's value scale is off by at most 2^-26 of the
- * row's largest such product, and by at most 2^-17 of the largest among the 128 positions (from a multiple of 128 on) that its key
- * lies in (2^-31 where that one towers over the row's others) and of 2^-60 of the row's: a key that a neighbour outweighs by
- * 2^32 reads as none. q and out float32 [max_tokens][heads dim], not overlapping; rows behind
- * starts[seqs] are left as they were. max_count is the largest counts[b] the caller expects (1 for a decode step): it chooses
- * how the work is cut, never what is computed (beyond the order of float32 sums). kv_heads (max_blocks block_size / 128 + 3) must stay
- * below 2^32. Uses the context's scratch, which grows on
- * first use: one eager call with this dim before a capture. */
+ * row's largest such product, and by no more than 2^-17 of the largest among the 128 positions (from a multiple of 128 on) that
+ * its key lies in (2^-31 where that one towers over the row's others), or than 2^-60 of the row's where that is more: a key that a
+ * neighbour outweighs by 2^32 reads as none. q and out float32 [max_tokens][heads dim], not overlapping; rows behind starts[seqs]
+ * are left as they were. max_count is the largest counts[b] the caller expects (1 for a decode step): it chooses how the work is
+ * cut, never what is computed (beyond the order of float32 sums). kv_heads (max_blocks block_size / 128 + 3) must stay below 2^32.
+ * Uses the context's scratch, which grows on first use: one eager call with this dim before a capture. */
 int32_t gq_paged_attn(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer, gq_buf q, uint64_t heads, float scale, const gq_paged_step* step,
                       uint64_t max_count, gq_buf out);
 /* The next token of every row, each row with settings of its own (float32 or int32 [rows], on the device, so that a captured
@@ -467,9 +466,10 @@ int32_t gq_paged_attn(gq_ctx* ctx, const gq_paged_cache* cache, uint64_t layer, 
  *   min_p   (<= 0: off) keeps w >= min_p;
  * the largest always stays. The draw is the inverse CDF in token order with u in [0, 1): the first kept token whose cumulative
  * weight exceeds u * total. u is uniforms[*draws % uniform_rows][row] (uniform_rows x rows floats), and the uint32 word
- * `draws` is advanced by one, so that a captured step takes the next numbers at each replay; draws == 0: the first row. temperature <= 0 takes the first largest. tokens: int32 per row, -1
- * where every logit is -inf; probs (0 = none) receives the token's share of what was kept; neither may overlap the inputs. Weights and the draw's sums are
- * float64; the masses that top_p compares are sums of whole multiples of 2^-40 of the largest weight; tokens below exp(-64) of it are never drawn. vocab at most 2^23.
+ * `draws` is advanced by one, so that a captured step takes the next numbers at each replay; draws == 0: the first row; no rows: it
+ * stays. temperature <= 0 takes the first largest. tokens: int32 per row, -1 where every logit is -inf; probs (0 = none) receives
+ * the token's share of what was kept; neither may overlap the inputs. Weights and the draw's sums are float64; the masses that top_p
+ * compares are sums of whole multiples of 2^-40 of the largest weight; tokens below exp(-64) of it are never drawn. vocab at most 2^23.
  * Replaces nothing of the reference: its sampler has one setting for all rows and no min_p (gq_sample). */
 int32_t gq_sample_rows(gq_ctx* ctx, gq_buf logits, uint64_t l_off, uint64_t rows, uint64_t vocab, gq_buf temperature, gq_buf top_k, gq_buf top_p,
                        gq_buf min_p, gq_buf uniforms, uint64_t uniform_rows, gq_buf draws, gq_buf tokens, gq_buf probs);
