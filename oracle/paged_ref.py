@@ -1,4 +1,4 @@
-"""Checker of the paged int8 KV cache and of sampling by rows: numpy, request by request, attention and sampling in
+"""Oracle of the paged int8 KV cache and of sampling by rows: numpy, request by request, attention and sampling in
 float64, the stored codes in the float32 steps that include/gq.h states."""
 import numpy as np
 

@@ -1,4 +1,4 @@
-"""The paged int8 cache where it could go wrong beside the cases of test_gpu_paged.py, whose twin of device and checker this uses:
+"""The paged int8 cache where it could go wrong beside the cases of test_gpu_paged.py, whose twin of device and oracle this uses:
 pools that run out and are filled again, contributions far apart, batches of many requests, sums near the ends of their range."""
 import numpy as np
 import pytest
@@ -107,7 +107,7 @@ def with_sink(keys, gap, at, value, dim=64, bs=64):
 @pytest.mark.parametrize("gap", [10.0, 14.0, 17.0, 40.0])
 @pytest.mark.parametrize("keys,at", [(200, 5), (4096, 0), (4096, 3000), (15000, 0), (15000, 14990)])
 def test_one_key_far_above_the_others(keys, at, gap, value):
-    """The allowance is the checker's: what a weight's whole steps lose is bounded tile by tile, so the row's other keys
+    """The allowance is the oracle's: what a weight's whole steps lose is bounded tile by tile, so the row's other keys
     keep their digits outside the lone key's own tile, and inside it down to 2^-31 of it."""
     t, st, want, q, scale = with_sink(keys, gap, at, value)
     exact, tol = t.ref.attend(q, t.codes["k"], t.codes["v"], t.scales["k"], t.scales["v"], t.table, t.lens, want, scale)
@@ -207,7 +207,7 @@ def test_attention_right_behind_an_int4_linear(dim):
 @pytest.mark.parametrize("dim,block", [(32, 128), (64, 128)])
 def test_a_range_of_more_tiles_than_the_integer_sums_may_hold(dim, block):
     """Tables that name a few blocks over and over: every CTA has some 700 tiles of one request, all of equal scores, codes of
-    127. Value scales of 0.99 and of just under 32 times that: a reference that a tile of small ones laid is not moved by the large ones,
+    127. Value scales of 0.99 and of just under 64 times that: a reference that a tile of small ones laid is not moved by the large ones,
     whose weights then fill their 32 bits, and the sums are read out only because they would leave 32 bits. The mean of the
     values is known exactly."""
     from grilly2_b200.infer.paged import PagedKvCache, PagedStep
@@ -216,7 +216,7 @@ def test_a_range_of_more_tiles_than_the_integer_sums_may_hold(dim, block):
     table = rng.integers(0, blocks, (seqs, entries)).astype(np.int32)
     last = entries * block - 1  # the last position of the table
     codes = np.full((blocks, 1, block, dim), 127, np.int8)
-    vscale = np.where(np.arange(blocks) % 8, 31.4, 0.99).astype(np.float32)[:, None]
+    vscale = np.where(np.arange(blocks) % 8, 62.5, 0.99).astype(np.float32)[:, None]
     cache = PagedKvCache(layers=1, kv_heads=1, head_dim=dim, blocks=blocks, seqs=seqs, max_blocks=entries, block_size=block,
                          buffers={"k": words(codes), "v": words(codes), "kscale": dev(np.ones((blocks, 1), np.float32)), "vscale": dev(vscale),
                                   "table": dev(table), "lens": dev(np.full(seqs, last, np.int32)), "free_count": dev(np.zeros(1, np.int32))})

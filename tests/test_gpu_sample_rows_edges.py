@@ -1,4 +1,4 @@
-"""Sampling with settings of each row where the kept tokens' weights lie far apart, against the float64 checker."""
+"""Sampling with settings of each row where the kept tokens' weights lie far apart, against the float64 oracle."""
 import numpy as np
 import pytest
 
